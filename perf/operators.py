@@ -26,12 +26,12 @@ own = False
 DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
 
 
-def _lm():
+def _package():
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorch-xdna2_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
-    from xdna_train import lm
-    return lm
+    import xdna_train
+    return xdna_train
 
 
 def listed():
@@ -161,23 +161,32 @@ def run(s):
 
 
 def _own(s):
-    lm, case = _lm(), s["case"]
+    xdna_train, case = _package(), s["case"]
+    lm = xdna_train.lm
+
+    def on(*names):  # the tensors on the package's device (the same memory), as leaves where a gradient is wanted
+        return [None if s[k] is None else xdna_train.as_xdna(s[k].detach()).requires_grad_(s[k].requires_grad)
+                for k in names]
+
     if case["op"] == "embedding":
-        y = lm.embedding(s["ids"], s["weight"], scale=s["scale"], padding_idx=s["padding_idx"])
+        ids, w = on("ids", "weight")
+        y = lm.embedding(ids, w, scale=s["scale"], padding_idx=s["padding_idx"])
         if not case["train"]:
             return {"y": y}
-        (dw,) = torch.autograd.grad(y, [s["weight"]], s["dy"])
+        (dw,) = torch.autograd.grad(y, [w], on("dy")[0])
         return {"y": y.detach(), "dw": dw}
     if case["op"] == "gated_mlp":
-        y = lm.gated_mlp(s["x"], s["w_gate"], s["w_up"], s["w_down"], activation=s["act"])
+        leaves = on("x", "w_gate", "w_up", "w_down")
+        y = lm.gated_mlp(*leaves, activation=s["act"])
         if not case["train"]:
             return {"y": y}
-        dx, dg, du, dd = torch.autograd.grad(y, [s["x"], s["w_gate"], s["w_up"], s["w_down"]], s["dy"])
+        dx, dg, du, dd = torch.autograd.grad(y, leaves, on("dy")[0])
         return {"y": y.detach(), "dx": dx, "dw_gate": dg, "dw_up": du, "dw_down": dd}
+    z, t, ids, w = on("logits", "teacher", "ids", "weight")
     if not case["train"]:
-        return {"loss": lm.distill_loss(s["logits"], s["teacher"], s["ids"], temperature=s["tau"], reduction="none")}
-    loss = lm.distill_loss(s["logits"], s["teacher"], s["ids"], temperature=s["tau"], row_weight=s["weight"])
-    (dz,) = torch.autograd.grad(loss, [s["logits"]])
+        return {"loss": lm.distill_loss(z, t, ids, temperature=s["tau"], reduction="none")}
+    loss = lm.distill_loss(z, t, ids, temperature=s["tau"], row_weight=w)
+    (dz,) = torch.autograd.grad(loss, [z])
     return {"loss": loss.detach(), "dlogits": dz}
 
 
