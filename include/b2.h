@@ -49,7 +49,7 @@ enum {
 };
 
 /* dtype codes used where a pointer can hold more than one element type */
-enum { B2_BF16 = 0, B2_F32 = 1 };
+enum { B2_BF16 = 0, B2_F32 = 1, B2_I32 = 2, B2_I64 = 3 };
 
 /* ---- runtime ------------------------------------------------------------ */
 
@@ -645,6 +645,67 @@ b2_status b2_region_bn_bwd_bf16(const void* dy, const void* y, const void* x,
                                 void* db, int64_t N, int64_t C, int64_t HW,
                                 float slope, int relu, void* workspace,
                                 size_t workspace_bytes, void* stream);
+
+/* ---- language-model operators (no counterpart in the reference) --------- */
+
+/* Scaled embedding lookup: y[t][:] = scale * weight[ids[t]][:] for T tokens.
+ * weight [V][D] with row stride ldw >= D (elements), dtype B2_BF16 or B2_F32;
+ * ids_dtype B2_I32 or B2_I64; y dense [T][D] of the weight's dtype, computed
+ * in fp32 and rounded once.  An id outside [0, V) gives a row of NaN and
+ * B2_ERR_INVALID in the device status word.  T, V, D below 2^31 - 1. */
+b2_status b2_embedding_fwd(const void* ids, int ids_dtype, int64_t T,
+                           const void* weight, int64_t ldw, int dtype,
+                           int64_t V, int64_t D, float scale, void* y,
+                           void* stream);
+/* Its gradient: dw[v][:] = scale * sum over the tokens with ids[t] == v of
+ * dy[t][:], dense [V][D] (every row is written, zero where no token has it and
+ * for padding_idx; -1: none; ids outside [0, V) add to no row).  dy has row
+ * stride lddy >= D.  fp32 sums in a fixed order over tokens sorted by id
+ * (bit-reproducible), rounded once.  Workspace: at least
+ * b2_embedding_bwd_workspace_bytes(T, V, D) bytes, 16-byte aligned. */
+size_t b2_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D);
+b2_status b2_embedding_bwd(const void* ids, int ids_dtype, int64_t T,
+                           const void* dy, int64_t lddy, int dtype, int64_t V,
+                           int64_t D, float scale, int64_t padding_idx,
+                           void* dw, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Distillation loss of N rows of V student logits z against the K top logits
+ * t of a teacher at vocabulary ids `ids` (a negative id: entry absent).  With
+ * p = softmax(t / temperature) over a row's present entries and q = softmax(z /
+ * temperature) over the vocabulary, row r's loss is
+ *   temperature^2 * sum_k p_k (log p_k - log q[ids_k])   (p_k = 0 adds 0)
+ * times row_weight[r] (fp32 [N], NULL: 1); a row without entries, or with
+ * weight 0, has loss and gradient 0.  reduction 0: the sum over the sum of the
+ * weights (0 if that is 0), 1: the sum, 2: none (loss is [N], else a scalar).
+ * z: dtype B2_BF16 / B2_F32, row stride ldz >= V; t: t_dtype, row stride ldt;
+ * ids: ids_dtype B2_I32 / B2_I64, row stride ldi; K <= 1024.  All statistics in
+ * fp32.  An id >= V makes its row's loss and gradient NaN and sets
+ * B2_ERR_INVALID in the device status word.  stats: fp32 [2N + 1], what the
+ * backward needs.  dz (may be NULL; the logits' dtype, row stride lddz >= V)
+ * gets the gradient for an upstream gradient of 1, in the same pass over the
+ * logits.  Workspace: b2_distill_workspace_bytes(N), 16-byte aligned. */
+size_t b2_distill_workspace_bytes(int64_t N);
+b2_status b2_distill_loss_fwd(const void* z, int64_t ldz, int dtype, int64_t N,
+                              int64_t V, const void* t, int64_t ldt,
+                              int t_dtype, const void* ids, int64_t ldi,
+                              int ids_dtype, int64_t K, float temperature,
+                              const float* row_weight, int reduction,
+                              float* loss, float* stats, void* dz,
+                              int64_t lddz, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* The gradient for any upstream gradient (fp32 device scalar, [N] for
+ * reduction 2), from the same arguments and the forward's stats.  With
+ * skip_ones != 0, rows whose upstream gradient is exactly 1 are left as they
+ * are (dz came from the forward). */
+b2_status b2_distill_loss_bwd(const void* z, int64_t ldz, int dtype, int64_t N,
+                              int64_t V, const void* t, int64_t ldt,
+                              int t_dtype, const void* ids, int64_t ldi,
+                              int ids_dtype, int64_t K, float temperature,
+                              const float* row_weight, int reduction,
+                              const float* stats, const float* upstream,
+                              int skip_ones, void* dz, int64_t lddz,
+                              void* stream);
 
 #ifdef __cplusplus
 }

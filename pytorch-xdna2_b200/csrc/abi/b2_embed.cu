@@ -1,0 +1,724 @@
+// Token embedding: scaled row lookup and its dense weight gradient.
+//
+//   forward   y[t][:]  = scale * W[id_t][:]
+//   backward  dW[v][:] = scale * sum over the tokens t with id_t == v, in token
+//             order, of dy[t][:]; rows without a token (and the padding row)
+//             are zero
+//
+// Both are bound by HBM: the lookup moves T*D elements in and out, the
+// gradient reads T*D elements of dy and writes all V*D of dW.
+//
+// The backward sorts the tokens by id (a stable least-significant-digit radix
+// sort of (id, token) pairs, written here), so that a row's tokens are
+// neighbours: every dy row is read once, every dW row is written once, the
+// sums are fp32 in a fixed order (bit-reproducible, no atomics on values) and
+// one frequent token spreads over many CTAs.  The sorted list is cut into
+// pieces of kPiece tokens whatever their ids; a run of equal ids inside one
+// piece is written directly, a run that crosses pieces leaves fp32 partial rows
+// that a last kernel adds in piece order.
+#include <algorithm>
+
+#include "b2_common.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kDigitBits = 9;  // widest digit; 512 counters per warp
+constexpr int kDigits = 1 << kDigitBits;
+constexpr int kPiece = 32;     // sorted tokens per accumulation piece
+constexpr int kAccThreads = 256;
+
+template <int BYTES>
+struct Vec;
+template <>
+struct Vec<16> { using type = uint4; };
+template <>
+struct Vec<8> { using type = uint2; };
+template <>
+struct Vec<4> { using type = uint32_t; };
+template <>
+struct Vec<2> { using type = uint16_t; };
+
+// N consecutive elements (T: uint16_t = bf16 bits, or float) <-> fp32
+template <typename T, int N>
+struct Pack {
+  using V = typename Vec<sizeof(T) * N>::type;
+  union {
+    V v;
+    T e[N];
+  };
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 2) return bf2f(e[i]);
+    else return e[i];
+  }
+  __device__ __forceinline__ void set(int i, float f) {
+    if constexpr (sizeof(T) == 2) {
+      __nv_bfloat16 h = __float2bfloat16_rn(f);
+      e[i] = *reinterpret_cast<uint16_t*>(&h);
+    } else {
+      e[i] = f;
+    }
+  }
+};
+
+__device__ __forceinline__ long long load_id(const void* ids, int is64, long long t) {
+  return is64 ? static_cast<const long long*>(ids)[t] : (long long)static_cast<const int*>(ids)[t];
+}
+
+// ---------------------------------------------------------------------------
+// forward: `lanes` threads (a power of two) walk one row, 256 / lanes rows per
+// CTA, U rows' loads in flight per thread.  An id outside [0, V) gives a row of
+// NaN and B2_ERR_INVALID in the device status word; nothing out of range is read.
+// ---------------------------------------------------------------------------
+template <typename T, int N, int U>
+__global__ void __launch_bounds__(256) embed_fwd_kernel(const void* __restrict__ ids, int is64, long long tokens,
+                                                        const T* __restrict__ w, long long ldw, long long V,
+                                                        int vecs, int log_lanes, float scale, T* __restrict__ y,
+                                                        long long D, int* status) {
+  const int lane = threadIdx.x & ((1 << log_lanes) - 1);
+  const int rows_per_pass = 256 >> log_lanes;
+  const long long t0 = (long long)blockIdx.x * rows_per_pass * U + (threadIdx.x >> log_lanes);
+  long long id[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long t = t0 + (long long)u * rows_per_pass;
+    id[u] = t < tokens ? load_id(ids, is64, t) : -1;
+    if (t < tokens && (id[u] < 0 || id[u] >= V)) {
+      id[u] = -1;
+      if (lane == 0 && blockIdx.y == 0) record_status(status, B2_ERR_INVALID);
+    }
+  }
+  for (int c = blockIdx.y * (1 << log_lanes) + lane; c < vecs; c += gridDim.y << log_lanes) {
+    Pack<T, N> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (id[u] >= 0) p[u].v = reinterpret_cast<const typename Pack<T, N>::V*>(w + id[u] * ldw)[c];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long t = t0 + (long long)u * rows_per_pass;
+      if (t >= tokens) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        p[u].set(i, id[u] >= 0 ? scale * p[u].get(i) : __int_as_float(0x7fc00000));
+      reinterpret_cast<typename Pack<T, N>::V*>(y + t * D)[c] = p[u].v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the sort
+// ---------------------------------------------------------------------------
+
+// Sort key of a token: its id, or V for a token that contributes to no row
+// (the padding id; an id out of range, reported by the forward).
+__device__ __forceinline__ uint32_t key_of(const void* ids, int is64, long long t, long long V, long long pad) {
+  const long long id = load_id(ids, is64, t);
+  return (id < 0 || id >= V || id == pad) ? uint32_t(V) : uint32_t(id);
+}
+
+// Shared memory of a sorting CTA: per warp one counter per digit, then the
+// digits' CTA-wide values.
+struct SortSmem {
+  uint32_t count[kSortWarps][kDigits];
+  uint32_t digit[kDigits];
+  uint32_t scan[kSortWarps];
+};
+
+// Exclusive prefix sum over 512 values held one per thread by threads 0..511
+// (all threads call).
+__device__ __forceinline__ uint32_t scan512(uint32_t v, uint32_t* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t n = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += n;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int i = 0; i < warp && i < 16; ++i) before += scratch[i];
+  return before + x - v;
+}
+
+// Stable ranks of this CTA's items by one digit.  Item i of a thread sits at
+// position warp * 32 * I + i * 32 + lane of the CTA's chunk.  On return rank[i]
+// is the item's place among the warp's equal digits and s.count[w][d] the
+// exclusive prefix over warps of digit d; the digit totals are in s.digit.
+template <int I>
+__device__ __forceinline__ void rank_items(SortSmem& s, const uint32_t (&key)[I], const bool (&valid)[I], int shift,
+                                           uint32_t mask, uint32_t (&rank)[I]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ndig = int(mask) + 1;
+  for (int d = lane; d < ndig; d += 32) s.count[warp][d] = 0;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const uint32_t d = (key[i] >> shift) & mask;
+    const uint32_t peers = __match_any_sync(0xffffffffu, valid[i] ? d : 0xffffffffu);
+    const uint32_t before = __popc(peers & ((1u << lane) - 1));
+    uint32_t base = 0;
+    if (valid[i]) base = s.count[warp][d];
+    __syncwarp();
+    rank[i] = base + before;
+    if (valid[i] && before == 0) s.count[warp][d] = base + __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < ndig; d += kSortThreads) {
+    uint32_t run = 0;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t c = s.count[w][d];
+      s.count[w][d] = run;
+      run += c;
+    }
+    s.digit[d] = run;
+  }
+  __syncthreads();
+}
+
+// Whole sort in one CTA (T <= 1024 * I): every pass goes through shared memory.
+template <int I>
+__global__ void __launch_bounds__(kSortThreads, 1)
+    embed_sort_one_kernel(const void* __restrict__ ids, int is64, int tokens, long long V, long long pad, int passes,
+                          int bits, uint32_t* __restrict__ key_out, uint32_t* __restrict__ tok_out) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
+  uint32_t* skey = reinterpret_cast<uint32_t*>(smem_raw + sizeof(SortSmem));
+  uint32_t* stok = skey + kSortThreads * I;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t key[I], tok[I], rank[I];
+  bool valid[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int pos = warp * 32 * I + i * 32 + lane;
+    valid[i] = pos < tokens;
+    tok[i] = uint32_t(pos);
+    key[i] = valid[i] ? key_of(ids, is64, pos, V, pad) : 0;
+  }
+  const uint32_t mask = (1u << bits) - 1;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    rank_items<I>(s, key, valid, shift, mask, rank);
+    const uint32_t total = threadIdx.x <= mask ? s.digit[threadIdx.x] : 0;
+    const uint32_t base = scan512(total, s.scan);
+    if (threadIdx.x <= mask) s.digit[threadIdx.x] = base;
+    __syncthreads();
+    const bool last = p + 1 == passes;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      if (!valid[i]) continue;
+      const uint32_t d = (key[i] >> shift) & mask;
+      const uint32_t pos = s.digit[d] + s.count[warp][d] + rank[i];
+      if (last) {
+        key_out[pos] = key[i];
+        tok_out[pos] = tok[i];
+      } else {
+        skey[pos] = key[i];
+        stok[pos] = tok[i];
+      }
+    }
+    if (last) break;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int pos = warp * 32 * I + i * 32 + lane;
+      if (valid[i]) {
+        key[i] = skey[pos];
+        tok[i] = stok[pos];
+      }
+    }
+  }
+}
+
+// Many CTAs, one launch per digit.  table[p][b][d]: tokens of chunk b with
+// digit d at the start of pass p.  This kernel fills pass 0's table and zeroes
+// the later ones; each pass adds up the next one's while it scatters.
+__global__ void __launch_bounds__(kSortThreads)
+    embed_hist_kernel(const void* __restrict__ ids, int is64, long long tokens, long long V, long long pad, int passes,
+                      int bits, int chunk, uint32_t* __restrict__ table) {
+  __shared__ uint32_t h[kDigits];
+  const uint32_t mask = (1u << bits) - 1;
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) h[d] = 0;
+  __syncthreads();
+  const long long t0 = (long long)blockIdx.x * chunk;
+  const long long t1 = min(tokens, t0 + chunk);
+  for (long long t = t0 + threadIdx.x; t < t1; t += kSortThreads)
+    atomicAdd(&h[key_of(ids, is64, t, V, pad) & mask], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
+    table[(long long)blockIdx.x * kDigits + d] = h[d];
+    for (int p = 1; p < passes; ++p) table[((long long)p * gridDim.x + blockIdx.x) * kDigits + d] = 0;
+  }
+}
+
+template <int I>
+__global__ void __launch_bounds__(kSortThreads)
+    embed_pass_kernel(const void* __restrict__ ids, int is64, long long tokens, long long V, long long pad, int pass,
+                      int passes, int bits, uint32_t* __restrict__ table, const uint32_t* __restrict__ key_in,
+                      const uint32_t* __restrict__ tok_in, uint32_t* __restrict__ key_out,
+                      uint32_t* __restrict__ tok_out) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int shift = pass * bits;
+  const uint32_t mask = (1u << bits) - 1;
+  constexpr int kChunk = kSortThreads * I;
+  uint32_t key[I], tok[I], rank[I];
+  bool valid[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const long long pos = (long long)blockIdx.x * kChunk + warp * 32 * I + i * 32 + lane;
+    valid[i] = pos < tokens;
+    key[i] = tok[i] = 0;
+    if (valid[i]) {
+      if (pass == 0) {
+        tok[i] = uint32_t(pos);
+        key[i] = key_of(ids, is64, pos, V, pad);
+      } else {
+        key[i] = key_in[pos];
+        tok[i] = tok_in[pos];
+      }
+    }
+  }
+  // this chunk's first place for every digit: smaller digits of all chunks,
+  // then the same digit in earlier chunks
+  const uint32_t* tab = table + (long long)pass * gridDim.x * kDigits;
+  uint32_t before = 0, total = 0;
+  if (threadIdx.x <= mask) {
+#pragma unroll 8
+    for (int b = 0; b < int(gridDim.x); ++b) {
+      const uint32_t c = tab[(long long)b * kDigits + threadIdx.x];
+      total += c;
+      if (b < int(blockIdx.x)) before += c;
+    }
+  }
+  rank_items<I>(s, key, valid, shift, mask, rank);
+  const uint32_t base = scan512(total, s.scan) + before;
+  if (threadIdx.x <= mask) s.digit[threadIdx.x] = base;
+  __syncthreads();
+  uint32_t* next = table + (long long)(pass + 1) * gridDim.x * kDigits;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    uint32_t pos = 0;
+    if (valid[i]) {
+      const uint32_t d = (key[i] >> shift) & mask;
+      pos = s.digit[d] + s.count[warp][d] + rank[i];
+      key_out[pos] = key[i];
+      tok_out[pos] = tok[i];
+    }
+    if (pass + 1 < passes) {
+      // one integer atomic per distinct (chunk, digit) of the warp
+      const uint32_t slot = valid[i] ? (pos / kChunk) * kDigits + ((key[i] >> (shift + bits)) & mask) : 0xffffffffu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, slot);
+      if (valid[i] && (peers & ((1u << lane) - 1)) == 0) atomicAdd(next + slot, uint32_t(__popc(peers)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// accumulation.  CTAs [0, acc_blocks) add the pieces' rows; the CTAs behind
+// them write zeros to the rows of dW that no token has.
+// ---------------------------------------------------------------------------
+
+// First position of the sorted keys with key >= want (all 256 threads call).
+__device__ __forceinline__ long long lower_bound(const uint32_t* __restrict__ key, long long n, uint32_t want) {
+  long long lo = 0;
+  while (n > 0) {
+    const long long step = (n + kAccThreads - 1) / kAccThreads;
+    const long long at = (long long)(threadIdx.x + 1) * step - 1;
+    const int below = __syncthreads_count(at < n && key[lo + at] < want);
+    lo += below * step;
+    // the answer lies in the first block whose last key is not below `want`
+    // (if it has a last key), without that key itself when it has been tested
+    n = min(step - 1, n - below * step);
+    if (n < 0) n = 0;
+  }
+  return lo;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* row, int c, const float (&acc)[N], float scale) {
+  Pack<T, N> p;
+#pragma unroll
+  for (int i = 0; i < N; ++i) p.set(i, scale * acc[i]);
+  reinterpret_cast<typename Pack<T, N>::V*>(row)[c] = p.v;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kAccThreads)
+    embed_acc_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ tok, long long tokens, long long V,
+                     const T* __restrict__ dy, long long lddy, int vecs, int log_lanes, long long D, float scale,
+                     T* __restrict__ dw, float* __restrict__ partial, long long pieces, int slabs,
+                     long long acc_blocks, int zero_rows) {
+  if ((long long)blockIdx.x >= acc_blocks) {
+    __shared__ uint8_t present[512];
+    const long long r0 = ((long long)blockIdx.x - acc_blocks) * zero_rows;
+    const int rows = int(min((long long)zero_rows, V - r0));
+    for (int i = threadIdx.x; i < rows; i += kAccThreads) present[i] = 0;
+    const long long lo = lower_bound(key, tokens, uint32_t(r0));
+    __syncthreads();
+    for (long long p = lo + threadIdx.x;; p += kAccThreads) {
+      const bool in = p < tokens && key[p] < uint32_t(r0 + rows);
+      if (in) present[key[p] - r0] = 1;
+      if (!__syncthreads_or(in)) break;
+    }
+    const int lane = threadIdx.x & ((1 << log_lanes) - 1);
+    for (int r = threadIdx.x >> log_lanes; r < rows; r += kAccThreads >> log_lanes) {
+      if (present[r]) continue;
+      auto* out = reinterpret_cast<typename Pack<T, N>::V*>(dw + (r0 + r) * D);
+      for (int c = lane; c < vecs; c += 1 << log_lanes) {
+        Pack<T, N> z;
+#pragma unroll
+        for (int i = 0; i < N; ++i) z.e[i] = T(0);
+        out[c] = z.v;
+      }
+    }
+    return;
+  }
+  const int per_block = kAccThreads >> log_lanes;
+  const int slab = int(blockIdx.x % slabs);
+  const long long piece = ((long long)blockIdx.x / slabs) * per_block + (threadIdx.x >> log_lanes);
+  const int c = (slab << log_lanes) + (threadIdx.x & ((1 << log_lanes) - 1));
+  if (piece >= pieces || c >= vecs) return;
+  const long long p0 = piece * kPiece, p1 = min(tokens, p0 + kPiece);
+  const uint32_t none = 0xffffffffu;
+  const uint32_t prev = p0 > 0 ? key[p0 - 1] : none;
+  const uint32_t next = p1 < tokens ? key[p1] : none;
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  uint32_t cur = key[p0];
+  bool begins = cur != prev;  // the current run starts in this piece
+  constexpr int U = 4;
+  for (long long p = p0; p < p1; p += U) {
+    uint32_t k[U];
+    Pack<T, N> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k[u] = p + u < p1 ? key[p + u] : none;
+      if (k[u] < V) v[u].v = reinterpret_cast<const typename Pack<T, N>::V*>(dy + (long long)tok[p + u] * lddy)[c];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k[u] == none) break;
+      if (k[u] != cur) {
+        // the run of `cur` ends here
+        if (begins)
+          store_row<T, N>(dw + (long long)cur * D, c, acc, scale);
+        else
+#pragma unroll
+          for (int i = 0; i < N; ++i) partial[(2 * piece) * D + (long long)c * N + i] = acc[i];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        cur = k[u];
+        begins = true;
+      }
+      if (k[u] >= V) return;  // only tokens without a row follow
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += v[u].get(i);
+    }
+  }
+  if (begins && cur != next) {
+    store_row<T, N>(dw + (long long)cur * D, c, acc, scale);
+  } else {
+    // slot 0: a run that came from the piece before; slot 1: one that starts here and goes on
+    float* out = partial + (2 * piece + (begins ? 1 : 0)) * D + (long long)c * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = acc[i];
+  }
+}
+
+// Adds the partial rows of every run that crosses pieces, in piece order.  The
+// CTA of the piece in which the run starts does it.
+template <typename T, int N>
+__global__ void __launch_bounds__(kAccThreads)
+    embed_join_kernel(const uint32_t* __restrict__ key, long long tokens, long long V, int vecs, long long D,
+                      float scale, T* __restrict__ dw, const float* __restrict__ partial, long long pieces) {
+  const long long piece = blockIdx.x;
+  const long long p0 = piece * kPiece, p1 = p0 + kPiece;
+  if (p1 >= tokens) return;  // the last piece's runs all end in it
+  const uint32_t k = key[p1 - 1];
+  if (k >= V || key[p1] != k) return;                                    // no run goes on
+  if (key[p0] == k && p0 > 0 && key[p0 - 1] == k) return;                // it started earlier
+  // the pieces after this one that start with k are its continuation
+  long long lo = piece + 1, hi = pieces;  // key[lo * kPiece] == k; find the first piece that does not start with k
+  while (lo + 1 < hi) {
+    const long long mid = (lo + hi) / 2;
+    if (key[mid * kPiece] == k) lo = mid;
+    else hi = mid;
+  }
+  const long long last = lo;
+  for (int c = blockIdx.y * kAccThreads + threadIdx.x; c < vecs; c += gridDim.y * kAccThreads) {
+    float acc[N];
+    const float* own_part = partial + (2 * piece + 1) * D + (long long)c * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = own_part[i];
+#pragma unroll 4
+    for (long long q = piece + 1; q <= last; ++q) {
+      const float* pp = partial + (2 * q) * D + (long long)c * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += pp[i];
+    }
+    store_row<T, N>(dw + (long long)k * D, c, acc, scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+// Widest vector (elements of `size` bytes, at most 16 bytes) that divides the
+// row length and strides and to which the pointers are aligned.
+int vec_elems(int size, int64_t D, int64_t ld, const void* a, const void* b) {
+  int n = 16 / size;
+  while (n > 1 && (D % n || ld % n || reinterpret_cast<uintptr_t>(a) % (size_t(n) * size) ||
+                   reinterpret_cast<uintptr_t>(b) % (size_t(n) * size)))
+    n /= 2;
+  return n;
+}
+
+int log_lanes_for(int vecs) {
+  int l = 0;
+  while (l < 8 && (1 << l) < vecs) ++l;
+  return l;
+}
+
+struct SortPlan {
+  int passes, bits;
+  bool one;      // whole sort in one CTA
+  int items;     // tokens per thread
+  int64_t blocks;
+};
+
+SortPlan sort_plan(int64_t T, int64_t V) {
+  SortPlan p{};
+  int bits = 1;
+  while (bits < 32 && (int64_t(1) << bits) <= V) ++bits;  // keys 0 .. V
+  p.passes = (bits + kDigitBits - 1) / kDigitBits;
+  p.bits = (bits + p.passes - 1) / p.passes;
+  p.one = T <= 8 * kSortThreads;
+  if (p.one) {
+    p.items = T <= kSortThreads ? 1 : T <= 2 * kSortThreads ? 2 : T <= 4 * kSortThreads ? 4 : 8;
+    p.blocks = 1;
+  } else {
+    p.items = T <= 128 * 2 * kSortThreads ? 2 : 8;
+    p.blocks = (T + int64_t(p.items) * kSortThreads - 1) / (int64_t(p.items) * kSortThreads);
+  }
+  return p;
+}
+
+struct EmbedWs {
+  size_t key0, tok0, key1, tok1, table, partial, total;
+};
+
+EmbedWs embed_ws(int64_t T, int64_t V, int64_t D) {
+  const SortPlan p = sort_plan(T, V);
+  EmbedWs w{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t r = at;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  w.key0 = take(size_t(T) * 4);
+  w.tok0 = take(size_t(T) * 4);
+  if (!p.one) {
+    w.key1 = take(size_t(T) * 4);
+    w.tok1 = take(size_t(T) * 4);
+    w.table = take(size_t(p.passes) * size_t(p.blocks) * kDigits * 4);
+  }
+  const int64_t pieces = (T + kPiece - 1) / kPiece;
+  w.partial = take(size_t(pieces) * 2 * size_t(D) * 4);
+  w.total = at;
+  return w;
+}
+
+// Once per kernel and device (`done`: a static of the caller).
+template <typename F>
+b2_status allow_smem(F kern, size_t bytes, bool (&done)[64]) {
+  int dev = 0;
+  B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  if (dev < 0 || dev >= 64) return set_error(B2_ERR_INVALID, "device index %d", dev);
+  if (done[dev]) return B2_OK;
+  B2_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
+                    "cudaFuncSetAttribute(embedding sort)"));
+  done[dev] = true;
+  return B2_OK;
+}
+
+template <int I>
+b2_status sort_one(const void* ids, int is64, int64_t T, int64_t V, int64_t pad, const SortPlan& p, uint32_t* key,
+                   uint32_t* tok, cudaStream_t st) {
+  const size_t smem = sizeof(SortSmem) + size_t(kSortThreads) * I * 8;
+  auto kern = embed_sort_one_kernel<I>;
+  static bool configured[64] = {};
+  B2_TRY(allow_smem(kern, smem, configured));
+  kern<<<1, kSortThreads, smem, st>>>(ids, is64, int(T), V, pad, p.passes, p.bits, key, tok);
+  return check_cuda(cudaGetLastError(), "embedding sort launch");
+}
+
+template <int I>
+b2_status sort_pass(const void* ids, int is64, int64_t T, int64_t V, int64_t pad, const SortPlan& p, int pass,
+                    uint32_t* table, const uint32_t* ki, const uint32_t* ti, uint32_t* ko, uint32_t* to,
+                    cudaStream_t st) {
+  const size_t smem = sizeof(SortSmem);
+  auto kern = embed_pass_kernel<I>;
+  static bool configured[64] = {};
+  B2_TRY(allow_smem(kern, smem, configured));
+  kern<<<unsigned(p.blocks), kSortThreads, smem, st>>>(ids, is64, T, V, pad, pass, p.passes, p.bits, table, ki, ti, ko,
+                                                       to);
+  return check_cuda(cudaGetLastError(), "embedding sort pass launch");
+}
+
+template <typename T, int N>
+b2_status run_fwd(const void* ids, int is64, int64_t tokens, const void* w, int64_t ldw, int64_t V, int64_t D,
+                  float scale, void* y, cudaStream_t st) {
+  constexpr int U = 4;
+  const int vecs = int(D / N);
+  const int ll = log_lanes_for(vecs);
+  const int rows = (256 >> ll) * U;
+  const int64_t bx = (tokens + rows - 1) / rows;
+  // few tokens: spread the columns over CTAs instead
+  const int by = bx >= 148 ? 1 : std::max(1, std::min((vecs + (1 << ll) - 1) >> ll, 64));
+  if (bx > INT32_MAX) return set_error(B2_ERR_UNSUPPORTED, "b2_embedding_fwd: too many tokens");
+  embed_fwd_kernel<T, N, U><<<dim3(unsigned(bx), unsigned(by)), 256, 0, st>>>(
+      ids, is64, tokens, static_cast<const T*>(w), ldw, V, vecs, ll, scale, static_cast<T*>(y), D,
+      device_status_ptr());
+  return check_cuda(cudaGetLastError(), "embedding forward launch");
+}
+
+template <typename T, int N>
+b2_status run_acc(const uint32_t* key, const uint32_t* tok, int64_t tokens, int64_t V, const void* dy, int64_t lddy,
+                  int64_t D, float scale, void* dw, float* partial, cudaStream_t st) {
+  const int vecs = int(D / N);
+  const int ll = log_lanes_for(vecs);
+  const int slabs = (vecs + (1 << ll) - 1) >> ll;
+  const int64_t pieces = (tokens + kPiece - 1) / kPiece;
+  const int per_block = kAccThreads >> ll;
+  const int64_t acc_blocks = (pieces + per_block - 1) / per_block * slabs;
+  // rows per zeroing CTA: about 64 KB of dW
+  const int zr = int(std::max<int64_t>(1, std::min<int64_t>(512, 65536 / (D * int64_t(sizeof(T))))));
+  const int64_t blocks = acc_blocks + (V + zr - 1) / zr;
+  if (blocks > INT32_MAX) return set_error(B2_ERR_UNSUPPORTED, "b2_embedding_bwd: too many rows");
+  embed_acc_kernel<T, N><<<unsigned(blocks), kAccThreads, 0, st>>>(
+      key, tok, tokens, V, static_cast<const T*>(dy), lddy, vecs, ll, D, scale, static_cast<T*>(dw), partial, pieces,
+      slabs, acc_blocks, zr);
+  B2_TRY(check_cuda(cudaGetLastError(), "embedding gradient launch"));
+  if (pieces > 1) {
+    const int by = std::max(1, std::min((vecs + kAccThreads - 1) / kAccThreads, 16));
+    embed_join_kernel<T, N><<<dim3(unsigned(pieces), unsigned(by)), kAccThreads, 0, st>>>(
+        key, tokens, V, vecs, D, scale, static_cast<T*>(dw), partial, pieces);
+    B2_TRY(check_cuda(cudaGetLastError(), "embedding gradient join launch"));
+  }
+  return B2_OK;
+}
+
+b2_status check_common(const char* who, int ids_dtype, int dtype, int64_t T, int64_t V, int64_t D, int64_t ld) {
+  if (ids_dtype != B2_I32 && ids_dtype != B2_I64) return set_error(B2_ERR_INVALID, "%s: ids must be int32 or int64", who);
+  if (dtype != B2_BF16 && dtype != B2_F32) return set_error(B2_ERR_INVALID, "%s: bad dtype %d", who, dtype);
+  if (T < 0 || V < 0 || D < 0 || ld < D) return set_error(B2_ERR_INVALID, "%s: bad shape", who);
+  if (T >= INT32_MAX || V >= INT32_MAX || D >= INT32_MAX)
+    return set_error(B2_ERR_UNSUPPORTED, "%s: tokens, vocabulary and width must be below 2^31 - 1", who);
+  return B2_OK;
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+b2_status b2_embedding_fwd(const void* ids, int ids_dtype, int64_t T, const void* weight, int64_t ldw, int dtype,
+                           int64_t V, int64_t D, float scale, void* y, void* stream) {
+  B2_TRY(check_common("b2_embedding_fwd", ids_dtype, dtype, T, V, D, ldw));
+  if (T == 0 || D == 0) return B2_OK;
+  if (!ids || !y || (!weight && V > 0)) return set_error(B2_ERR_INVALID, "b2_embedding_fwd: null pointer");
+  const auto st = static_cast<cudaStream_t>(stream);
+  const int is64 = ids_dtype == B2_I64;
+  if (dtype == B2_BF16) {
+    switch (vec_elems(2, D, ldw, weight, y)) {
+      case 8: return run_fwd<uint16_t, 8>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+      case 4: return run_fwd<uint16_t, 4>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+      case 2: return run_fwd<uint16_t, 2>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+      default: return run_fwd<uint16_t, 1>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+    }
+  }
+  switch (vec_elems(4, D, ldw, weight, y)) {
+    case 4: return run_fwd<float, 4>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+    case 2: return run_fwd<float, 2>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+    default: return run_fwd<float, 1>(ids, is64, T, weight, ldw, V, D, scale, y, st);
+  }
+}
+
+size_t b2_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) {
+  if (T <= 0 || V <= 0 || D <= 0 || T >= INT32_MAX || V >= INT32_MAX) return 0;
+  return embed_ws(T, V, D).total;
+}
+
+b2_status b2_embedding_bwd(const void* ids, int ids_dtype, int64_t T, const void* dy, int64_t lddy, int dtype,
+                           int64_t V, int64_t D, float scale, int64_t padding_idx, void* dw, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  B2_TRY(check_common("b2_embedding_bwd", ids_dtype, dtype, T, V, D, lddy));
+  if (V == 0 || D == 0) return B2_OK;
+  if (!dw) return set_error(B2_ERR_INVALID, "b2_embedding_bwd: null pointer");
+  const auto st = static_cast<cudaStream_t>(stream);
+  if (T == 0)
+    return check_cuda(cudaMemsetAsync(dw, 0, size_t(V) * size_t(D) * (dtype == B2_BF16 ? 2 : 4), st),
+                      "embedding gradient memset");
+  if (!ids || !dy || !workspace) return set_error(B2_ERR_INVALID, "b2_embedding_bwd: null pointer");
+  const EmbedWs w = embed_ws(T, V, D);
+  if (workspace_bytes < w.total || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return set_error(B2_ERR_WORKSPACE, "b2_embedding_bwd: workspace of %zu bytes (16-byte aligned) needed, got %zu",
+                     w.total, workspace_bytes);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  auto u32 = [&](size_t off) { return reinterpret_cast<uint32_t*>(base + off); };
+  const int is64 = ids_dtype == B2_I64;
+  const SortPlan p = sort_plan(T, V);
+  uint32_t *key = u32(w.key0), *tok = u32(w.tok0);
+  if (p.one) {
+    switch (p.items) {
+      case 1: B2_TRY(sort_one<1>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
+      case 2: B2_TRY(sort_one<2>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
+      case 4: B2_TRY(sort_one<4>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
+      default: B2_TRY(sort_one<8>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
+    }
+  } else {
+    uint32_t* table = u32(w.table);
+    embed_hist_kernel<<<unsigned(p.blocks), kSortThreads, 0, st>>>(ids, is64, T, V, padding_idx, p.passes, p.bits,
+                                                                   p.items * kSortThreads, table);
+    B2_TRY(check_cuda(cudaGetLastError(), "embedding histogram launch"));
+    uint32_t *ko = key, *to = tok, *ki = u32(w.key1), *ti = u32(w.tok1);
+    for (int pass = 0; pass < p.passes; ++pass) {
+      if (p.items == 2)
+        B2_TRY(sort_pass<2>(ids, is64, T, V, padding_idx, p, pass, table, ki, ti, ko, to, st));
+      else
+        B2_TRY(sort_pass<8>(ids, is64, T, V, padding_idx, p, pass, table, ki, ti, ko, to, st));
+      std::swap(ki, ko);
+      std::swap(ti, to);
+    }
+    key = ki;
+    tok = ti;
+  }
+  float* partial = reinterpret_cast<float*>(base + w.partial);
+  if (dtype == B2_BF16) {
+    switch (vec_elems(2, D, lddy, dy, dw)) {
+      case 8: return run_acc<uint16_t, 8>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+      case 4: return run_acc<uint16_t, 4>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+      case 2: return run_acc<uint16_t, 2>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+      default: return run_acc<uint16_t, 1>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+    }
+  }
+  switch (vec_elems(4, D, lddy, dy, dw)) {
+    case 4: return run_acc<float, 4>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+    case 2: return run_acc<float, 2>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+    default: return run_acc<float, 1>(key, tok, T, V, dy, lddy, D, scale, dw, partial, st);
+  }
+}
+
+}  // extern "C"

@@ -9,6 +9,7 @@
 
 #include <cstdlib>
 
+#include "lm.h"
 #include "xdna.h"
 
 namespace xdna {
@@ -443,4 +444,6 @@ PYBIND11_MODULE(_C, m) {
   m.def("region_bn_bwd", &region_bn_bwd);
   m.def("region_bn_forward", &region_bn_forward);
   m.def("region_bn_backward", &region_bn_backward);
+  bind_embedding(m);
+  bind_distill(m);
 }

@@ -7,6 +7,7 @@ the reference's ``xdna_train/__init__.py``); ``xdna:i`` is CUDA device ``i``.
 from .device import (
     allocator_stats,
     as_cuda,
+    as_xdna,
     async_dw_stats,
     autotune_result,
     bo_handle,
@@ -34,6 +35,7 @@ from .device import (
     try_register_xdna_device,
     wait_for_builds,
 )
+from . import lm
 
 __version__ = "0.1.0"
 
@@ -68,5 +70,7 @@ __all__ = [
     "coherency_state",
     "materialize",
     "as_cuda",
+    "as_xdna",
     "device_status",
+    "lm",
 ]

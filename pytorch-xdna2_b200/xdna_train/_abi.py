@@ -13,7 +13,7 @@ from pathlib import Path
 _LIB = None
 LIB_PATH = Path(__file__).resolve().parent / "libxdna_b200.so"
 
-B2_OK, B2_BF16, B2_F32 = 0, 0, 1
+B2_OK, B2_BF16, B2_F32, B2_I32, B2_I64 = 0, 0, 1, 2, 3
 
 i32, i64, f32, f64, vp, sz = C.c_int, C.c_int64, C.c_float, C.c_double, C.c_void_p, C.c_size_t
 
@@ -118,13 +118,22 @@ SIGNATURES = {
                                         vp],
     "b2_region_bn_fwd_bf16": [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32, f32, f32, i32, vp, sz, vp],
     "b2_region_bn_bwd_bf16": [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32, i32, vp, sz, vp],
+    "b2_embedding_fwd": [vp, i32, i64, vp, i64, i32, i64, i64, f32, vp, vp],
+    "b2_embedding_bwd_workspace_bytes": [i64, i64, i64],
+    "b2_embedding_bwd": [vp, i32, i64, vp, i64, i32, i64, i64, f32, i64, vp, vp, sz, vp],
+    "b2_distill_workspace_bytes": [i64],
+    "b2_distill_loss_fwd": [vp, i64, i32, i64, i64, vp, i64, i32, vp, i64, i32, i64, f32, vp, i32, vp, vp, vp, i64, vp,
+                            sz, vp],
+    "b2_distill_loss_bwd": [vp, i64, i32, i64, i64, vp, i64, i32, vp, i64, i32, i64, f32, vp, i32, vp, vp, i32, vp, i64,
+                            vp],
 }
 _RESTYPES = {"b2_last_error": C.c_char_p, "b2_conv3x3_wgrad_workspace_bytes": sz,
              "b2_pack_rows_dbias_workspace_bytes": sz, "b2_region_bn_workspace_bytes": sz,
              "b2_conv1x1_wgrad_workspace_bytes": sz, "b2_direct_conv_weight_floats": sz, "b2_gemm_splitk_workspace_bytes": sz,
              "b2_batch_norm_workspace_bytes": sz, "b2_channel_sum_nhwc_workspace_bytes": sz,
              "b2_gemm_bf16_workspace_bytes": sz,
-             "b2_conv3x3_wgrad_noalloc_max_bytes": sz}
+             "b2_conv3x3_wgrad_noalloc_max_bytes": sz, "b2_embedding_bwd_workspace_bytes": sz,
+             "b2_distill_workspace_bytes": sz}
 
 
 class B2Error(RuntimeError):

@@ -421,6 +421,13 @@ def as_cuda(tensor: torch.Tensor) -> torch.Tensor:
     return _C.as_cuda(tensor)
 
 
+def as_xdna(tensor: torch.Tensor) -> torch.Tensor:
+    """Zero-copy xdna tensor over a CUDA tensor's memory, which it keeps alive
+    (the way back from ``as_cuda``: data that CUDA code made, without a copy)."""
+    register_xdna_device()
+    return _C.adopt(tensor)
+
+
 def device_status(device: int = 0) -> int:
     """Reads and clears the device-side error word (0 = no kernel gave up)."""
     register_xdna_device()

@@ -1,0 +1,68 @@
+"""The plain CPU path of xdna_train.lm against the definitions, and the C
+ABI's argument checks that need no GPU."""
+import math
+
+import pytest
+import torch
+
+from xdna_train import _abi, lm
+
+
+def test_embedding_on_cpu():
+    w = torch.randn(7, 5, requires_grad=True)
+    ids = torch.tensor([[1, 6], [1, 0]])
+    y = lm.embedding(ids, w, scale=3.0, padding_idx=0)
+    assert torch.equal(y, 3.0 * w[ids])
+    (dw,) = torch.autograd.grad(y.sum(), [w])
+    assert torch.equal(dw[:, 0], torch.tensor([0.0, 6, 0, 0, 0, 0, 3]))
+    with pytest.raises(ValueError, match="padding_idx"):
+        lm.embedding(ids, w, padding_idx=7)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_distill_loss_on_cpu(reduction):
+    g = torch.Generator().manual_seed(0)
+    z = torch.randn(4, 9, generator=g, requires_grad=True)
+    t = torch.randn(4, 3, generator=g)
+    ids = torch.tensor([[0, 4, 8], [1, -1, 2], [-1, -1, -1], [3, 3, 5]])
+    w = torch.tensor([1.0, 0.5, 1.0, 2.0])
+    tau = 2.0
+    loss = lm.distill_loss(z, t, ids, tau, w, reduction)
+    rows = []
+    for r in range(4):
+        kept = [k for k in range(3) if ids[r, k] >= 0]
+        p = torch.softmax(t[r, kept] / tau, 0)
+        logq = torch.log_softmax(z[r] / tau, 0)
+        rows.append(w[r] * tau ** 2 * sum(p[i] * (p[i].log() - logq[ids[r, k]]) for i, k in enumerate(kept)))
+    rows = torch.stack([torch.as_tensor(r, dtype=torch.float32) for r in rows])
+    ref = {"mean": rows.sum() / w.sum(), "sum": rows.sum(), "none": rows}[reduction]
+    assert torch.allclose(loss, ref, rtol=1e-5, atol=1e-6)
+    (a,) = torch.autograd.grad(loss.sum(), [z], retain_graph=True)
+    (b,) = torch.autograd.grad(ref.sum(), [z])
+    assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
+def test_distill_loss_masks_on_cpu():
+    z = torch.randn(3, 6)
+    z[1] = math.nan
+    z[2, 4:] = -math.inf
+    z.requires_grad_()
+    loss = lm.distill_loss(z, torch.zeros(3, 2), torch.tensor([[0, 1], [0, 1], [2, 3]]),
+                           row_weight=torch.tensor([1.0, 0.0, 1.0]))
+    (dz,) = torch.autograd.grad(loss, [z])
+    assert loss.isfinite() and dz.isfinite().all() and not dz[1].any()
+
+
+def test_argument_errors_need_no_gpu():
+    L = _abi.lib()
+    assert L.b2_embedding_fwd(None, _abi.B2_I64, 3, None, 8, _abi.B2_F32, 5, 8, 1.0, None, None) == 1
+    assert b"null pointer" in L.b2_last_error()
+    assert L.b2_embedding_fwd(8, _abi.B2_F32, 3, 8, 8, _abi.B2_F32, 5, 8, 1.0, 8, None) == 1
+    assert b"int32 or int64" in L.b2_last_error()
+    assert L.b2_embedding_bwd(8, _abi.B2_I64, 3, 8, 7, _abi.B2_F32, 5, 8, 1.0, -1, 8, 8, 0, None) == 1
+    assert b"bad shape" in L.b2_last_error()
+    assert L.b2_embedding_fwd(8, _abi.B2_I64, 1 << 31, 8, 8, _abi.B2_F32, 5, 8, 1.0, 8, None) == 3
+    args = [8, 50, _abi.B2_F32, 3, 50, 8, 4, _abi.B2_F32, 8, 4, _abi.B2_I64, 4, 1.0, None, 0, 8, 8, None, 50, 8, 0, None]
+    assert L.b2_distill_loss_fwd(*args) == 5 and b"workspace" in L.b2_last_error()
+    assert L.b2_distill_loss_fwd(*args[:12], -1.0, *args[13:]) == 1 and b"temperature" in L.b2_last_error()
+    assert L.b2_distill_loss_fwd(*args[:11], 1025, *args[12:]) == 3 and b"1024" in L.b2_last_error()
