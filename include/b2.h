@@ -707,6 +707,40 @@ b2_status b2_distill_loss_bwd(const void* z, int64_t ldz, int dtype, int64_t N,
                               int skip_ones, void* dz, int64_t lddz,
                               void* stream);
 
+/* Gated feed-forward block on bf16 tensors: h = act(x Wg^T) * (x Wu^T), y = h
+ * Wd^T.  x [M][D], w_gate and w_up [F][D], w_down [E][F], y [M][E], each with a
+ * row stride in elements (any; rows that are not 16-byte aligned are copied to
+ * the workspace first).  act 0: silu, 1: gelu (erf), 2: relu.  fp32 sums; h is
+ * rounded to bf16 as an operand of the second product.  saved (may be NULL): what
+ * the backward needs, bf16 [M][3][F rounded up to 8] (h, u act'(g), act(g)),
+ * 16-byte aligned.  Workspace: b2_gated_mlp_fwd_workspace_bytes(), 256-byte aligned. */
+size_t b2_gated_mlp_fwd_workspace_bytes(int64_t M, int64_t D, int64_t F,
+                                        int64_t E);
+b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate,
+                                int64_t ldg, const void* w_up, int64_t ldu,
+                                const void* w_down, int64_t ldd, int act,
+                                void* y, int64_t ldy, void* saved, int64_t M,
+                                int64_t D, int64_t F, int64_t E,
+                                void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* Its gradients from dy [M][E] (row stride lddy), the forward's operands and
+ * saved: dh = dy Wd, dg = dh u act'(g), du = dh act(g); dx = dg Wg + du Wu [M][D],
+ * dw_gate = dg^T x and dw_up = du^T x [F][D], dw_down = dy^T h [E][F], all dense
+ * bf16, each may be NULL.  dg and du are rounded to bf16 as operands.  With
+ * M == 0 the weights' gradients are zero.  Workspace:
+ * b2_gated_mlp_bwd_workspace_bytes(), 256-byte aligned. */
+size_t b2_gated_mlp_bwd_workspace_bytes(int64_t M, int64_t D, int64_t F,
+                                        int64_t E);
+b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x,
+                                int64_t ldx, const void* w_gate, int64_t ldg,
+                                const void* w_up, int64_t ldu,
+                                const void* w_down, int64_t ldd, int act,
+                                const void* saved, void* dx, void* dw_gate,
+                                void* dw_up, void* dw_down, int64_t M,
+                                int64_t D, int64_t F, int64_t E,
+                                void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

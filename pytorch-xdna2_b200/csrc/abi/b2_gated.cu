@@ -1,0 +1,1099 @@
+// Gated feed-forward block, forward and backward, on the tcgen05 tensor cores.
+//
+//   forward   g = x Wg^T, u = x Wu^T, h = act(g) * u, y = h Wd^T
+//   backward  dh = dy Wd
+//             dg = dh * u * act'(g), du = dh * act(g)
+//             dx = dg Wg + du Wu
+//             dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// x [M][D], Wg and Wu [F][D], Wd [E][F], y [M][E]; bf16 with fp32 sums.  Five
+// products of the same size, 6 M D F operations forward and 12 M D F backward;
+// all of them run in one kernel template, a persistent SM-pair GEMM
+// (tcgen05.mma.cta_group::2, 256 x PBN output tiles) that differs in its
+// epilogue:
+//   kGate      both projections in one tile: the pair's first CTA brings PBN/2
+//              rows of Wg as its half of the B operand, the second the same
+//              rows of Wu, so a thread finds g and u of the same hidden unit in
+//              its own accumulator row and writes h in one epilogue; for
+//              training also the factors P = u act'(g) and A = act(g)
+//   kGateBwd   the tile of dh with P and A of the same place: writes dg = dh P
+//              and du = dh A
+//   kStore     a plain product, up to three of them in one launch; the two
+//              halves of dx are one reduction over 2F whose operands change in
+//              the middle
+// h, P, A, dg and du are rounded to bf16 once each, from fp32: a relative error
+// of at most 2^-8, that of the tensors themselves.  Keeping the factors P and A rather
+// than g and u costs no more room beside h, leaves the backward's epilogue two
+// products instead of an exponential, and is more exact (a rounded g moves
+// act'(g) and with it h, dg and du: 1.8 against 1.2 roundings in dWd).
+//
+// Everything is bound by the tensor pipe or, for few tokens, by reading the
+// weights.  Reductions whose tiles would leave most SM pairs idle are split;
+// the fp32 partial tiles are added in split order by a second kernel that then
+// runs the same epilogue (bit-reproducible).
+#include <algorithm>
+
+#include "b2_common.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int BK = 64;
+constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2..9 epilogue
+constexpr int kEpiWarps = 8;
+constexpr int kABytes = 128 * BK * 2;
+constexpr int kMaxProblems = 3;
+constexpr int kGroupM = 8;     // row tiles walked together (operand reuse in L2)
+
+enum Epi : int { kStore = 0, kGate = 1, kGateBwd = 2 };
+enum Act : int { kSilu = 0, kGelu = 1, kRelu = 2 };
+
+struct Problem {
+  int tiles_m, tiles_n;
+  int M, N;           // valid output rows / columns (kGate: N = F)
+  int kb, kb_first;   // k-blocks; of these, the ones from the first operand pair
+  int splits, kb_per_split;
+  int item_begin;     // first work item
+  int tma_out;
+  uint16_t* out;
+  long long ldo;
+  float* partial;     // splits > 1: [tiles][splits] partial tiles
+};
+
+struct Maps {
+  CUtensorMap a[kMaxProblems], b[kMaxProblems], o[kMaxProblems];
+};
+
+struct Params {
+  Problem p[kMaxProblems];
+  int problems, items;
+  int act;
+  // the factors P and A: kGate writes them if train, kGateBwd reads them
+  int train;
+  const uint16_t *fp, *fa;
+  long long ldf;
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t cvt2(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint16_t cvt1(float v) {
+  __nv_bfloat16 h = __float2bfloat16_rn(v);
+  return *reinterpret_cast<uint16_t*>(&h);
+}
+
+// act(g) and act'(g)
+__device__ __forceinline__ float act_value(int act, float g) {
+  if (act == kSilu) return __fdividef(g, 1.f + __expf(-g));
+  if (act == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  return g > 0.f || g != g ? g : 0.f;
+}
+__device__ __forceinline__ void act_both(int act, float g, float& a, float& slope) {
+  if (act == kSilu) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    a = g * s;
+    slope = s * (1.f + g * (1.f - s));
+  } else if (act == kGelu) {
+    const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    a = g * cdf;
+    slope = cdf + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+  } else {
+    a = g > 0.f || g != g ? g : 0.f;
+    slope = g > 0.f ? 1.f : 0.f;
+  }
+}
+
+template <int EPI, int PBN>
+struct Config {
+  static constexpr int kBHalf = PBN / 2;
+  static constexpr int kStage = kABytes + kBHalf * BK * 2;
+  // per epilogue warp: kStore two 32 x 64 boxes, kGate three 32 x 32 boxes, kGateBwd two pairs of 32 x 32 boxes
+  static constexpr int kEpiBytes = EPI == kGate ? 3 * 2048 : 2 * 4096;
+  static constexpr int kStages = PBN == 256 ? 5 : (EPI == kGate ? 7 : 6);
+  static constexpr size_t kSmem = size_t(kStages) * kStage + kEpiWarps * kEpiBytes + 1024 + 256;
+};
+
+struct Item {
+  int prob, mt, nt, split, kb0, kb1, tile;
+};
+
+__device__ __forceinline__ Item decode(const Params& p, int t) {
+  Item it;
+  int i = 0;
+  while (i + 1 < p.problems && t >= p.p[i + 1].item_begin) ++i;
+  const Problem& q = p.p[i];
+  t -= q.item_begin;
+  it.prob = i;
+  // the splits of a tile are neighbours
+  it.split = t % q.splits;
+  t /= q.splits;
+  it.tile = t;
+  const int group = t / (kGroupM * q.tiles_n);
+  const int first = group * kGroupM;
+  const int rows = min(kGroupM, q.tiles_m - first);
+  const int in = t - first * q.tiles_n;
+  it.mt = first + in % rows;
+  it.nt = in / rows;
+  it.kb0 = it.split * q.kb_per_split;
+  it.kb1 = min(q.kb, it.kb0 + q.kb_per_split);
+  return it;
+}
+
+// Partial tiles: [tile][split][rank * 8 + warp][chunk][4-column group][lane]
+// float4, so that a warp's accesses are contiguous.  Returns the float4 of
+// 4-column group q of accumulator columns [32 j, 32 j + 32) of one warp.
+template <int PBN>
+__device__ __forceinline__ float4* partial_at(const Problem& q, int tile, int split, int region, int j, int lane) {
+  return reinterpret_cast<float4*>(q.partial) +
+         ((((long long)tile * q.splits + split) * 16 + region) * (PBN / 64) + j) * 256 + lane;
+}
+
+// 32 columns of one row of the factors P and A.  Their rows hold a multiple of
+// 8 columns, so a 16-byte load that starts below N stays inside the row.
+struct Factors {
+  uint32_t v[2][16];
+  __device__ __forceinline__ void load(const Params& p, int row, int c0, int N, int M) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      if (row < M && c0 + c * 8 < N) {
+        a = *reinterpret_cast<const uint4*>(p.fp + (long long)row * p.ldf + c0 + c * 8);
+        b = *reinterpret_cast<const uint4*>(p.fa + (long long)row * p.ldf + c0 + c * 8);
+      }
+      v[0][4 * c] = a.x;
+      v[0][4 * c + 1] = a.y;
+      v[0][4 * c + 2] = a.z;
+      v[0][4 * c + 3] = a.w;
+      v[1][4 * c] = b.x;
+      v[1][4 * c + 1] = b.y;
+      v[1][4 * c + 2] = b.z;
+      v[1][4 * c + 3] = b.w;
+    }
+  }
+};
+
+// 32 bf16 columns (packed in pairs) of this thread's row, elementwise
+__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&v)[16], int cols) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c)
+    if (c < cols) dst[c] = uint16_t((c & 1) ? (v[c >> 1] >> 16) : (v[c >> 1] & 0xffff));
+}
+
+template <int EPI, int PBN, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gated_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using C = Config<EPI, PBN>;
+  constexpr int STAGES = C::kStages;
+  constexpr uint32_t kIdesc = idesc_bf16_f32(256, PBN, A_MN, B_MN);
+  constexpr uint32_t kTmemCols = 2 * PBN;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi_stage = smem + STAGES * C::kStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi_stage + kEpiWarps * C::kEpiBytes);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + STAGES;
+  uint64_t* tfull = bars + 2 * STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* mma_done = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cluster = blockIdx.x >> 1;
+  const int nclusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&tfull[a]), 1);
+      mbar_init(smem_u32(&tempty[a]), 2 * kEpiWarps);
+    }
+    mbar_init(smem_u32(mma_done), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers initialized before any cross-CTA signal
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------ producer (both CTAs) -----------------
+      int stage = 0;
+      uint32_t phase = 0;
+      int last_par[STAGES];
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) last_par[s] = -1;
+      bool ok = true;
+      for (int t = cluster; t < p.items && ok; t += nclusters) {
+        const Item it = decode(p, t);
+        const Problem& q = p.p[it.prob];
+        const int row0 = it.mt * 256 + int(rank) * 128;
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          if (!mbar_wait(smem_u32(&empty[stage]), phase ^ 1, p.status, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb_local = smem_u32(&full[stage]);
+          if (leader) mbar_arrive_expect_tx(fb_local, 2 * C::kStage);
+          last_par[stage] = int(phase);
+          const uint32_t fb = mapa_shared(fb_local, 0);
+          const uint32_t sa = smem_u32(smem + stage * C::kStage);
+          const uint32_t sb = sa + kABytes;
+          // the reduction's second half has operands of its own (dx)
+          const bool second = kb >= q.kb_first;
+          const int k0 = (second ? kb - q.kb_first : kb) * BK;
+          const CUtensorMap* ma = &maps.a[it.prob + (second ? 1 : 0)];
+          const CUtensorMap* mb = &maps.b[it.prob + (second ? 1 : 0)];
+          // B: this CTA's half of the tile's columns; kGate: the tile's hidden units in Wg or Wu
+          int n0 = it.nt * PBN + int(rank) * C::kBHalf;
+          if constexpr (EPI == kGate) {
+            mb = &maps.b[rank];
+            n0 = it.nt * C::kBHalf;
+          }
+          if constexpr (A_MN) {
+            tma_load_3d_pair(sa, ma, fb, row0, k0, 0);
+            tma_load_3d_pair(sa + 8192, ma, fb, row0 + 64, k0, 0);
+          } else {
+            tma_load_3d_pair(sa, ma, fb, k0, row0, 0);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int h = 0; h < C::kBHalf / 64; ++h) tma_load_3d_pair(sb + h * 8192, mb, fb, n0 + h * 64, k0, 0);
+          } else {
+            tma_load_3d_pair(sb, mb, fb, k0, n0, 0);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok && leader) {  // let issued copies land before the CTA goes away
+        for (int s = 0; s < STAGES; ++s)
+          if (last_par[s] >= 0) mbar_wait(smem_u32(&full[s]), uint32_t(last_par[s]), p.status, nullptr);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ------------------------------ MMA issuer (leader CTA) --------------
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int t = cluster; t < p.items && ok; t += nclusters) {
+        const Item it = decode(p, t);
+        if (!mbar_wait(smem_u32(&tempty[acc]), acc_phase ^ 1, p.status, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + uint32_t(acc * PBN);
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          if (!mbar_wait(smem_u32(&full[stage]), phase, p.status, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * C::kStage);
+          const uint32_t sb = sa + kABytes;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint64_t ad =
+                A_MN ? smem_desc_sw128(sa + k * 2048, 8192, 1024) : smem_desc_sw128(sa + k * 32, 16, 1024);
+            const uint64_t bd =
+                B_MN ? smem_desc_sw128(sb + k * 2048, 8192, 1024) : smem_desc_sw128(sb + k * 32, 16, 1024);
+            tc_mma_pair(d_tmem, ad, bd, kIdesc, (kb > it.kb0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit_pair_mc(smem_u32(&empty[stage]), uint16_t(0x3));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair_mc(smem_u32(&tfull[acc]), uint16_t(0x3));
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+      tc_commit_pair(smem_u32(mma_done));
+      mbar_wait(smem_u32(mma_done), 0, p.status, nullptr);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------- epilogue (both CTAs) ------------------
+    const int quarter = warp & 3;         // tensor-memory lane quarter this warp may read
+    const int half = (warp - 2) >> 2;     // half of the accumulator's columns
+    const int region = int(rank) * 8 + half * 4 + quarter;
+    const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
+    uint8_t* buf = epi_stage + (warp - 2) * C::kEpiBytes;
+    int sel = 0;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = cluster; t < p.items; t += nclusters) {
+      const Item it = decode(p, t);
+      const Problem& q = p.p[it.prob];
+      const int row0 = it.mt * 256 + int(rank) * 128 + quarter * 32;
+      const int row = row0 + lane;
+      // the first factors of the tile travel while its product is still running
+      Factors factors;
+      if constexpr (EPI == kGateBwd)
+        if (q.splits == 1) factors.load(p, row, it.nt * PBN + half * (PBN / 2), q.N, q.M);
+      bool ok = mbar_wait(smem_u32(&tfull[acc]), acc_phase, p.status, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t tacc = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * PBN);
+      const uint32_t thalf = tacc + uint32_t(half * (PBN / 2));
+      if (q.splits > 1) {
+        if (row0 < q.M) {
+#pragma unroll 1
+          for (int j = 0; j < PBN / 64; ++j) {
+            uint32_t r[32];
+            tmem_ld32(thalf + j * 32, r);
+            tc_wait_ld();
+            float4* dst = partial_at<PBN>(q, it.tile, it.split, region, j, lane);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              dst[c * 32] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]),
+                                        __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
+          }
+        }
+      } else if constexpr (EPI == kStore) {
+        if (q.tma_out) {
+          // Boxes of 32 rows x 64 columns staged with the tensor map's 128-byte
+          // swizzle (16-byte chunk c of row r at chunk c ^ (r & 7): the eight
+          // rows of a store phase hit distinct banks) and written by the TMA
+          // unit in whole rows, clipped at M and N; one box fills while the
+          // other's store reads it.
+#pragma unroll 1
+          for (int j = 0; j < PBN / 128; ++j) {
+            const int c0 = it.nt * PBN + half * (PBN / 2) + j * 64;
+            if (c0 >= q.N || row0 >= q.M) break;
+            uint32_t r[2][32];
+            tmem_ld32(thalf + j * 64, r[0]);
+            tmem_ld32(thalf + j * 64 + 32, r[1]);
+            tc_wait_ld();
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+            uint8_t* box = buf + sel * 4096;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint32_t* v = &r[c >> 2][(c & 3) * 8];
+              *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                  make_uint4(cvt2(__uint_as_float(v[0]), __uint_as_float(v[1])),
+                             cvt2(__uint_as_float(v[2]), __uint_as_float(v[3])),
+                             cvt2(__uint_as_float(v[4]), __uint_as_float(v[5])),
+                             cvt2(__uint_as_float(v[6]), __uint_as_float(v[7])));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&maps.o[it.prob], smem_u32(box), c0, row0, 0);
+              bulk_commit();
+            }
+            sel ^= 1;
+          }
+        } else {
+          // output rows that no 16-byte store can address: element by element
+#pragma unroll 1
+          for (int j = 0; j < PBN / 64; ++j) {
+            const int c0 = it.nt * PBN + half * (PBN / 2) + j * 32;
+            uint32_t r[32], v[16];
+            tmem_ld32(thalf + j * 32, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) v[c] = cvt2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+            if (row < q.M) store_row32(q.out + (long long)row * q.ldo + c0, v, min(32, q.N - c0));
+          }
+        }
+      } else {
+        // gate epilogues: 32 hidden units at a time, staged in 32 x 32 boxes
+        // (64-byte swizzle: chunk c of row r at chunk c ^ ((r >> 1) & 3))
+        auto fill = [&](uint8_t* box, const uint32_t (&v)[16]) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        };
+        if constexpr (EPI == kGate) {
+          const int f0 = it.nt * (PBN / 2) + half * (PBN / 4);
+#pragma unroll 1
+          for (int j = 0; j < PBN / 128; ++j) {
+            const int c0 = f0 + j * 32;
+            if (c0 >= q.N || row0 >= q.M) break;
+            uint32_t g[32], u[32];
+            tmem_ld32(tacc + uint32_t(half * (PBN / 4) + j * 32), g);
+            tmem_ld32(tacc + uint32_t(PBN / 2 + half * (PBN / 4) + j * 32), u);
+            tc_wait_ld();
+            if (lane == 0) bulk_wait_read<0>();  // the boxes' last stores have read them
+            __syncwarp();
+            uint32_t h[16];
+            if (p.train) {
+              uint32_t fp[16], fa[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float u0 = __uint_as_float(u[2 * c]), u1 = __uint_as_float(u[2 * c + 1]);
+                float a0, s0, a1, s1;
+                act_both(p.act, __uint_as_float(g[2 * c]), a0, s0);
+                act_both(p.act, __uint_as_float(g[2 * c + 1]), a1, s1);
+                h[c] = cvt2(a0 * u0, a1 * u1);
+                fp[c] = cvt2(s0 * u0, s1 * u1);
+                fa[c] = cvt2(a0, a1);
+              }
+              fill(buf + 2048, fp);
+              fill(buf + 4096, fa);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 16; ++c)
+                h[c] = cvt2(act_value(p.act, __uint_as_float(g[2 * c])) * __uint_as_float(u[2 * c]),
+                            act_value(p.act, __uint_as_float(g[2 * c + 1])) * __uint_as_float(u[2 * c + 1]));
+            }
+            fill(buf, h);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&maps.o[0], smem_u32(buf), c0, row0, 0);
+              if (p.train) {
+                tma_store_3d(&maps.o[1], smem_u32(buf + 2048), c0, row0, 0);
+                tma_store_3d(&maps.o[2], smem_u32(buf + 4096), c0, row0, 0);
+              }
+              bulk_commit();
+            }
+          }
+        } else {
+          const int f0 = it.nt * PBN + half * (PBN / 2);
+#pragma unroll 1
+          for (int j = 0; j < PBN / 64; ++j) {
+            const int c0 = f0 + j * 32;
+            if (c0 >= q.N || row0 >= q.M) break;
+            uint32_t pv[16], av[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              pv[c] = factors.v[0][c];
+              av[c] = factors.v[1][c];
+            }
+            factors.load(p, row, c0 + 32, j + 1 < PBN / 64 ? q.N : 0, q.M);
+            uint32_t d[32];
+            tmem_ld32(thalf + j * 32, d);
+            tc_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float d0 = __uint_as_float(d[2 * c]), d1 = __uint_as_float(d[2 * c + 1]);
+              pv[c] = cvt2(d0 * __uint_as_float(pv[c] << 16), d1 * __uint_as_float(pv[c] & 0xffff0000u));
+              av[c] = cvt2(d0 * __uint_as_float(av[c] << 16), d1 * __uint_as_float(av[c] & 0xffff0000u));
+            }
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+            uint8_t* box = buf + sel * 4096;
+            fill(box, pv);
+            fill(box + 2048, av);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&maps.o[1], smem_u32(box), c0, row0, 0);
+              tma_store_3d(&maps.o[2], smem_u32(box + 2048), c0, row0, 0);
+              bulk_commit();
+            }
+            sel ^= 1;
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader)
+          mbar_arrive(smem_u32(&tempty[acc]));
+        else
+          mbar_arrive_remote(tempty_leader[acc]);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_all();  // stores done before the CTA's shared memory goes away
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its pair may still signal or read it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+// Adds a problem's partial tiles in split order and finishes them with its
+// epilogue.  A thread takes 8 columns of one row (kGate: of g and of u); the
+// lanes of a warp are 32 rows, so its partial reads are contiguous.
+struct ReduceArgs {
+  Problem q;
+  int act, train;
+  uint16_t *h, *o1, *o2;           // kGate: h, P, A; kGateBwd: -, dg, du
+  const uint16_t *fp, *fa;
+  long long ldh, ldo, ldf;
+};
+
+template <int PBN>
+__device__ __forceinline__ void sum8(const Problem& q, int tile, int region, int j, int oct, int lane, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < q.splits; ++s) {
+    const float4* src = partial_at<PBN>(q, tile, s, region, j, lane) + oct * 64;
+    const float4 a = __ldcg(src), b = __ldcg(src + 32);
+    v[0] += a.x;
+    v[1] += a.y;
+    v[2] += a.z;
+    v[3] += a.w;
+    v[4] += b.x;
+    v[5] += b.y;
+    v[6] += b.z;
+    v[7] += b.w;
+  }
+}
+
+__device__ __forceinline__ void put8(uint16_t* dst, const float (&v)[8], int cols, bool vec) {
+  if (vec && cols >= 8) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(cvt2(v[0], v[1]), cvt2(v[2], v[3]), cvt2(v[4], v[5]), cvt2(v[6], v[7]));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < cols) dst[i] = cvt1(v[i]);
+}
+
+template <int EPI, int PBN>
+__global__ void __launch_bounds__(256) gated_reduce_kernel(const __grid_constant__ ReduceArgs a) {
+  const Problem& q = a.q;
+  constexpr int kCols = EPI == kGate ? PBN / 2 : PBN;  // output columns of a tile
+  constexpr int kOcts = kCols / 8;
+  const int lane = threadIdx.x & 31;
+  const long long units = (long long)q.tiles_m * q.tiles_n * 8 * kOcts;  // (tile, 32-row block, 8 columns)
+  for (long long w = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5; w < units; w += (long long)gridDim.x * 8) {
+    const int oc = int(w % kOcts);
+    const long long rest = w / kOcts;
+    const int rows = int(rest % 8);  // rank * 4 + quarter
+    const int tile = int(rest / 8);
+    const int group = tile / (kGroupM * q.tiles_n), first = group * kGroupM;
+    const int gm = min(kGroupM, q.tiles_m - first), in = tile - first * q.tiles_n;
+    const int mt = first + in % gm, nt = in / gm;
+    const int row = mt * 256 + rows * 32 + lane;
+    const int col = nt * kCols + oc * 8;
+    if (row >= q.M || col >= q.N) continue;
+    const int rank = rows >> 2, quarter = rows & 3;
+    const int cols = q.N - col;
+    float v[8];
+    if constexpr (EPI == kGate) {
+      float g[8];
+      sum8<PBN>(q, tile, rank * 8 + quarter, oc / 4, oc & 3, lane, g);
+      sum8<PBN>(q, tile, rank * 8 + 4 + quarter, oc / 4, oc & 3, lane, v);
+      float h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float act, slope;
+        act_both(a.act, g[i], act, slope);
+        h[i] = act * v[i];
+        v[i] *= slope;
+        g[i] = act;
+      }
+      put8(a.h + (long long)row * a.ldh + col, h, cols, true);
+      if (a.train) {
+        put8(a.o1 + (long long)row * a.ldo + col, v, cols, true);
+        put8(a.o2 + (long long)row * a.ldo + col, g, cols, true);
+      }
+    } else {
+      const int half = oc / (PBN / 16), o = oc % (PBN / 16);
+      sum8<PBN>(q, tile, rank * 8 + half * 4 + quarter, o / 4, o & 3, lane, v);
+      if constexpr (EPI == kStore) {
+        uint16_t* dst = q.out + (long long)row * q.ldo + col;
+        put8(dst, v, cols, (reinterpret_cast<uintptr_t>(dst) & 15) == 0);
+      } else {
+        const uint4 pv = *reinterpret_cast<const uint4*>(a.fp + (long long)row * a.ldf + col);
+        const uint4 av = *reinterpret_cast<const uint4*>(a.fa + (long long)row * a.ldf + col);
+        const uint16_t* pe = reinterpret_cast<const uint16_t*>(&pv);
+        const uint16_t* ae = reinterpret_cast<const uint16_t*>(&av);
+        float dg[8], du[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dg[i] = v[i] * bf2f(pe[i]);
+          du[i] = v[i] * bf2f(ae[i]);
+        }
+        put8(a.o1 + (long long)row * a.ldo + col, dg, cols, true);
+        put8(a.o2 + (long long)row * a.ldo + col, du, cols, true);
+      }
+    }
+  }
+}
+
+// Copies of matrices whose rows no TMA map can address (a row stride that is
+// not a multiple of 16 bytes, or a misaligned base) into rows that one can.
+struct PadArgs {
+  const uint16_t* src[5];
+  uint16_t* dst[5];
+  long long lds[5];
+  int rows[5], cols[5], ldd[5];
+  long long begin[6];  // prefix sums of 8-column groups
+  int n;
+};
+__global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ PadArgs a) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.begin[a.n]; i += (long long)gridDim.x * 256) {
+    int m = 0;
+    while (i >= a.begin[m + 1]) ++m;
+    const long long at = i - a.begin[m];
+    const int groups = a.ldd[m] / 8;
+    const long long row = at / groups;
+    const int col = int(at - row * groups) * 8;
+    const uint16_t* s = a.src[m] + row * a.lds[m] + col;
+    uint16_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = col + e < a.cols[m] ? s[e] : uint16_t(0);
+    *reinterpret_cast<uint4*>(a.dst[m] + row * a.ldd[m] + col) = *reinterpret_cast<uint4*>(v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+bool tma_rows(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
+
+// A matrix in memory: rows x cols, row stride ld.
+struct Mat {
+  const void* p = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0;
+};
+
+b2_status map2d(CUtensorMap* m, const Mat& a, uint32_t box_cols, uint32_t box_rows, int swizzle) {
+  const uint64_t dims[3] = {uint64_t(a.cols), uint64_t(a.rows), 1};
+  const uint64_t strides[2] = {uint64_t(a.ld) * 2, uint64_t(a.ld) * 2 * uint64_t(a.rows)};
+  const uint32_t box[3] = {box_cols, box_rows, 1};
+  return encode_tmap_sw(m, a.p, 3, dims, strides, box, swizzle);
+}
+
+// One product: out[M][N] = A B with the operands as stored.  A: [M][K] or, MN
+// (k-rows), [K][M]; B: [N][K] or [K][N].
+struct Product {
+  Mat a[2], b[2];   // the second pair continues the reduction (or, kGate, b[1] is Wu)
+  int64_t M = 0, N = 0, K = 0;
+  int pairs = 1;
+  void* out = nullptr;
+  int64_t ldo = 0;
+};
+
+struct Plan {
+  int pbn = 256;
+  int splits = 1;
+  size_t partial_bytes = 0;
+};
+
+// Tile width and reduction splits of a product.  Cost in SM clocks of a pair
+// on its busiest pair: a k-block of a 256-wide tile takes 512 clocks of the
+// tensor pipe, of a 128-wide one 256 but about 400 to bring its operands from
+// L2; each tile adds a pipeline fill and drain; a split adds writing and
+// reading the fp32 partials and the second kernel.
+Plan plan_product(int64_t M, int64_t N, int64_t K, int pairs, bool gate, int sms) {
+  const int clusters = std::max(1, sms / 2);
+  const int64_t kb = (K + BK - 1) / BK * pairs;
+  Plan best{};
+  double best_cost = 1e300;
+  for (int pbn : {256, 128}) {
+    const int64_t cols = gate ? pbn / 2 : pbn;
+    const int64_t tiles = ((M + 255) / 256) * ((N + cols - 1) / cols);
+    for (int s = 1; s <= 16; ++s) {
+      if (s > 1 && (kb / s < 4 || tiles * s > 2 * clusters)) break;
+      const int64_t kps = (kb + s - 1) / s;
+      const int64_t splits = (kb + kps - 1) / kps;
+      if (splits != s) continue;
+      const int64_t waves = (tiles * s + clusters - 1) / clusters;
+      double cost = double(waves) * (double(kps) * (pbn == 256 ? 512 : 400) + 800) + 2500;
+      if (s > 1) cost += 4000 + double(tiles) * 256 * pbn * 4 * s * 2 / 2500.0;
+      if (cost < best_cost) {
+        best_cost = cost;
+        best.pbn = pbn;
+        best.splits = s;
+        best.partial_bytes = s > 1 ? size_t(tiles) * s * 256 * pbn * 4 : 0;
+      }
+    }
+  }
+  return best;
+}
+
+template <int EPI, int PBN, bool A_MN, bool B_MN>
+b2_status launch_gemm(const Maps& maps, const Params& p, cudaStream_t st) {
+  using C = Config<EPI, PBN>;
+  auto kern = gated_kernel<EPI, PBN, A_MN, B_MN>;
+  int dev = 0;
+  B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  static bool configured[64] = {};
+  if (dev < 0 || dev >= 64) return set_error(B2_ERR_INVALID, "device index %d", dev);
+  if (!configured[dev]) {
+    B2_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(C::kSmem)),
+                      "cudaFuncSetAttribute(gated)"));
+    configured[dev] = true;
+  }
+  const int clusters = std::min(p.items, sm_count(dev) / 2);
+  kern<<<2 * clusters, kThreads, C::kSmem, st>>>(maps, p);
+  return check_cuda(cudaGetLastError(), "gated product launch");
+}
+
+// The gate epilogues' tensors.
+struct Gate {
+  int act = 0, train = 0;
+  Mat h, o1, o2;                 // written: h, P, A (kGate) or dg, du (kGateBwd)
+  const uint16_t *fp = nullptr, *fa = nullptr;
+  int64_t ldf = 0;
+};
+
+template <int EPI, bool A_MN, bool B_MN>
+b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial, const Gate* gate, cudaStream_t st) {
+  Maps maps;
+  Params p{};
+  p.problems = n;
+  p.status = device_status_ptr();
+  const int pbn = plan.pbn, bhalf = pbn / 2;
+  uint8_t* part = static_cast<uint8_t*>(partial);
+  for (int i = 0; i < n; ++i) {
+    const Product& x = pr[i];
+    Problem& q = p.p[i];
+    const int cols = EPI == kGate ? pbn / 2 : pbn;
+    q.tiles_m = int((x.M + 255) / 256);
+    q.tiles_n = int((x.N + cols - 1) / cols);
+    q.M = int(x.M);
+    q.N = int(x.N);
+    q.kb_first = int((x.K + BK - 1) / BK);
+    q.kb = q.kb_first * x.pairs;
+    q.splits = plan.splits;
+    q.kb_per_split = (q.kb + q.splits - 1) / q.splits;
+    q.splits = (q.kb + q.kb_per_split - 1) / q.kb_per_split;
+    q.item_begin = p.items;
+    q.out = static_cast<uint16_t*>(x.out);
+    q.ldo = x.ldo;
+    q.tma_out = EPI != kStore || tma_rows(x.out, x.ldo);
+    const int tiles = q.tiles_m * q.tiles_n;
+    if (q.splits > 1) {
+      q.partial = reinterpret_cast<float*>(part);
+      part += size_t(tiles) * q.splits * 256 * pbn * 4;
+    }
+    p.items += tiles * q.splits;
+    const int operands = x.pairs;
+    for (int k = 0; k < operands; ++k) {
+      B2_TRY(A_MN ? map2d(&maps.a[i + k], x.a[k], 64, 64, 128) : map2d(&maps.a[i + k], x.a[k], 64, 128, 128));
+      B2_TRY(B_MN ? map2d(&maps.b[i + k], x.b[k], 64, 64, 128)
+                  : map2d(&maps.b[i + k], x.b[k], 64, uint32_t(bhalf), 128));
+    }
+    if (EPI == kGate) B2_TRY(map2d(&maps.b[1], x.b[1], 64, uint32_t(bhalf), 128));
+    if (EPI == kStore && q.tma_out) B2_TRY(map2d(&maps.o[i], {x.out, x.M, x.N, x.ldo}, 64, 32, 128));
+  }
+  if (EPI != kStore) {
+    p.act = gate->act;
+    p.train = gate->train;
+    p.fp = gate->fp;
+    p.fa = gate->fa;
+    p.ldf = gate->ldf;
+    if (EPI == kGate) B2_TRY(map2d(&maps.o[0], gate->h, 32, 32, 64));
+    if (EPI == kGateBwd || gate->train) {
+      B2_TRY(map2d(&maps.o[1], gate->o1, 32, 32, 64));
+      B2_TRY(map2d(&maps.o[2], gate->o2, 32, 32, 64));
+    }
+  }
+  B2_TRY((pbn == 256 ? launch_gemm<EPI, 256, A_MN, B_MN>(maps, p, st) : launch_gemm<EPI, 128, A_MN, B_MN>(maps, p, st)));
+  for (int i = 0; i < n; ++i) {
+    if (p.p[i].splits <= 1) continue;
+    ReduceArgs r{};
+    r.q = p.p[i];
+    if (EPI != kStore) {
+      r.act = gate->act;
+      r.train = gate->train;
+      r.h = static_cast<uint16_t*>(const_cast<void*>(gate->h.p));
+      r.o1 = static_cast<uint16_t*>(const_cast<void*>(gate->o1.p));
+      r.o2 = static_cast<uint16_t*>(const_cast<void*>(gate->o2.p));
+      r.fp = gate->fp;
+      r.fa = gate->fa;
+      r.ldh = gate->h.ld;
+      r.ldo = gate->o1.ld;
+      r.ldf = gate->ldf;
+    }
+    const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * ((EPI == kGate ? pbn / 2 : pbn) / 8);
+    const unsigned blocks = unsigned(std::min<long long>((units + 7) / 8, 148 * 16));
+    if (pbn == 256)
+      gated_reduce_kernel<EPI, 256><<<blocks, 256, 0, st>>>(r);
+    else
+      gated_reduce_kernel<EPI, 128><<<blocks, 256, 0, st>>>(r);
+    B2_TRY(check_cuda(cudaGetLastError(), "gated reduce launch"));
+  }
+  return B2_OK;
+}
+
+// Carves a workspace; with a null base it only counts.
+struct Carve {
+  uint8_t* base;
+  size_t at = 0;
+  explicit Carve(void* b) : base(static_cast<uint8_t*>(b)) {}
+  void* take(size_t bytes) {
+    void* r = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  }
+};
+
+struct Shape {
+  int64_t M, D, F, E;
+};
+
+// Brings operands into TMA-addressable rows where they are not, in one launch.
+struct Padder {
+  PadArgs a{};
+  void add(Mat& m, Carve& ws) {
+    if (!m.p || m.rows == 0 || m.cols == 0) return;
+    // room is reserved by the shape alone, so that the workspace size does not depend on the pointers
+    if (tma_rows(m.p, m.ld)) return;
+    const int64_t ld = up8(m.cols);
+    void* d = ws.take(size_t(m.rows) * size_t(ld) * 2);
+    const int i = a.n++;
+    a.src[i] = static_cast<const uint16_t*>(m.p);
+    a.dst[i] = static_cast<uint16_t*>(d);
+    a.lds[i] = m.ld;
+    a.rows[i] = int(m.rows);
+    a.cols[i] = int(m.cols);
+    a.ldd[i] = int(ld);
+    a.begin[i + 1] = a.begin[i] + m.rows * (ld / 8);
+    m.p = d;
+    m.ld = ld;
+  }
+  b2_status run(cudaStream_t st) {
+    if (a.n == 0) return B2_OK;
+    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 255) / 256, 148 * 16));
+    gated_pad_kernel<<<blocks, 256, 0, st>>>(a);
+    return check_cuda(cudaGetLastError(), "gated pad launch");
+  }
+};
+
+int current_sms() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
+}
+
+struct FwdPlan {
+  Plan gate, down;
+};
+FwdPlan fwd_plan(const Shape& s, int sms) {
+  return {plan_product(s.M, s.F, s.D, 1, true, sms), plan_product(s.M, s.E, s.F, 1, false, sms)};
+}
+struct BwdPlan {
+  Plan dh, dx, dw;
+};
+BwdPlan bwd_plan(const Shape& s, int sms) {
+  BwdPlan b;
+  b.dh = plan_product(s.M, s.F, s.E, 1, false, sms);
+  b.dx = plan_product(s.M, s.D, s.F, 2, false, sms);
+  // the three weight gradients share one launch: their tiles together
+  b.dw = plan_product(2 * s.F + s.E * s.F / std::max<int64_t>(1, s.D), s.D, s.M, 1, false, sms);
+  return b;
+}
+size_t dw_partial_bytes(const Shape& s, const Plan& p) {
+  if (p.splits <= 1) return 0;
+  auto tiles = [&](int64_t m, int64_t n) { return size_t((m + 255) / 256) * size_t((n + p.pbn - 1) / p.pbn); };
+  return (2 * tiles(s.F, s.D) + tiles(s.E, s.F)) * size_t(p.splits) * 256 * size_t(p.pbn) * 4;
+}
+
+size_t padded_bytes(int64_t rows, int64_t cols) { return size_t(rows) * size_t(up8(cols)) * 2 + 256; }
+
+b2_status check_shape(const char* who, int64_t M, int64_t D, int64_t F, int64_t E, int act) {
+  if (M < 0 || D < 1 || F < 1 || E < 1) return set_error(B2_ERR_INVALID, "%s: bad shape", who);
+  if (act < kSilu || act > kRelu) return set_error(B2_ERR_INVALID, "%s: bad activation %d", who, act);
+  const int64_t big = int64_t(1) << 30;
+  if (M >= big || D >= big || F >= big || E >= big)
+    return set_error(B2_ERR_UNSUPPORTED, "%s: sizes must be below 2^30", who);
+  return B2_OK;
+}
+
+b2_status check_ws(const char* who, size_t need, const void* ws, size_t got) {
+  if (!ws || got < need || reinterpret_cast<uintptr_t>(ws) % 256)
+    return set_error(B2_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need, got);
+  return B2_OK;
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+size_t b2_gated_mlp_fwd_workspace_bytes(int64_t M, int64_t D, int64_t F, int64_t E) {
+  if (M <= 0 || D <= 0 || F <= 0 || E <= 0) return 0;
+  const FwdPlan p = fwd_plan({M, D, F, E}, current_sms());
+  return padded_bytes(M, F) + padded_bytes(M, D) + 2 * padded_bytes(F, D) + padded_bytes(E, F) +
+         std::max(p.gate.partial_bytes, p.down.partial_bytes) + 256;
+}
+
+b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up,
+                                int64_t ldu, const void* w_down, int64_t ldd, int act, void* y, int64_t ldy,
+                                void* saved, int64_t M, int64_t D, int64_t F, int64_t E, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  B2_TRY(check_shape("b2_gated_mlp_fwd_bf16", M, D, F, E, act));
+  if (M == 0) return B2_OK;
+  if (!x || !w_gate || !w_up || !w_down || !y) return set_error(B2_ERR_INVALID, "b2_gated_mlp_fwd_bf16: null pointer");
+  if (ldx < D || ldg < D || ldu < D || ldd < F || ldy < E)
+    return set_error(B2_ERR_INVALID, "b2_gated_mlp_fwd_bf16: bad row stride");
+  if (saved && reinterpret_cast<uintptr_t>(saved) % 16)
+    return set_error(B2_ERR_INVALID, "b2_gated_mlp_fwd_bf16: saved must be 16-byte aligned");
+  B2_TRY(check_ws("b2_gated_mlp_fwd_bf16", b2_gated_mlp_fwd_workspace_bytes(M, D, F, E), workspace, workspace_bytes));
+  const auto st = static_cast<cudaStream_t>(stream);
+  const int sms = current_sms();
+  const FwdPlan plan = fwd_plan({M, D, F, E}, sms);
+  Carve ws(workspace);
+  const int64_t Fp = up8(F);
+  const Mat h = saved ? Mat{saved, M, F, 3 * Fp} : Mat{ws.take(size_t(M) * Fp * 2), M, F, Fp};
+  Mat mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
+  Padder pad;
+  pad.add(mx, ws);
+  pad.add(mg, ws);
+  pad.add(mu, ws);
+  pad.add(md, ws);
+  B2_TRY(pad.run(st));
+  void* partial = ws.take(std::max(plan.gate.partial_bytes, plan.down.partial_bytes));
+  Gate gate;
+  gate.act = act;
+  gate.train = saved != nullptr;
+  gate.h = h;
+  if (saved) {
+    gate.o1 = {static_cast<uint16_t*>(saved) + Fp, M, F, 3 * Fp};
+    gate.o2 = {static_cast<uint16_t*>(saved) + 2 * Fp, M, F, 3 * Fp};
+  }
+  Product up;
+  up.a[0] = mx;
+  up.b[0] = mg;
+  up.b[1] = mu;
+  up.M = M;
+  up.N = F;
+  up.K = D;
+  B2_TRY((run_products<kGate, false, false>(&up, 1, plan.gate, partial, &gate, st)));
+  Product down;
+  down.a[0] = h;
+  down.b[0] = md;
+  down.M = M;
+  down.N = E;
+  down.K = F;
+  down.out = y;
+  down.ldo = ldy;
+  return run_products<kStore, false, false>(&down, 1, plan.down, partial, nullptr, st);
+}
+
+size_t b2_gated_mlp_bwd_workspace_bytes(int64_t M, int64_t D, int64_t F, int64_t E) {
+  if (M <= 0 || D <= 0 || F <= 0 || E <= 0) return 0;
+  const Shape s{M, D, F, E};
+  const BwdPlan p = bwd_plan(s, current_sms());
+  return 2 * padded_bytes(M, F) + padded_bytes(M, D) + padded_bytes(M, E) + 2 * padded_bytes(F, D) +
+         padded_bytes(E, F) +
+         std::max({p.dh.partial_bytes, p.dx.partial_bytes, dw_partial_bytes(s, p.dw)}) + 256;
+}
+
+b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_gate,
+                                int64_t ldg, const void* w_up, int64_t ldu, const void* w_down, int64_t ldd, int act,
+                                const void* saved, void* dx, void* dw_gate, void* dw_up, void* dw_down, int64_t M,
+                                int64_t D, int64_t F, int64_t E, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  B2_TRY(check_shape("b2_gated_mlp_bwd_bf16", M, D, F, E, act));
+  const auto st = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    // no tokens: the weights' gradients are zero
+    void* out[3] = {dw_gate, dw_up, dw_down};
+    for (int i = 0; i < 3; ++i)
+      if (out[i])
+        B2_TRY(check_cuda(cudaMemsetAsync(out[i], 0, size_t(F) * size_t(i < 2 ? D : E) * 2, st), "gradient memset"));
+    return B2_OK;
+  }
+  if (!dy || !x || !w_gate || !w_up || !w_down || !saved)
+    return set_error(B2_ERR_INVALID, "b2_gated_mlp_bwd_bf16: null pointer");
+  if (lddy < E || ldx < D || ldg < D || ldu < D || ldd < F)
+    return set_error(B2_ERR_INVALID, "b2_gated_mlp_bwd_bf16: bad row stride");
+  if (reinterpret_cast<uintptr_t>(saved) % 16)
+    return set_error(B2_ERR_INVALID, "b2_gated_mlp_bwd_bf16: saved must be 16-byte aligned");
+  B2_TRY(check_ws("b2_gated_mlp_bwd_bf16", b2_gated_mlp_bwd_workspace_bytes(M, D, F, E), workspace, workspace_bytes));
+  const Shape s{M, D, F, E};
+  const BwdPlan plan = bwd_plan(s, current_sms());
+  Carve ws(workspace);
+  const int64_t Fp = up8(F);
+  const Mat h{saved, M, F, 3 * Fp};
+  uint16_t* dgu = static_cast<uint16_t*>(ws.take(size_t(M) * Fp * 4));
+  const Mat dg{dgu, M, F, 2 * Fp}, du{dgu + Fp, M, F, 2 * Fp};
+  Mat mdy{dy, M, E, lddy}, mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
+  Padder pad;
+  pad.add(mdy, ws);
+  if (dw_gate || dw_up) pad.add(mx, ws);
+  if (dx) {
+    pad.add(mg, ws);
+    pad.add(mu, ws);
+  }
+  pad.add(md, ws);
+  B2_TRY(pad.run(st));
+  void* partial =
+      ws.take(std::max({plan.dh.partial_bytes, plan.dx.partial_bytes, dw_partial_bytes(s, plan.dw)}));
+  Gate gate;
+  gate.o1 = dg;
+  gate.o2 = du;
+  gate.fp = static_cast<const uint16_t*>(saved) + Fp;
+  gate.fa = gate.fp + Fp;
+  gate.ldf = 3 * Fp;
+  Product t;
+  t.a[0] = mdy;
+  t.b[0] = md;
+  t.M = M;
+  t.N = F;
+  t.K = E;
+  B2_TRY((run_products<kGateBwd, false, true>(&t, 1, plan.dh, partial, &gate, st)));
+  if (dx) {
+    Product d;
+    d.a[0] = dg;
+    d.a[1] = du;
+    d.b[0] = mg;
+    d.b[1] = mu;
+    d.pairs = 2;
+    d.M = M;
+    d.N = D;
+    d.K = F;
+    d.out = dx;
+    d.ldo = D;
+    B2_TRY((run_products<kStore, false, true>(&d, 1, plan.dx, partial, nullptr, st)));
+  }
+  Product w[3];
+  int n = 0;
+  auto weight = [&](void* out, const Mat& a, const Mat& b) {
+    if (!out) return;
+    Product& q = w[n++];
+    q.a[0] = a;  // [M][rows]: the tokens are the reduction
+    q.b[0] = b;
+    q.M = a.cols;
+    q.N = b.cols;
+    q.K = M;
+    q.out = out;
+    q.ldo = b.cols;
+  };
+  weight(dw_gate, dg, mx);
+  weight(dw_up, du, mx);
+  weight(dw_down, mdy, h);
+  if (n == 0) return B2_OK;
+  return run_products<kStore, true, true>(w, n, plan.dw, partial, nullptr, st);
+}
+
+}  // extern "C"

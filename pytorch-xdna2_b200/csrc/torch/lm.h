@@ -36,5 +36,6 @@ inline void no_double_backward(const char* op) {
 
 void bind_embedding(pybind11::module_& m);  // embed_ops.cpp
 void bind_distill(pybind11::module_& m);    // distill_ops.cpp
+void bind_gated(pybind11::module_& m);      // gated_ops.cpp
 
 }  // namespace xdna

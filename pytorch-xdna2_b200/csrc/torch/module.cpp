@@ -446,4 +446,5 @@ PYBIND11_MODULE(_C, m) {
   m.def("region_bn_backward", &region_bn_backward);
   bind_embedding(m);
   bind_distill(m);
+  bind_gated(m);
 }

@@ -126,6 +126,11 @@ SIGNATURES = {
                             sz, vp],
     "b2_distill_loss_bwd": [vp, i64, i32, i64, i64, vp, i64, i32, vp, i64, i32, i64, f32, vp, i32, vp, vp, i32, vp, i64,
                             vp],
+    "b2_gated_mlp_fwd_workspace_bytes": [i64, i64, i64, i64],
+    "b2_gated_mlp_fwd_bf16": [vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, i64, vp, sz, vp],
+    "b2_gated_mlp_bwd_workspace_bytes": [i64, i64, i64, i64],
+    "b2_gated_mlp_bwd_bf16": [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, vp, vp, vp, vp, i64, i64, i64, i64,
+                              vp, sz, vp],
 }
 _RESTYPES = {"b2_last_error": C.c_char_p, "b2_conv3x3_wgrad_workspace_bytes": sz,
              "b2_pack_rows_dbias_workspace_bytes": sz, "b2_region_bn_workspace_bytes": sz,
@@ -133,7 +138,8 @@ _RESTYPES = {"b2_last_error": C.c_char_p, "b2_conv3x3_wgrad_workspace_bytes": sz
              "b2_batch_norm_workspace_bytes": sz, "b2_channel_sum_nhwc_workspace_bytes": sz,
              "b2_gemm_bf16_workspace_bytes": sz,
              "b2_conv3x3_wgrad_noalloc_max_bytes": sz, "b2_embedding_bwd_workspace_bytes": sz,
-             "b2_distill_workspace_bytes": sz}
+             "b2_distill_workspace_bytes": sz, "b2_gated_mlp_fwd_workspace_bytes": sz,
+             "b2_gated_mlp_bwd_workspace_bytes": sz}
 
 
 class B2Error(RuntimeError):

@@ -1,8 +1,9 @@
-"""Operators of language models on the xdna device: token embedding and the
-distillation loss.
+"""Operators of language models on the xdna device: token embedding, the gated
+feed-forward block and the distillation loss.
 
 Each function is one differentiable operator with its own sm_100a kernels
-(``b2_embedding_*``, ``b2_distill_*`` in ``include/b2.h``).  The reference has
+(``b2_embedding_*``, ``b2_gated_mlp_*``, ``b2_distill_*`` in
+``include/b2.h``).  The reference has
 no counterpart.  Their tensors live on one ``xdna`` device
 (``xdna_train.as_xdna`` brings a CUDA tensor there without a copy) and the work
 runs on its current stream.  On CPU tensors, and with ``set_npu_mode(0)``, the
@@ -17,8 +18,9 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-__all__ = ["embedding", "distill_loss"]
+__all__ = ["embedding", "gated_mlp", "distill_loss"]
 
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
@@ -46,6 +48,30 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         y = F.embedding(ids, weight, padding_idx)
         return y if scale == 1.0 else (y.float() * scale).to(weight.dtype)
     return C.lm_embedding(ids, weight, float(scale), -1 if padding_idx is None else int(padding_idx))
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              activation: str = "silu") -> torch.Tensor:
+    """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T``.
+
+    ``x`` ``[..., D]``, ``w_gate`` and ``w_up`` ``[F, D]``, ``w_down``
+    ``[E, F]`` (as ``nn.Linear`` keeps them), all bfloat16; the result is
+    ``[..., E]``.  ``activation``: ``"silu"``, ``"gelu"`` (erf form) or
+    ``"relu"``.  Sums are fp32; the hidden tensor is rounded to bfloat16
+    between the products, and the backward keeps it and the two factors
+    ``act(gate)`` and ``up * act'(gate)`` in bfloat16.  Inside ``torch.autocast("xdna")`` other
+    floating-point arguments are cast first, as for a matrix product."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"gated_mlp: activation must be one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
+    C = _native(x)
+    if C is None:
+        return F.linear(_ACT[activation](F.linear(x, w_gate)) * F.linear(x, w_up), w_down)
+    if torch.is_autocast_enabled("xdna"):
+        x, w_gate, w_up, w_down = (t.to(torch.bfloat16) for t in (x, w_gate, w_up, w_down))
+    return C.lm_gated_mlp(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
+
+
+_ACT = {"silu": F.silu, "gelu": F.gelu, "relu": F.relu}
 
 
 def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,

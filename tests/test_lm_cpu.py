@@ -53,8 +53,25 @@ def test_distill_loss_masks_on_cpu():
     assert loss.isfinite() and dz.isfinite().all() and not dz[1].any()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_mlp_on_cpu(act):
+    g = torch.Generator().manual_seed(1)
+    x, wg, wu, wd = (torch.randn(*s, generator=g) for s in ((2, 3, 5), (7, 5), (7, 5), (4, 7)))
+    fn = getattr(torch.nn.functional, act)
+    assert torch.allclose(lm.gated_mlp(x, wg, wu, wd, act), (fn(x @ wg.t()) * (x @ wu.t())) @ wd.t(), atol=1e-5)
+    with pytest.raises(ValueError, match="activation"):
+        lm.gated_mlp(x, wg, wu, wd, "tanh")
+
+
 def test_argument_errors_need_no_gpu():
     L = _abi.lib()
+    assert L.b2_gated_mlp_fwd_bf16(8, 16, 8, 16, 8, 16, 8, 24, 3, 8, 8, None, 4, 16, 24, 8, 8, 0, None) == 1
+    assert b"activation" in L.b2_last_error()
+    assert L.b2_gated_mlp_fwd_bf16(8, 15, 8, 16, 8, 16, 8, 24, 0, 8, 8, None, 4, 16, 24, 8, 8, 0, None) == 1
+    assert b"row stride" in L.b2_last_error()
+    assert L.b2_gated_mlp_fwd_bf16(256, 16, 8, 16, 8, 16, 8, 24, 0, 8, 8, None, 4, 16, 24, 8, 256, 0, None) == 5
+    assert L.b2_gated_mlp_bwd_bf16(8, 8, 8, 16, 8, 16, 8, 16, 8, 24, 0, None, 8, 8, 8, 8, 4, 16, 24, 8, 8, 0, None) == 1
+    assert b"null pointer" in L.b2_last_error()
     assert L.b2_embedding_fwd(None, _abi.B2_I64, 3, None, 8, _abi.B2_F32, 5, 8, 1.0, None, None) == 1
     assert b"null pointer" in L.b2_last_error()
     assert L.b2_embedding_fwd(8, _abi.B2_F32, 3, 8, 8, _abi.B2_F32, 5, 8, 1.0, 8, None) == 1
