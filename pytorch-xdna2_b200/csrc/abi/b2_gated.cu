@@ -67,11 +67,7 @@ struct Maps {
 struct Params {
   Problem p[kMaxProblems];
   int problems, items;
-  int act;
-  // the factors P and A: kGate writes them if train, kGateBwd reads them
-  int train;
-  const uint16_t *fp, *fa;
-  long long ldf;
+  int train;  // kGate: write the factors P and A (kGateBwd reads them through maps.a[1] and maps.b[1])
   int* status;
 };
 
@@ -84,18 +80,17 @@ __device__ __forceinline__ uint16_t cvt1(float v) {
   return *reinterpret_cast<uint16_t*>(&h);
 }
 
-// act(g) and act'(g)
-__device__ __forceinline__ float act_value(int act, float g) {
-  if (act == kSilu) return __fdividef(g, 1.f + __expf(-g));
-  if (act == kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-  return g > 0.f || g != g ? g : 0.f;
-}
-__device__ __forceinline__ void act_both(int act, float g, float& a, float& slope) {
-  if (act == kSilu) {
+// act(g) and act'(g).  The activation is a template argument of every kernel
+// that needs it: chosen at run time inside the unrolled element loops it put
+// all three into them, and the epilogue of a 256-wide tile took 8 us instead of
+// its 3.
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& a, float& slope) {
+  if constexpr (ACT == kSilu) {
     const float s = __fdividef(1.f, 1.f + __expf(-g));
     a = g * s;
     slope = s * (1.f + g * (1.f - s));
-  } else if (act == kGelu) {
+  } else if constexpr (ACT == kGelu) {
     const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     a = g * cdf;
     slope = cdf + g * 0.39894228040143268f * __expf(-0.5f * g * g);
@@ -103,6 +98,12 @@ __device__ __forceinline__ void act_both(int act, float g, float& a, float& slop
     a = g > 0.f || g != g ? g : 0.f;
     slope = g > 0.f ? 1.f : 0.f;
   }
+}
+template <int ACT>
+__device__ __forceinline__ float act_value(float g) {
+  float a, slope;
+  act_both<ACT>(g, a, slope);
+  return a;
 }
 
 template <int EPI, int PBN>
@@ -112,7 +113,7 @@ struct Config {
   // per epilogue warp: kStore two 32 x 64 boxes, kGate three 32 x 32 boxes, kGateBwd two pairs of 32 x 32 boxes
   static constexpr int kEpiBytes = EPI == kGate ? 3 * 2048 : 2 * 4096;
   static constexpr int kStages = PBN == 256 ? 5 : (EPI == kGate ? 7 : 6);
-  static constexpr size_t kSmem = size_t(kStages) * kStage + kEpiWarps * kEpiBytes + 1024 + 256;
+  static constexpr size_t kSmem = size_t(kStages) * kStage + kEpiWarps * kEpiBytes + 1024 + 512;
 };
 
 struct Item {
@@ -150,38 +151,38 @@ __device__ __forceinline__ float4* partial_at(const Problem& q, int tile, int sp
          ((((long long)tile * q.splits + split) * 16 + region) * (PBN / 64) + j) * 256 + lane;
 }
 
-// 32 columns of one row of the factors P and A.  Their rows hold a multiple of
-// 8 columns, so a 16-byte load that starts below N stays inside the row.
-struct Factors {
-  uint32_t v[2][16];
-  __device__ __forceinline__ void load(const Params& p, int row, int c0, int N, int M) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint4 a = make_uint4(0, 0, 0, 0), b = a;
-      if (row < M && c0 + c * 8 < N) {
-        a = *reinterpret_cast<const uint4*>(p.fp + (long long)row * p.ldf + c0 + c * 8);
-        b = *reinterpret_cast<const uint4*>(p.fa + (long long)row * p.ldf + c0 + c * 8);
-      }
-      v[0][4 * c] = a.x;
-      v[0][4 * c + 1] = a.y;
-      v[0][4 * c + 2] = a.z;
-      v[0][4 * c + 3] = a.w;
-      v[1][4 * c] = b.x;
-      v[1][4 * c + 1] = b.y;
-      v[1][4 * c + 2] = b.z;
-      v[1][4 * c + 3] = b.w;
-    }
-  }
-};
+// Programmatic dependence: `wait` returns when the kernels before this one in
+// the stream have ended and their writes are visible, `release` lets the next
+// one be set up.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// 32 bf16 columns (packed in pairs) of this thread's row, elementwise
-__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&v)[16], int cols) {
-#pragma unroll
-  for (int c = 0; c < 32; ++c)
-    if (c < cols) dst[c] = uint16_t((c & 1) ? (v[c >> 1] >> 16) : (v[c >> 1] & 0xffff));
+// A staged 32 x 64 box (128-byte rows, chunk c of row r at c ^ (r & 7)) to output
+// rows that no TMA store can address: the warp writes row after row, 4-byte
+// words in consecutive lanes where the row's parity allows, so that a row's 128
+// bytes are one access (a thread writing its own row's elements took 17 us a
+// tile).  All lanes call; cols, rows: what is inside the output.
+__device__ __forceinline__ void store_box_rows(const uint8_t* box, uint16_t* dst, long long ld, int rows, int cols,
+                                               int lane) {
+  auto at = [&](int r, int c) {
+    return *reinterpret_cast<const uint16_t*>(box + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+  };
+  rows = min(rows, 32);
+  cols = min(cols, 64);
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    uint16_t* d = dst + r * ld;
+    const int odd = int(reinterpret_cast<uintptr_t>(d) >> 1) & 1;
+    const int c = 2 * lane + odd;
+    if (c + 1 < cols)
+      *reinterpret_cast<uint32_t*>(d + c) = uint32_t(at(r, c)) | (uint32_t(at(r, c + 1)) << 16);
+    else if (c < cols)
+      d[c] = at(r, c);
+    if (odd && lane == 31) d[0] = at(r, 0);
+  }
 }
 
-template <int EPI, int PBN, bool A_MN, bool B_MN>
+template <int EPI, int PBN, bool A_MN, bool B_MN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gated_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C = Config<EPI, PBN>;
@@ -198,7 +199,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* tfull = bars + 2 * STAGES;
   uint64_t* tempty = tfull + 2;
   uint64_t* mma_done = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* factor_bars = mma_done + 1;  // kGateBwd: two per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(factor_bars + 2 * kEpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32;
@@ -218,18 +220,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&tempty[a]), 2 * kEpiWarps);
     }
     mbar_init(smem_u32(mma_done), 1);
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(smem_u32(&factor_bars[i]), 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
     tmem_relinquish_pair();
+  } else if (warp == 0 && lane < 4) {
+    // the tensor maps travel while the barriers are set up
+    const bool two = EPI != kStore || p.problems > 1 || p.p[0].kb > p.p[0].kb_first;
+    if (lane < (two ? 2 : 1)) tma_prefetch_desc(&maps.a[EPI == kGate ? 0 : lane]);
+    if (lane < (two ? 2 : 1)) tma_prefetch_desc(&maps.b[lane]);
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers initialized before any cross-CTA signal
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  chain_wait();
+  chain_release();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -345,6 +355,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
     uint8_t* buf = epi_stage + (warp - 2) * C::kEpiBytes;
     int sel = 0;
+    uint64_t* factor_bar = factor_bars + (warp - 2) * 2;  // one per box pair
+    int factor_phase = 0;
+    // loads a 32 x 32 box of P and one of A into box pair `which`, once the last store from it has read it
+    auto fetch_factors = [&](int c0, int row, int which) {
+      if (lane == 0) {
+        bulk_wait_read<0>();
+        const uint32_t bar = smem_u32(&factor_bar[which]);
+        mbar_arrive_expect_tx(bar, 4096);
+        tma_load_3d(smem_u32(buf + which * 4096), &maps.a[1], bar, c0, row, 0);
+        tma_load_3d(smem_u32(buf + which * 4096 + 2048), &maps.b[1], bar, c0, row, 0);
+      }
+      __syncwarp();
+    };
+    (void)factor_phase;
+    (void)fetch_factors;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = cluster; t < p.items; t += nclusters) {
@@ -352,13 +377,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Problem& q = p.p[it.prob];
       const int row0 = it.mt * 256 + int(rank) * 128 + quarter * 32;
       const int row = row0 + lane;
-      // the first factors of the tile travel while its product is still running
-      Factors factors;
-      if constexpr (EPI == kGateBwd)
-        if (q.splits == 1) factors.load(p, row, it.nt * PBN + half * (PBN / 2), q.N, q.M);
+      // kGateBwd: this warp's 32-column chunks of the tile; the first one's
+      // factors travel while its product is still running
+      int chunks = 0;
+      if constexpr (EPI == kGateBwd) {
+        const int f0 = it.nt * PBN + half * (PBN / 2);
+        if (q.splits == 1 && row0 < q.M && f0 < q.N) chunks = min(PBN / 64, (q.N - f0 + 31) / 32);
+        if (chunks > 0) fetch_factors(f0, row0, sel);
+      }
       bool ok = mbar_wait(smem_u32(&tfull[acc]), acc_phase, p.status, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!ok) {  // the factors on their way land before the CTA goes away
+        if (chunks > 0) mbar_wait(smem_u32(&factor_bar[sel]), uint32_t(factor_phase >> sel) & 1u, p.status, nullptr);
+        break;
+      }
       tc_fence_after();
       const uint32_t tacc = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * PBN);
       const uint32_t thalf = tacc + uint32_t(half * (PBN / 2));
@@ -377,52 +409,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       } else if constexpr (EPI == kStore) {
-        if (q.tma_out) {
-          // Boxes of 32 rows x 64 columns staged with the tensor map's 128-byte
-          // swizzle (16-byte chunk c of row r at chunk c ^ (r & 7): the eight
-          // rows of a store phase hit distinct banks) and written by the TMA
-          // unit in whole rows, clipped at M and N; one box fills while the
-          // other's store reads it.
+        // Boxes of 32 rows x 64 columns staged with the tensor map's 128-byte
+        // swizzle (16-byte chunk c of row r at chunk c ^ (r & 7): the eight
+        // rows of a store phase hit distinct banks) and written by the TMA
+        // unit in whole rows, clipped at M and N; one box fills while the
+        // other's store reads it.
 #pragma unroll 1
-          for (int j = 0; j < PBN / 128; ++j) {
-            const int c0 = it.nt * PBN + half * (PBN / 2) + j * 64;
-            if (c0 >= q.N || row0 >= q.M) break;
-            uint32_t r[2][32];
-            tmem_ld32(thalf + j * 64, r[0]);
-            tmem_ld32(thalf + j * 64 + 32, r[1]);
-            tc_wait_ld();
-            if (lane == 0) bulk_wait_read<1>();
-            __syncwarp();
-            uint8_t* box = buf + sel * 4096;
+        for (int j = 0; j < PBN / 128; ++j) {
+          const int c0 = it.nt * PBN + half * (PBN / 2) + j * 64;
+          if (c0 >= q.N || row0 >= q.M) break;
+          uint32_t r[2][32];
+          tmem_ld32(thalf + j * 64, r[0]);
+          tmem_ld32(thalf + j * 64 + 32, r[1]);
+          tc_wait_ld();
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+          uint8_t* box = buf + sel * 4096;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t* v = &r[c >> 2][(c & 3) * 8];
-              *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_uint4(cvt2(__uint_as_float(v[0]), __uint_as_float(v[1])),
-                             cvt2(__uint_as_float(v[2]), __uint_as_float(v[3])),
-                             cvt2(__uint_as_float(v[4]), __uint_as_float(v[5])),
-                             cvt2(__uint_as_float(v[6]), __uint_as_float(v[7])));
-            }
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t* v = &r[c >> 2][(c & 3) * 8];
+            *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                make_uint4(cvt2(__uint_as_float(v[0]), __uint_as_float(v[1])),
+                           cvt2(__uint_as_float(v[2]), __uint_as_float(v[3])),
+                           cvt2(__uint_as_float(v[4]), __uint_as_float(v[5])),
+                           cvt2(__uint_as_float(v[6]), __uint_as_float(v[7])));
+          }
+          if (q.tma_out) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
               tma_store_3d(&maps.o[it.prob], smem_u32(box), c0, row0, 0);
               bulk_commit();
             }
-            sel ^= 1;
+          } else {
+            __syncwarp();
+            store_box_rows(box, q.out + (long long)row0 * q.ldo + c0, q.ldo, q.M - row0, q.N - c0, lane);
           }
-        } else {
-          // output rows that no 16-byte store can address: element by element
-#pragma unroll 1
-          for (int j = 0; j < PBN / 64; ++j) {
-            const int c0 = it.nt * PBN + half * (PBN / 2) + j * 32;
-            uint32_t r[32], v[16];
-            tmem_ld32(thalf + j * 32, r);
-            tc_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 16; ++c) v[c] = cvt2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-            if (row < q.M) store_row32(q.out + (long long)row * q.ldo + c0, v, min(32, q.N - c0));
-          }
+          sel ^= 1;
         }
       } else {
         // gate epilogues: 32 hidden units at a time, staged in 32 x 32 boxes
@@ -432,6 +455,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
                 make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        };
+        auto read = [&](const uint8_t* box, uint32_t (&v)[16]) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
+            v[4 * c] = w.x;
+            v[4 * c + 1] = w.y;
+            v[4 * c + 2] = w.z;
+            v[4 * c + 3] = w.w;
+          }
         };
         if constexpr (EPI == kGate) {
           const int f0 = it.nt * (PBN / 2) + half * (PBN / 4);
@@ -452,8 +485,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               for (int c = 0; c < 16; ++c) {
                 const float u0 = __uint_as_float(u[2 * c]), u1 = __uint_as_float(u[2 * c + 1]);
                 float a0, s0, a1, s1;
-                act_both(p.act, __uint_as_float(g[2 * c]), a0, s0);
-                act_both(p.act, __uint_as_float(g[2 * c + 1]), a1, s1);
+                act_both<ACT>(__uint_as_float(g[2 * c]), a0, s0);
+                act_both<ACT>(__uint_as_float(g[2 * c + 1]), a1, s1);
                 h[c] = cvt2(a0 * u0, a1 * u1);
                 fp[c] = cvt2(s0 * u0, s1 * u1);
                 fa[c] = cvt2(a0, a1);
@@ -463,8 +496,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             } else {
 #pragma unroll
               for (int c = 0; c < 16; ++c)
-                h[c] = cvt2(act_value(p.act, __uint_as_float(g[2 * c])) * __uint_as_float(u[2 * c]),
-                            act_value(p.act, __uint_as_float(g[2 * c + 1])) * __uint_as_float(u[2 * c + 1]));
+                h[c] = cvt2(act_value<ACT>(__uint_as_float(g[2 * c])) * __uint_as_float(u[2 * c]),
+                            act_value<ACT>(__uint_as_float(g[2 * c + 1])) * __uint_as_float(u[2 * c + 1]));
             }
             fill(buf, h);
             fence_proxy_async_smem();
@@ -481,28 +514,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         } else {
           const int f0 = it.nt * PBN + half * (PBN / 2);
 #pragma unroll 1
-          for (int j = 0; j < PBN / 64; ++j) {
+          for (int j = 0; j < chunks; ++j) {
             const int c0 = f0 + j * 32;
-            if (c0 >= q.N || row0 >= q.M) break;
-            uint32_t pv[16], av[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              pv[c] = factors.v[0][c];
-              av[c] = factors.v[1][c];
-            }
-            factors.load(p, row, c0 + 32, j + 1 < PBN / 64 ? q.N : 0, q.M);
+            // the other box pair takes the next chunk's factors
+            if (j + 1 < chunks) fetch_factors(c0 + 32, row0, sel ^ 1);
+            ok = mbar_wait(smem_u32(&factor_bar[sel]), uint32_t(factor_phase >> sel) & 1u, p.status, abort_flag);
+            factor_phase ^= 1 << sel;
             uint32_t d[32];
             tmem_ld32(thalf + j * 32, d);
             tc_wait_ld();
+            uint8_t* box = buf + sel * 4096;
+            uint32_t pv[16], av[16];
+            read(box, pv);
+            read(box + 2048, av);
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               const float d0 = __uint_as_float(d[2 * c]), d1 = __uint_as_float(d[2 * c + 1]);
               pv[c] = cvt2(d0 * __uint_as_float(pv[c] << 16), d1 * __uint_as_float(pv[c] & 0xffff0000u));
               av[c] = cvt2(d0 * __uint_as_float(av[c] << 16), d1 * __uint_as_float(av[c] & 0xffff0000u));
             }
-            if (lane == 0) bulk_wait_read<1>();
-            __syncwarp();
-            uint8_t* box = buf + sel * 4096;
+            // a lane writes its results over the factors that it read
             fill(box, pv);
             fill(box + 2048, av);
             fence_proxy_async_smem();
@@ -545,7 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // lanes of a warp are 32 rows, so its partial reads are contiguous.
 struct ReduceArgs {
   Problem q;
-  int act, train;
+  int train;
   uint16_t *h, *o1, *o2;           // kGate: h, P, A; kGateBwd: -, dg, du
   const uint16_t *fp, *fa;
   long long ldh, ldo, ldf;
@@ -580,8 +611,9 @@ __device__ __forceinline__ void put8(uint16_t* dst, const float (&v)[8], int col
     if (i < cols) dst[i] = cvt1(v[i]);
 }
 
-template <int EPI, int PBN>
+template <int EPI, int PBN, int ACT>
 __global__ void __launch_bounds__(256) gated_reduce_kernel(const __grid_constant__ ReduceArgs a) {
+  chain_wait();
   const Problem& q = a.q;
   constexpr int kCols = EPI == kGate ? PBN / 2 : PBN;  // output columns of a tile
   constexpr int kOcts = kCols / 8;
@@ -609,7 +641,7 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(const __grid_constant
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float act, slope;
-        act_both(a.act, g[i], act, slope);
+        act_both<ACT>(g[i], act, slope);
         h[i] = act * v[i];
         v[i] *= slope;
         g[i] = act;
@@ -643,6 +675,20 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(const __grid_constant
   }
 }
 
+// 16 bytes that start `shift` bits (a multiple of 16) into the 32 bytes lo, hi.
+__device__ __forceinline__ uint4 shift_words(const uint4& lo, const uint4& hi, int shift) {
+  const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  const int words = shift >> 5, bits = shift & 31;
+  uint32_t o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t x = words == 0 ? v[e] : words == 1 ? v[e + 1] : words == 2 ? v[e + 2] : v[e + 3];
+    const uint32_t y = words == 0 ? v[e + 1] : words == 1 ? v[e + 2] : words == 2 ? v[e + 3] : v[e + 4];
+    o[e] = __funnelshift_r(x, y, bits);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 // Copies of matrices whose rows no TMA map can address (a row stride that is
 // not a multiple of 16 bytes, or a misaligned base) into rows that one can.
 struct PadArgs {
@@ -654,19 +700,271 @@ struct PadArgs {
   int n;
 };
 __global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ PadArgs a) {
+  chain_wait();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.begin[a.n]; i += (long long)gridDim.x * 256) {
     int m = 0;
     while (i >= a.begin[m + 1]) ++m;
-    const long long at = i - a.begin[m];
-    const int groups = a.ldd[m] / 8;
+    const unsigned at = unsigned(i - a.begin[m]);  // below 2^31 groups of a matrix (checked by the host)
+    const unsigned groups = unsigned(a.ldd[m]) / 8;
     const long long row = at / groups;
-    const int col = int(at - row * groups) * 8;
+    const int col = int(at - unsigned(row) * groups) * 8;
     const uint16_t* s = a.src[m] + row * a.lds[m] + col;
-    uint16_t v[8];
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(s);
+    const int shift = int(addr & 15) * 8;  // bits
+    uint4 out;
+    // the two aligned 16-byte words around the 8 elements, where both lie inside this row
+    if (col >= 8 && col + 16 <= a.cols[m]) {
+      const uint4* w = reinterpret_cast<const uint4*>(addr & ~uintptr_t(15));
+      const uint4 lo = w[0];
+      const uint4 hi = shift ? w[1] : lo;
+      out = shift_words(lo, hi, shift);
+    } else {
+      uint16_t v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = col + e < a.cols[m] ? s[e] : uint16_t(0);
-    *reinterpret_cast<uint4*>(a.dst[m] + row * a.ldd[m] + col) = *reinterpret_cast<uint4*>(v);
+      for (int e = 0; e < 8; ++e) v[e] = col + e < a.cols[m] ? s[e] : uint16_t(0);
+      out = *reinterpret_cast<uint4*>(v);
+    }
+    *reinterpret_cast<uint4*>(a.dst[m] + row * a.ldd[m] + col) = out;
   }
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens (M <= kFewTokens): reading the weights once is everything, and a
+// 256-row tile per token would idle most of the machine.  A CTA takes 16 weight
+// rows (kGate: of Wg and of Wu), its 4 warps interleave the reduction in steps
+// of 32, and a cluster of up to 8 CTAs shares a reduction where there are few
+// rows.  The products run on mma.sync m16n8k16 with the weights as the 16-row
+// operand and the tokens as the columns: a lane's 16-byte load of a weight row
+// holds 8 consecutive k, which two instructions take in an order of their own
+// (the same for both operands, so the sum is the same); weights go from memory
+// straight to registers, a batch of U steps ahead of the products.  Partial
+// sums are added in warp and CTA order.
+// ---------------------------------------------------------------------------
+constexpr int kFewThreads = 128;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kFewPerSm = 4;   // resident CTAs a SM
+constexpr int kFewTokens = 32;
+
+struct FewMat {
+  const uint16_t* p;
+  const uint16_t* end;  // one past the last element
+  long long ld;
+  int aligned;          // every row starts at 16 bytes
+};
+struct FewArgs {
+  FewMat w[2];   // kGate: Wg, Wu; kStore: Wd
+  FewMat x;      // [M][K]
+  int M, rows, K;
+  int early;     // the weights were not written by the kernel before this one
+  uint16_t *out, *o1, *o2;  // kGate: h, P, A (or null); kStore: y
+  long long ldo;            // of all of them
+};
+
+// 8 consecutive elements of a weight row from k, zeros from K on: in one
+// aligned word, or (ALIGNED false) in the two aligned words around them, to be
+// shifted together when they are used -- a shift at the load would wait for it.
+template <bool ALIGNED>
+struct RowWord;
+template <>
+struct RowWord<true> {
+  uint4 lo;
+  __device__ __forceinline__ void clear() { lo = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const FewMat&, const uint16_t* row, int k, int K) {
+    if (k + 8 <= K) {
+      lo = __ldg(reinterpret_cast<const uint4*>(row + k));
+    } else {
+      clear();
+      uint16_t* e = reinterpret_cast<uint16_t*>(&lo);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < K) e[i] = row[k + i];
+    }
+  }
+  __device__ __forceinline__ uint4 get(int) const { return lo; }
+};
+template <>
+struct RowWord<false> {
+  uint4 lo, hi;
+  __device__ __forceinline__ void clear() { lo = hi = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const FewMat& m, const uint16_t* row, int k, int K) {
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(row + k);
+    const uint4* w = reinterpret_cast<const uint4*>(addr & ~uintptr_t(15));
+    const uint16_t* first = reinterpret_cast<const uint16_t*>(w);
+    if (k + 8 <= K && first >= m.p && first + 16 <= m.end) {
+      lo = __ldg(w);
+      hi = __ldg(w + 1);
+    } else {  // at the ends of the row or the matrix: what is inside, element by element
+      clear();
+      uint16_t *l = reinterpret_cast<uint16_t*>(&lo), *h = reinterpret_cast<uint16_t*>(&hi);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (first + i >= row + k && first + i < row + K) l[i] = first[i];
+        if (first + 8 + i < row + K) h[i] = first[8 + i];
+      }
+    }
+  }
+  __device__ __forceinline__ uint4 get(int shift) const { return shift_words(lo, hi, shift); }
+};
+
+// The tokens' operand is read from L2: until chain_wait the kernel before may
+// be writing it.
+__device__ __forceinline__ uint4 load_tokens(const FewMat& m, const uint16_t* row, int k, int K) {
+  if (m.aligned && k + 8 <= K) return __ldcg(reinterpret_cast<const uint4*>(row + k));
+  union {
+    uint4 v;
+    uint16_t e[8];
+  } r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.e[i] = k + i < K ? __ldcg(row + k + i) : uint16_t(0);
+  return r.v;
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int EPI, int NT, int ACT, bool ALIGNED>
+__global__ void __launch_bounds__(kFewThreads, kFewPerSm) gated_few_kernel(const __grid_constant__ FewArgs a,
+                                                                           int cluster) {
+  constexpr int kMats = EPI == kGate ? 2 : 1;
+  // steps whose loads are in flight together
+  constexpr int U = (NT <= 2 ? 4 : 2) / (ALIGNED || EPI == kStore ? 1 : 2);
+  constexpr int kOut = 16 * 8 * NT;   // sums per matrix
+  __shared__ float red[kFewWarps][kMats][kOut];
+  __shared__ float total[kMats][kOut];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, q = lane & 3;
+  const int rank = cluster > 1 ? int(cluster_ctarank()) : 0;
+  const int row0 = (blockIdx.x / cluster) * 16;
+  const uint16_t* wrow[kMats][2];
+  bool live[2];
+  int shift[kMats][2];
+  int k0 = (rank * kFewWarps + warp) * 32 + q * 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    live[i] = row0 + g + 8 * i < a.rows;
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) {
+      wrow[m][i] = a.w[m].p + (long long)(live[i] ? row0 + g + 8 * i : row0) * a.w[m].ld;
+      shift[m][i] = int(reinterpret_cast<uintptr_t>(wrow[m][i] + k0) & 15) * 8;  // the same at every step
+    }
+  }
+  const uint16_t* xrow[NT];
+  bool xlive[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    xlive[n] = n * 8 + g < a.M;
+    xrow[n] = a.x.p + (long long)(xlive[n] ? n * 8 + g : 0) * a.x.ld;
+  }
+  float c[kMats][NT][4];
+#pragma unroll
+  for (int m = 0; m < kMats; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[m][n][i] = 0.f;
+  const int stride = kFewWarps * cluster * 32;
+  RowWord<ALIGNED> wv[U][kMats][2];
+  uint4 xv[U][NT];
+  auto load_w = [&](int k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < kMats; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int at = k + u * stride;
+          if (at < a.K && live[i])
+            wv[u][m][i].load(a.w[m], wrow[m][i], at, a.K);
+          else
+            wv[u][m][i].clear();
+        }
+  };
+  auto load_x = [&](int k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int at = k + u * stride;
+        xv[u][n] = make_uint4(0, 0, 0, 0);
+        if (at < a.K && xlive[n]) xv[u][n] = load_tokens(a.x, xrow[n], at, a.K);
+      }
+  };
+  if (!a.early) chain_wait();
+  chain_release();
+  load_w(k0);
+  if (a.early) chain_wait();  // the tokens' operand comes from the kernel before
+  load_x(k0);
+  for (; k0 - q * 8 < a.K; k0 += U * stride) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < kMats; ++m) {
+        const uint4 w0 = wv[u][m][0].get(shift[m][0]), w1 = wv[u][m][1].get(shift[m][1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816(c[m][n], w0.x, w1.x, w0.y, w1.y, xv[u][n].x, xv[u][n].y);
+          mma16816(c[m][n], w0.z, w1.z, w0.w, w1.w, xv[u][n].z, xv[u][n].w);
+        }
+      }
+    load_w(k0 + U * stride);
+    load_x(k0 + U * stride);
+  }
+#pragma unroll
+  for (int m = 0; m < kMats; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        red[warp][m][(n * 8 + 2 * q + (i & 1)) * 16 + g + 8 * (i >> 1)] = c[m][n][i];
+  __syncthreads();
+  for (int t = threadIdx.x; t < kMats * kOut; t += kFewThreads) {
+    const int m = t / kOut, o = t % kOut;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) v += red[w][m][o];
+    total[m][o] = v;
+  }
+  if (cluster > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (rank == 0) {
+    for (int t = threadIdx.x; t < kOut; t += kFewThreads) {
+      const int row = row0 + (t & 15), token = t >> 4;
+      float v[kMats];
+#pragma unroll
+      for (int m = 0; m < kMats; ++m) {
+        v[m] = total[m][t];
+        for (int r = 1; r < cluster; ++r) {
+          float o;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                       : "=f"(o)
+                       : "r"(mapa_shared(smem_u32(&total[m][t]), uint32_t(r)))
+                       : "memory");
+          v[m] += o;
+        }
+      }
+      if (row >= a.rows || token >= a.M) continue;
+      const long long at = (long long)token * a.ldo + row;
+      if constexpr (EPI == kGate) {
+        float act, slope;
+        act_both<ACT>(v[0], act, slope);
+        a.out[at] = cvt1(act * v[1]);
+        if (a.o1) {
+          a.o1[at] = cvt1(slope * v[1]);
+          a.o2[at] = cvt1(act);
+        }
+      } else {
+        a.out[at] = cvt1(v[0]);
+      }
+    }
+  }
+  if (cluster > 1) cluster_sync();  // no CTA leaves while the first may read it
 }
 
 // ---------------------------------------------------------------------------
@@ -707,9 +1005,10 @@ struct Plan {
 
 // Tile width and reduction splits of a product.  Cost in SM clocks of a pair
 // on its busiest pair: a k-block of a 256-wide tile takes 512 clocks of the
-// tensor pipe, of a 128-wide one 256 but about 400 to bring its operands from
-// L2; each tile adds a pipeline fill and drain; a split adds writing and
-// reading the fp32 partials and the second kernel.
+// tensor pipe but about 800 to bring its operands from L2 when the clock is high
+// (32 KB at 41 bytes a clock and SM; 24 KB of a 128-wide one: 600); each tile
+// adds a pipeline fill and drain; a split adds writing and reading the fp32
+// partials and the second kernel.
 Plan plan_product(int64_t M, int64_t N, int64_t K, int pairs, bool gate, int sms) {
   const int clusters = std::max(1, sms / 2);
   const int64_t kb = (K + BK - 1) / BK * pairs;
@@ -724,8 +1023,10 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int pairs, bool gate, int sms
       const int64_t splits = (kb + kps - 1) / kps;
       if (splits != s) continue;
       const int64_t waves = (tiles * s + clusters - 1) / clusters;
-      double cost = double(waves) * (double(kps) * (pbn == 256 ? 512 : 400) + 800) + 2500;
-      if (s > 1) cost += 4000 + double(tiles) * 256 * pbn * 4 * s * 2 / 2500.0;
+      double cost = double(waves) * (double(kps) * (pbn == 256 ? 800 : 600) + 800) + 2500;
+      // the epilogue writes the 32-row blocks that hold tokens
+      const double rows = std::min<double>(double(M + 31) / 32 * 32, double((M + 255) / 256 * 256));
+      if (s > 1) cost += 4000 + double(tiles) / double((M + 255) / 256) * rows * pbn * 4 * s * 2 / 2500.0;
       if (cost < best_cost) {
         best_cost = cost;
         best.pbn = pbn;
@@ -737,10 +1038,30 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int pairs, bool gate, int sms
   return best;
 }
 
-template <int EPI, int PBN, bool A_MN, bool B_MN>
+// Launches with programmatic dependence: the kernel may be set up on SMs that
+// the kernel before it in the stream has left while that one still runs, and
+// waits for its end (and its writes) at its own griddepcontrol.wait, which
+// stands before every access to global memory.
+template <typename K, typename... A>
+b2_status launch_chained(K kern, unsigned grid, unsigned block, size_t smem, cudaStream_t st, const char* what,
+                         const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
+}
+
+template <int EPI, int PBN, bool A_MN, bool B_MN, int ACT>
 b2_status launch_gemm(const Maps& maps, const Params& p, cudaStream_t st) {
   using C = Config<EPI, PBN>;
-  auto kern = gated_kernel<EPI, PBN, A_MN, B_MN>;
+  auto kern = gated_kernel<EPI, PBN, A_MN, B_MN, ACT>;
   int dev = 0;
   B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
   static bool configured[64] = {};
@@ -751,19 +1072,18 @@ b2_status launch_gemm(const Maps& maps, const Params& p, cudaStream_t st) {
     configured[dev] = true;
   }
   const int clusters = std::min(p.items, sm_count(dev) / 2);
-  kern<<<2 * clusters, kThreads, C::kSmem, st>>>(maps, p);
-  return check_cuda(cudaGetLastError(), "gated product launch");
+  return launch_chained(kern, 2 * clusters, kThreads, C::kSmem, st, "gated product launch", maps, p);
 }
 
 // The gate epilogues' tensors.
 struct Gate {
-  int act = 0, train = 0;
+  int train = 0;
   Mat h, o1, o2;                 // written: h, P, A (kGate) or dg, du (kGateBwd)
   const uint16_t *fp = nullptr, *fa = nullptr;
   int64_t ldf = 0;
 };
 
-template <int EPI, bool A_MN, bool B_MN>
+template <int EPI, bool A_MN, bool B_MN, int ACT = kSilu>
 b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial, const Gate* gate, cudaStream_t st) {
   Maps maps;
   Params p{};
@@ -804,24 +1124,25 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
     if (EPI == kStore && q.tma_out) B2_TRY(map2d(&maps.o[i], {x.out, x.M, x.N, x.ldo}, 64, 32, 128));
   }
   if (EPI != kStore) {
-    p.act = gate->act;
     p.train = gate->train;
-    p.fp = gate->fp;
-    p.fa = gate->fa;
-    p.ldf = gate->ldf;
-    if (EPI == kGate) B2_TRY(map2d(&maps.o[0], gate->h, 32, 32, 64));
+    if (EPI == kGate) {
+      B2_TRY(map2d(&maps.o[0], gate->h, 32, 32, 64));
+    } else {
+      B2_TRY(map2d(&maps.a[1], {gate->fp, pr[0].M, pr[0].N, gate->ldf}, 32, 32, 64));
+      B2_TRY(map2d(&maps.b[1], {gate->fa, pr[0].M, pr[0].N, gate->ldf}, 32, 32, 64));
+    }
     if (EPI == kGateBwd || gate->train) {
       B2_TRY(map2d(&maps.o[1], gate->o1, 32, 32, 64));
       B2_TRY(map2d(&maps.o[2], gate->o2, 32, 32, 64));
     }
   }
-  B2_TRY((pbn == 256 ? launch_gemm<EPI, 256, A_MN, B_MN>(maps, p, st) : launch_gemm<EPI, 128, A_MN, B_MN>(maps, p, st)));
+  B2_TRY((pbn == 256 ? launch_gemm<EPI, 256, A_MN, B_MN, ACT>(maps, p, st)
+                     : launch_gemm<EPI, 128, A_MN, B_MN, ACT>(maps, p, st)));
   for (int i = 0; i < n; ++i) {
     if (p.p[i].splits <= 1) continue;
     ReduceArgs r{};
     r.q = p.p[i];
     if (EPI != kStore) {
-      r.act = gate->act;
       r.train = gate->train;
       r.h = static_cast<uint16_t*>(const_cast<void*>(gate->h.p));
       r.o1 = static_cast<uint16_t*>(const_cast<void*>(gate->o1.p));
@@ -834,13 +1155,83 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
     }
     const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * ((EPI == kGate ? pbn / 2 : pbn) / 8);
     const unsigned blocks = unsigned(std::min<long long>((units + 7) / 8, 148 * 16));
-    if (pbn == 256)
-      gated_reduce_kernel<EPI, 256><<<blocks, 256, 0, st>>>(r);
-    else
-      gated_reduce_kernel<EPI, 128><<<blocks, 256, 0, st>>>(r);
-    B2_TRY(check_cuda(cudaGetLastError(), "gated reduce launch"));
+    B2_TRY((pbn == 256 ? launch_chained(gated_reduce_kernel<EPI, 256, ACT>, blocks, 256, 0, st, "gated reduce launch", r)
+                       : launch_chained(gated_reduce_kernel<EPI, 128, ACT>, blocks, 256, 0, st, "gated reduce launch", r)));
   }
   return B2_OK;
+}
+
+FewMat few_mat(const Mat& m) {
+  const auto* p = static_cast<const uint16_t*>(m.p);
+  return {p, p + (m.rows - 1) * m.ld + m.cols, m.ld, tma_rows(m.p, m.ld) ? 1 : 0};
+}
+
+template <int EPI, int NT, int ACT, bool ALIGNED>
+b2_status launch_few_nt(const FewArgs& a, cudaStream_t st) {
+  int dev = 0;
+  B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  const int groups = (a.rows + 15) / 16;
+  const int steps = (a.K + 31) / 32;
+  // a reduction is shared by as many CTAs as stay resident together, while every warp has two steps or more
+  int cluster = 1;
+  while (cluster < 8 && groups * cluster * 2 <= kFewPerSm * sm_count(dev) && steps >= 4 * kFewWarps * cluster)
+    cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(groups * cluster));
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return check_cuda(cudaLaunchKernelEx(&cfg, gated_few_kernel<EPI, NT, ACT, ALIGNED>, a, cluster),
+                    "gated few-token launch");
+}
+
+template <int EPI, int ACT, bool ALIGNED>
+b2_status launch_few_rows(const FewArgs& a, cudaStream_t st) {
+  if (a.M <= 8) return launch_few_nt<EPI, 1, ACT, ALIGNED>(a, st);
+  if (a.M <= 16) return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
+  return launch_few_nt<EPI, 4, ACT, ALIGNED>(a, st);
+}
+template <int EPI, int ACT>
+b2_status launch_few(const FewArgs& a, cudaStream_t st) {
+  const bool aligned = a.w[0].aligned && (EPI == kStore || a.w[1].aligned);
+  return aligned ? launch_few_rows<EPI, ACT, true>(a, st) : launch_few_rows<EPI, ACT, false>(a, st);
+}
+
+// The forward of few tokens: two launches, no padded copies.
+b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd, int act, const Mat& h, uint16_t* fp,
+                      uint16_t* fa, void* y, int64_t ldy, cudaStream_t st) {
+  FewArgs a{};
+  a.w[0] = few_mat(wg);
+  a.w[1] = few_mat(wu);
+  a.x = few_mat(x);
+  a.M = int(x.rows);
+  a.rows = int(wg.rows);
+  a.K = int(x.cols);
+  a.out = static_cast<uint16_t*>(const_cast<void*>(h.p));
+  a.o1 = fp;
+  a.o2 = fa;
+  a.ldo = h.ld;
+  B2_TRY((act == kSilu   ? launch_few<kGate, kSilu>(a, st)
+          : act == kGelu ? launch_few<kGate, kGelu>(a, st)
+                         : launch_few<kGate, kRelu>(a, st)));
+  FewArgs d{};
+  d.w[0] = few_mat(wd);
+  d.x = few_mat(h);
+  d.M = a.M;
+  d.rows = int(wd.rows);
+  d.K = int(wd.cols);
+  d.early = 1;
+  d.out = static_cast<uint16_t*>(y);
+  d.ldo = ldy;
+  return launch_few<kStore, kSilu>(d, st);
 }
 
 // Carves a workspace; with a null base it only counts.
@@ -881,9 +1272,11 @@ struct Padder {
   }
   b2_status run(cudaStream_t st) {
     if (a.n == 0) return B2_OK;
+    for (int i = 0; i < a.n; ++i)
+      if (a.begin[i + 1] - a.begin[i] > UINT32_MAX)
+        return set_error(B2_ERR_UNSUPPORTED, "gated_mlp: an operand of unaligned rows is too large to copy");
     const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 255) / 256, 148 * 16));
-    gated_pad_kernel<<<blocks, 256, 0, st>>>(a);
-    return check_cuda(cudaGetLastError(), "gated pad launch");
+    return launch_chained(gated_pad_kernel, blocks, 256, 0, st, "gated pad launch", a);
   }
 };
 
@@ -965,6 +1358,10 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   const int64_t Fp = up8(F);
   const Mat h = saved ? Mat{saved, M, F, 3 * Fp} : Mat{ws.take(size_t(M) * Fp * 2), M, F, Fp};
   Mat mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
+  if (M <= kFewTokens) {
+    uint16_t* keep = static_cast<uint16_t*>(saved);
+    return few_forward(mx, mg, mu, md, act, h, keep ? keep + Fp : nullptr, keep ? keep + 2 * Fp : nullptr, y, ldy, st);
+  }
   Padder pad;
   pad.add(mx, ws);
   pad.add(mg, ws);
@@ -973,7 +1370,6 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   B2_TRY(pad.run(st));
   void* partial = ws.take(std::max(plan.gate.partial_bytes, plan.down.partial_bytes));
   Gate gate;
-  gate.act = act;
   gate.train = saved != nullptr;
   gate.h = h;
   if (saved) {
@@ -987,7 +1383,9 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   up.M = M;
   up.N = F;
   up.K = D;
-  B2_TRY((run_products<kGate, false, false>(&up, 1, plan.gate, partial, &gate, st)));
+  B2_TRY((act == kSilu   ? run_products<kGate, false, false, kSilu>(&up, 1, plan.gate, partial, &gate, st)
+          : act == kGelu ? run_products<kGate, false, false, kGelu>(&up, 1, plan.gate, partial, &gate, st)
+                         : run_products<kGate, false, false, kRelu>(&up, 1, plan.gate, partial, &gate, st)));
   Product down;
   down.a[0] = h;
   down.b[0] = md;
