@@ -15,6 +15,16 @@
 // shared memory while its maximum and sum are formed (one running maximum and
 // sum per thread, fp32), spread over a cluster of up to 8 CTAs when it is
 // longer than one CTA's share; the gradient is then written from the held row.
+// Two kernels do that: distill_stream_kernel, persistent, loads rows ahead of
+// the arithmetic and keeps the memory system busy through it (many long rows);
+// distill_row_kernel gives every row CTAs of its own (few rows, short rows, or
+// rows that no cluster holds, which it reads twice).
+//
+// Exponents are base 2: with c = log2(e) / tau and R = max * c (rounded), a
+// thread's sum is sum 2^(z c - R), one fused multiply-add and one 2^x per logit;
+// since every later use refers to the same rounded R, its rounding cancels.
+// Where R is not finite (rows whose largest logit is the type's lowest value,
+// or an infinity) the difference is taken before the product.
 // The backward proper has nothing to do when the upstream gradient is 1 (a
 // loss that is differentiated directly); for any other value it writes the
 // gradient again from the logits and the row's statistics, so that each
@@ -31,6 +41,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;        // teacher entries per row
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
 
 enum Reduction : int { kMean = 0, kSum = 1, kNone = 2 };
 
@@ -112,18 +123,39 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Running maximum and sum of exponentials relative to it.  An empty pair is
-// (-inf, 0); a maximum of -inf means that nothing above -inf was seen.
+// Maximum and the sum of exponentials relative to it (relative to its rounded R
+// where that is finite).  An empty pair is (-inf, 0); a maximum of -inf means
+// that nothing above -inf was seen.
 struct MaxSum {
   float m, s;
 };
-// (base-2 exponents: c = log2(e) / tau)
+// log2 of the factor that brings a sum relative to `from` to one relative to `to`
+__device__ __forceinline__ float rescale(float from, float to, float c) {
+  const float a = from * c, b = to * c;
+  return fabsf(a) < INFINITY && fabsf(b) < INFINITY ? a - b : (from - to) * c;
+}
 __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
   const float m = fmaxf(a.m, b.m);
   // -inf - -inf would be NaN: a side that saw nothing keeps its sum of 0 (or a NaN that it saw)
-  const float fa = a.m == m ? 1.f : ex2((a.m - m) * c);
-  const float fb = b.m == m ? 1.f : ex2((b.m - m) * c);
+  const float fa = a.m == m ? 1.f : ex2(rescale(a.m, m, c));
+  const float fb = b.m == m ? 1.f : ex2(rescale(b.m, m, c));
   return {m, a.s * fa + b.s * fb};
+}
+// The pair of W neighbouring lanes' pairs, in each of them: the maximum first,
+// then each lane's sum relative to it once, then the sum of those.
+template <int W>
+__device__ __forceinline__ MaxSum warp_pair(MaxSum v, float c) {
+  float m = v.m;
+#pragma unroll
+  for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float s = v.m == m ? v.s : v.s * ex2(rescale(v.m, m, c));
+#pragma unroll
+  for (int o = W / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return {m, s};
+}
+// One value: 2^0 of the sum if it is the maximum, NaN if it is +inf (inf - inf)
+__device__ __forceinline__ MaxSum one_value(float x) {
+  return {x, x == INFINITY ? __int_as_float(0x7fc00000) : 1.f};
 }
 
 template <typename F>
@@ -144,7 +176,10 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch, F f) {
   return v;
 }
 
-// The row's teacher entries in dynamic shared memory, [K] each.
+// Teacher arrays in shared memory hold a multiple of four entries.
+__host__ __device__ constexpr int padded_top(int K) { return (K + 3) / 4 * 4; }
+
+// The row's teacher entries in dynamic shared memory.
 struct TeacherSmem {
   float* p;
   int* id;
@@ -164,9 +199,11 @@ __device__ __forceinline__ Teacher load_teacher(const Args& a, long long r, cons
   Teacher t;
   float m = -INFINITY;
   int bad = 0, nan = 0;
-  for (int k = threadIdx.x; k < a.K; k += kThreads) {
-    const long long id = a.ids64 ? static_cast<const long long*>(a.ids)[r * a.ldi + k]
-                                 : (long long)static_cast<const int*>(a.ids)[r * a.ldi + k];
+  for (int k = threadIdx.x; k < padded_top(a.K); k += kThreads) {
+    long long id = -1;
+    if (k < a.K)
+      id = a.ids64 ? static_cast<const long long*>(a.ids)[r * a.ldi + k]
+                   : (long long)static_cast<const int*>(a.ids)[r * a.ldi + k];
     float v = -INFINITY;
     if (id >= 0) {
       const long long at = r * a.ldt + k;
@@ -198,13 +235,20 @@ __device__ __forceinline__ Teacher load_teacher(const Args& a, long long r, cons
   return t;
 }
 
-// Probability the teacher gives to id (entries with the same id add up, in
-// entry order), for entry k.
+// Probability the teacher gives to entry k's id (entries with the same id add
+// up, in entry order).  Ids are compared four at a time; the arrays hold a
+// multiple of four entries, 16-byte aligned, absent ones with id -1.
 __device__ __forceinline__ float teacher_p(const TeacherSmem& sm, int K, int k) {
   const int id = sm.id[k];
   float p = 0.f;
-  for (int j = 0; j < K; ++j)
-    if (sm.id[j] == id) p += sm.p[j];
+  const int4* ids = reinterpret_cast<const int4*>(sm.id);
+  for (int j = 0; j < K; j += 4) {
+    const int4 v = ids[j / 4];
+    if (v.x == id) p += sm.p[j];
+    if (v.y == id) p += sm.p[j + 1];
+    if (v.z == id) p += sm.p[j + 2];
+    if (v.w == id) p += sm.p[j + 3];
+  }
   return p;
 }
 
@@ -222,17 +266,135 @@ struct RowParts {
   }
 };
 
-// The gradient of 16 bytes of logits: a * 2^((z - m) c - l2s)
+// A thread's running pair over 16-byte vectors of logits.  The common case --
+// its maximum so far times c is finite -- is one multiply-add, one 2^x and one
+// addition per logit; the test for it and for a new maximum is made once for up
+// to 8 vectors (some lane of a warp sees a new maximum nearly every time, so its
+// dozen instructions are the price of every test).
 template <typename T>
-__device__ __forceinline__ uint4 grad_vec(const Vec16<T>& x, float m, float c, float l2s, float a) {
+struct Running {
+  static constexpr int E = Vec16<T>::N;
+  float c;
+  MaxSum ms;
+  float ref;    // ms.m * c
+  bool plain;   // finite
+  __device__ __forceinline__ explicit Running(float c_) : c(c_), ms{-INFINITY, 0.f}, ref(-INFINITY), plain(false) {}
+  __device__ __forceinline__ void grow(float m) {
+    ms.s *= ex2(rescale(ms.m, m, c));  // 0 * 2^-inf = 0 for the first
+    ms.m = m;
+    ref = m * c;
+    plain = fabsf(ref) < INFINITY;
+  }
+  __device__ __forceinline__ void add1(float x) {
+    ms = merge(ms, one_value(x), c);
+    ref = ms.m * c;
+    plain = fabsf(ref) < INFINITY;
+  }
+  template <int V>
+  static __device__ __forceinline__ float max_of(const Vec16<T> (&x)[V]) {
+    if constexpr (sizeof(T) == 2) {
+      __nv_bfloat162 m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = reinterpret_cast<const __nv_bfloat162*>(&x[0].v)[i];
+#pragma unroll
+      for (int v = 1; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = __hmax2(m[i], reinterpret_cast<const __nv_bfloat162*>(&x[v].v)[i]);
+      const __nv_bfloat162 all = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+      return fmaxf(__low2float(all), __high2float(all));
+    } else {
+      float m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = x[0].get(i);
+#pragma unroll
+      for (int v = 1; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], x[v].get(i));
+      return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    }
+  }
+  template <int V>
+  __device__ __forceinline__ void add(const Vec16<T> (&x)[V]) {
+    const float mx = max_of(x);
+    if (mx > ms.m) grow(mx);
+    if (plain) {
+      float sum[4] = {ms.s, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum[j % 4] += ex2(fmaf(x[v].get(j), c, -ref));
+      ms.s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    } else {
+      // nothing above -inf yet (or only NaN): relative to 0, so that -inf gives 0 and NaN stays
+      const float m = ms.m == -INFINITY ? 0.f : ms.m;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int j = 0; j < E; ++j) ms.s += ex2((x[v].get(j) - m) * c);
+    }
+  }
+  // vectors first, first + step, ... of src[0 .. n)
+  template <int V>
+  __device__ __forceinline__ int add_some(const uint4* src, int i, int n, int step) {
+#pragma unroll 1
+    for (; i + (V - 1) * step < n; i += V * step) {
+      Vec16<T> x[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v].v = src[i + v * step];
+      add(x);
+    }
+    return i;
+  }
+  __device__ __forceinline__ void add_slice(const uint4* src, int first, int n, int step) {
+    int i = add_some<8>(src, first, n, step);
+    i = add_some<4>(src, i, n, step);
+    add_some<1>(src, i, n, step);
+  }
+};
+
+// A row's statistics as its gradient and loss use them: log2 q = z c - R - l2s.
+template <typename T>
+struct Prob {
+  float c, m, l2s, ref;
+  bool plain;
+  __device__ __forceinline__ Prob(float c_, float m_, float l2s_)
+      : c(c_), m(m_), l2s(l2s_), ref(m_ * c_), plain(fabsf(m_ * c_) < INFINITY) {}
+  __device__ __forceinline__ float log2q(float z) const {
+    return (plain ? fmaf(z, c, -ref) : (z - m) * c) - l2s;
+  }
+  __device__ __forceinline__ float operator()(float z) const {
+    if (plain) return fast(z);
+    return ex2(log2q(z));
+  }
+  // `plain` rows.  bf16 results round at 2^-8: the two offsets are added up first
+  // (an error of 2^-24 of their size); fp32 keeps z c - R exact where it matters,
+  // near the top.
+  __device__ __forceinline__ float fast(float z) const {
+    if constexpr (sizeof(T) == 2) return ex2(fmaf(z, c, -(ref + l2s)));
+    else return ex2(fmaf(z, c, -ref) - l2s);
+  }
+};
+
+// The gradient of 16 bytes of logits, a * q.  PLAIN: a positive factor joins the
+// exponent (off: its logarithm less the offsets), which saves the product.
+template <typename T, bool PLAIN>
+__device__ __forceinline__ uint4 grad_vec(const Vec16<T>& x, const Prob<T>& q, float a, float off) {
   constexpr int E = Vec16<T>::N;
   float g[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) g[i] = a * ex2((x.get(i) - m) * c - l2s);
+  for (int i = 0; i < E; ++i) {
+    if constexpr (!PLAIN) g[i] = a * ex2(q.log2q(x.get(i)));
+    else if constexpr (sizeof(T) == 2) g[i] = ex2(fmaf(x.get(i), q.c, off));
+    else g[i] = ex2(fmaf(x.get(i), q.c, -q.ref) + off);
+  }
   if constexpr (sizeof(T) == 2)
     return make_uint4(cvt2(g[0], g[1]), cvt2(g[2], g[3]), cvt2(g[4], g[5]), cvt2(g[6], g[7]));
   else
     return make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3]));
+}
+template <typename T>
+__device__ __forceinline__ float grad_offset(const Prob<T>& q, float a) {
+  return sizeof(T) == 2 ? log2f(a) - (q.ref + q.l2s) : log2f(a) - q.l2s;
 }
 
 template <typename T>
@@ -243,6 +405,30 @@ __device__ __forceinline__ void put_vec(T* dst, const uint4& v, bool aligned) {
     const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
     for (int i = 0; i < Vec16<T>::N; ++i) dst[i] = e[i];
+  }
+}
+
+// The gradient of vectors first, first + step, ... of src[0 .. n) to dst
+template <typename T>
+__device__ __forceinline__ void grad_slice(const uint4* src, T* dst, int first, int n, int step, const Prob<T>& q,
+                                           float a) {
+  if (q.plain && a > 0.f && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    const float off = grad_offset(q, a);
+    uint4* d = reinterpret_cast<uint4*>(dst);
+#pragma unroll 2
+    for (int i = first; i < n; i += step) {
+      Vec16<T> x;
+      x.v = src[i];
+      d[i] = grad_vec<T, true>(x, q, a, off);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = first; i < n; i += step) {
+      Vec16<T> x;
+      x.v = src[i];
+      put_vec<T>(dst + (long long)i * Vec16<T>::N, grad_vec<T, false>(x, q, a, 0.f),
+                 (reinterpret_cast<uintptr_t>(dst) & 15) == 0);
+    }
   }
 }
 
@@ -276,13 +462,13 @@ __global__ void __launch_bounds__(1024) distill_begin_kernel(const Args a) {
 // cluster per row; CTA `rank` owns `slice` vectors of it (the first also the
 // head, the last also the tail).
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int cluster) {
+__global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int cluster) {
   constexpr int E = Vec16<T>::N;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint4* held = reinterpret_cast<uint4*>(smem_raw);
   __shared__ float teacher_scratch[kWarps];
   float* teacher_p0 = reinterpret_cast<float*>(held + a.tile);
-  const TeacherSmem teacher{teacher_p0, reinterpret_cast<int*>(teacher_p0 + a.K), teacher_scratch};
+  const TeacherSmem teacher{teacher_p0, reinterpret_cast<int*>(teacher_p0 + padded_top(a.K)), teacher_scratch};
   __shared__ uint64_t bar;
   __shared__ float share[2];          // this CTA's maximum and sum, read by the cluster
   __shared__ float scratch[2][kWarps];
@@ -336,9 +522,7 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
     }
   } else {
     const float c = kLog2e / a.tau;
-    MaxSum ms{-INFINITY, 0.f};
-    // one value: 2^0 of the sum if it is the maximum, NaN if it is +inf (inf - inf)
-    auto add1 = [&](float x) { ms = merge(ms, {x, x == INFINITY ? __int_as_float(0x7fc00000) : 1.f}, c); };
+    Running<T> run(c);
     // the unaligned ends straight from memory
     float edge = 0.f;
     const bool has_head = rank == 0 && int(threadIdx.x) < part.head;
@@ -346,12 +530,12 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
     const T* edge_tail = row + part.head + part.vecs * E + threadIdx.x;
     if (has_head) {
       edge = load1(row + threadIdx.x);
-      add1(edge);
+      run.add1(edge);
     }
     float edge2 = 0.f;
     if (has_tail) {
       edge2 = load1(edge_tail);
-      add1(edge2);
+      run.add1(edge2);
     }
     for (long long b = v0; b < v1; b += a.tile) {
       if (b > v0) {
@@ -359,38 +543,18 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
         fetch(b);
       }
       landed();
-      const int n = int(min(a.tile, v1 - b));
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        Vec16<T> x;
-        x.v = held[i];
-        float mx = x.get(0);
-#pragma unroll
-        for (int j = 1; j < E; ++j) mx = fmaxf(mx, x.get(j));
-        if (mx > ms.m) {
-          ms.s *= ex2((ms.m - mx) * c);  // 0 * 2^-inf = 0 for the first
-          ms.m = mx;
-        }
-        // nothing above -inf yet (or only NaN): exponents relative to 0, so that -inf gives 0 and NaN stays
-        const float ref = ms.m == -INFINITY ? 0.f : ms.m;
-#pragma unroll
-        for (int j = 0; j < E; ++j) ms.s += ex2((x.get(j) - ref) * c);
-      }
+      run.add_slice(held, int(threadIdx.x), int(min(a.tile, v1 - b)), kThreads);
     }
+    MaxSum ms = run.ms;
     // this CTA's pair
     {
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        MaxSum other{__shfl_xor_sync(0xffffffffu, ms.m, o), __shfl_xor_sync(0xffffffffu, ms.s, o)};
-        ms = merge(ms, other, c);
-      }
+      ms = warp_pair<32>(ms, c);
       if ((threadIdx.x & 31) == 0) {
         scratch[0][threadIdx.x >> 5] = ms.m;
         scratch[1][threadIdx.x >> 5] = ms.s;
       }
       __syncthreads();
-      ms = {scratch[0][0], scratch[1][0]};
-#pragma unroll
-      for (int i = 1; i < kWarps; ++i) ms = merge(ms, {scratch[0][i], scratch[1][i]}, c);
+      ms = warp_pair<kWarps>({scratch[0][threadIdx.x % kWarps], scratch[1][threadIdx.x % kWarps]}, c);
     }
     if (cluster > 1) {
       if (threadIdx.x == 0) {
@@ -409,7 +573,8 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
     if (rank == 0) {
       // the loss: sum over entries of p (log p - log q), in entry order per thread
       const float inv_tau = 1.f / a.tau;
-      const float ln_mass = logf(tch.mass), ln_s = logf(ms.s);
+      const float ln_mass = logf(tch.mass);
+      const Prob<T> qs(c, ms.m, l2s);
       float sum = 0.f;
       for (int k = threadIdx.x; k < a.K; k += kThreads) {
         const float p = teacher.p[k];
@@ -418,7 +583,7 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
         const long long at = r * a.ldt + k;
         const float tv = a.t_f32 ? static_cast<const float*>(a.t)[at] : bf2f(static_cast<const uint16_t*>(a.t)[at]);
         const float logp = (tv - tch.m) * inv_tau - ln_mass;
-        const float logq = (load1(row + id) - ms.m) * inv_tau - ln_s;
+        const float logq = qs.log2q(load1(row + id)) * kLn2;
         sum += p * (logp - logq);
       }
       loss = block_reduce(sum, scratch[0], [](float x, float y) { return x + y; }) * a.tau * a.tau;
@@ -431,29 +596,24 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
     }
     if constexpr (GRAD) {
       const float f = tch.bad ? __int_as_float(0x7fc00000) : w * a.tau;
+      const Prob<T> q(c, ms.m, l2s);
       for (long long b = v0; b < v1; b += a.tile) {
         if (!single) {
           __syncthreads();
           fetch(b);
           landed();
         }
-        const int n = int(min(a.tile, v1 - b));
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-          Vec16<T> x;
-          x.v = held[i];
-          put_vec<T>(out + part.head + (b + i) * E, grad_vec<T>(x, ms.m, c, l2s, f), out_aligned);
-        }
+        grad_slice<T>(held, out + part.head + b * E, int(threadIdx.x), int(min(a.tile, v1 - b)), kThreads, q, f);
       }
-      if (has_head) store1(out + threadIdx.x, f * ex2((edge - ms.m) * c - l2s));
-      if (has_tail) store1(out + part.head + part.vecs * E + threadIdx.x, f * ex2((edge2 - ms.m) * c - l2s));
+      if (has_head) store1(out + threadIdx.x, f * q(edge));
+      if (has_tail) store1(out + part.head + part.vecs * E + threadIdx.x, f * q(edge2));
       __syncthreads();  // the entries' elements are written again, from both terms
       const long long lo = rank == 0 ? 0 : part.head + v0 * E;
       const long long hi = rank == cluster - 1 ? a.V : part.head + v1 * E;
       for (int k = threadIdx.x; k < a.K; k += kThreads) {
         const int id = teacher.id[k];
         if (id < lo || id >= hi) continue;
-        const float q = ex2((load1(row + id) - ms.m) * c - l2s);
-        store1(out + id, f * (q - teacher_p(teacher, a.K, k)));
+        store1(out + id, f * (q(load1(row + id)) - teacher_p(teacher, a.K, k)));
       }
     }
     if (cluster > 1) cluster_wait();
@@ -478,6 +638,404 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const Args a, int
   if (threadIdx.x == 0) *a.loss = sum;
 }
 
+// ---------------------------------------------------------------------------
+// The persistent kernel.  Three CTAs a SM, so that one's copies, another's
+// exponentials and a third's stores overlap; clusters of them walk the rows
+// cluster by cluster, each CTA with a ring of one to kRing slices.  Warp 8 runs
+// ahead: it reads a row's weight and teacher entries, starts the copy of the
+// slice unless the row is masked, meanwhile makes the teacher's probabilities
+// and, from the slice's entries, its part of the loss.  Warps 0..7 form the
+// slice's maximum and sum, exchange all that with the cluster's CTAs (a remote
+// store and a remote arrival each) and write the gradient; then the entries'
+// elements once more, from both terms.
+//
+// The loss in parts: with m_j the maximum of slice j, P_j the probability of the
+// entries in it and lse the row's log-sum-exp of z / tau,
+//   sum_k p_k (log p_k - log q_k) = sum_j [ sum_{k in j} p_k (log p_k - (z_k -
+//   m_j) / tau) + P_j (lse - m_j / tau) ]
+// whose slice sums need nothing of the other slices.
+//
+// 8192 rows of 131072 bf16 logits with 64 entries, a seventh of them masked:
+// 876 us with the gradient (4.5 TB/s of the 6.45 measured), 530 us the loss
+// alone; a row's 10 us in a CTA are 2.5 of copy, 2.5 of sums, 0.7 of reduction,
+// 1.6 of exchange, 2.1 of gradient and 0.9 of entries.  (One CTA of 16 warps a SM
+// with a ring of three slices took 1610 us: a row at a time leaves the SM waiting
+// in every reduction.  Slices of half the size, with a ring of two, 1130 us.)
+//
+// Statistics slots: a CTA's publication of its row i + 2 follows its end of row
+// i + 1, which needed this CTA's publication of row i + 1, which this CTA made
+// after its own end of row i: two slots are never overrun.
+// ---------------------------------------------------------------------------
+constexpr int kStreamWarps = 8;
+constexpr int kStreamThreads = (kStreamWarps + 1) * 32;
+constexpr int kStreamPerSm = 3;
+constexpr int kRing = 4;
+constexpr int kSlots = 2;
+
+// What the forward warp knows of a row in the ring.
+struct RowMeta {
+  long long row;
+  int skip, bad;
+  float w, side, P, top;  // the slice's part of the loss relative to a logit of `top`, its entries' probability
+  float head[8], tail[8];
+};
+
+// Logit `id` of a row, from this CTA's held slice (vectors from v0) or the row's unaligned ends.
+template <typename T>
+__device__ __forceinline__ float slice_logit(const uint4* slice, const RowMeta& mt, const RowParts<T>& parts,
+                                             long long v0, int id) {
+  const long long tail0 = parts.head + parts.vecs * Vec16<T>::N;
+  return id < parts.head ? mt.head[id]
+         : id >= tail0   ? mt.tail[id - tail0]
+                         : load1(reinterpret_cast<const T*>(slice) + (id - parts.head - v0 * Vec16<T>::N));
+}
+
+// Waits of the persistent kernel: the thread is parked by the hardware (a hint
+// of 1 ms a try) instead of polling, since the pollers of one CTA would take the
+// issue slots of the others on the SM.  Same limit as mbar_wait.  CLUSTER: the
+// phase is completed by other CTAs' arrivals, whose stores become visible.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity, int* status) {
+  const uint32_t hint = 1000000;
+  unsigned long long t0 = 0;
+  for (;;) {
+    uint32_t ok;
+    if constexpr (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(hint)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(hint)
+          : "memory");
+    if (ok) return true;
+    const unsigned long long t = globaltimer();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitLimitNs) {
+      record_status(status, B2_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_kernel(const Args a, int cluster, int ring) {
+  constexpr int E = Vec16<T>::N;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ uint64_t full[kRing], top_full[kRing], empty[kRing], slot_bar[kSlots];
+  __shared__ float4 slot[kSlots][kMaxCluster];  // a slice's maximum, sum, loss part and P
+  __shared__ RowMeta meta[kRing];
+  __shared__ float part[2][kStreamWarps][2];
+  __shared__ float final_part[kStreamWarps];
+  __shared__ int last_row;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = int(threadIdx.x);
+  const int rank = cluster > 1 ? int(cluster_ctarank()) : 0;
+  const long long first = blockIdx.x / cluster, step = gridDim.x / cluster;
+  const float c = kLog2e / a.tau;
+  uint4* held = reinterpret_cast<uint4*>(smem_raw);
+  float* top_p = reinterpret_cast<float*>(held + ring * a.slice);
+  const int Kp = padded_top(a.K);
+  int* top_id = reinterpret_cast<int*>(top_p + (ring + 1) * Kp);
+  if (tid == 0) {
+    for (int b = 0; b < kRing; ++b) {
+      mbar_init(smem_u32(&full[b]), 1);
+      mbar_init(smem_u32(&top_full[b]), 1);
+      mbar_init(smem_u32(&empty[b]), kStreamWarps);
+    }
+    for (int b = 0; b < kSlots; ++b) mbar_init(smem_u32(&slot_bar[b]), uint32_t(cluster));
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (cluster > 1) cluster_sync();  // every CTA's barriers exist before a remote arrival
+
+  if (warp == kStreamWarps) {
+    // ------------------------------ the forward warp ------------------------
+    // A row's weight, teacher entries and unaligned ends, read before its buffer
+    // is free, so that its copy starts the moment it is.
+    struct Ahead {
+      float w, m, edge;
+      int bad;
+      bool skip;
+    };
+    auto look = [&](long long r, int slot_at) {
+      Ahead h{};
+      const T* row = static_cast<const T*>(a.z) + r * a.ldz;
+      const RowParts<T> parts(row, a.V);
+      float* p = top_p + slot_at * Kp;
+      int* ids = top_id + slot_at * Kp;
+      h.w = row_factor(a, r);
+      h.m = -INFINITY;
+      h.skip = true;
+      if (h.w == 0.f) return h;
+      // lanes 0..7: the head, 8..15: the tail
+      if (rank == 0 && lane < parts.head) h.edge = load1(row + lane);
+      if (rank == cluster - 1 && lane >= 8 && lane - 8 < parts.tail)
+        h.edge = load1(row + parts.head + parts.vecs * E + lane - 8);
+      int nan = 0;
+      for (int k = a.K + lane; k < Kp; k += 32) ids[k] = -1;
+      for (int k = lane; k < a.K; k += 32) {
+        const long long at = r * a.ldt + k;
+        const long long id = a.ids64 ? static_cast<const long long*>(a.ids)[r * a.ldi + k]
+                                     : (long long)static_cast<const int*>(a.ids)[r * a.ldi + k];
+        float v = a.t_f32 ? static_cast<const float*>(a.t)[at] : bf2f(static_cast<const uint16_t*>(a.t)[at]);
+        if (id < 0) v = -INFINITY;
+        if (id >= a.V) h.bad = 1;
+        if (v != v) nan = 1;
+        ids[k] = id >= 0 && id < a.V ? int(id) : -1;
+        p[k] = v;
+        h.m = fmaxf(h.m, v);
+      }
+      h.bad = __any_sync(0xffffffffu, h.bad);
+      nan = __any_sync(0xffffffffu, nan);
+      h.m = warp_reduce(h.m, [](float x, float y) { return fmaxf(x, y); });
+      h.skip = !(h.m > -INFINITY || nan || h.bad);
+      return h;
+    };
+    long long n = 0;
+    Ahead next{};
+    if (first < a.N) next = look(first, 0);
+    for (long long r = first; r < a.N; r += step, ++n) {
+      const int b = int(n % ring);
+      const int top_at = int(n % (ring + 1));
+      const Ahead h = next;
+      bool ok = true;
+      if (n >= ring) ok = mbar_wait_parked<false>(smem_u32(&empty[b]), uint32_t((n / ring - 1) & 1), a.status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const T* row = static_cast<const T*>(a.z) + r * a.ldz;
+      const RowParts<T> parts(row, a.V);
+      const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
+      if (lane < 8) meta[b].head[lane] = h.edge;
+      else if (lane < 16) meta[b].tail[lane - 8] = h.edge;
+      if (lane == 0) {
+        meta[b].row = r;
+        meta[b].skip = h.skip;
+        meta[b].bad = h.bad;
+        meta[b].w = h.w;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t bytes = h.skip ? 0u : uint32_t((v1 - v0) * 16);
+        if (bytes) {
+          mbar_arrive_expect_tx(smem_u32(&full[b]), bytes);
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(row + parts.head) + v0 * 16;
+          const uint32_t dst = smem_u32(held + b * a.slice);
+          for (uint32_t at = 0; at < bytes; at += 16384)
+            bulk_load_1d(dst + at, src + at, min(16384u, bytes - at), smem_u32(&full[b]));
+        } else {
+          mbar_arrive(smem_u32(&full[b]));
+        }
+        if (h.bad && rank == 0) record_status(a.status, B2_ERR_INVALID);
+      }
+      if (!h.skip) {
+        float* p = top_p + top_at * Kp;
+        float s = 0.f;
+        for (int k = lane; k < a.K; k += 32) {
+          const float v = p[k];
+          const float e = v == -INFINITY ? 0.f : ex2((v - h.m) * c);
+          p[k] = e;
+          s += e;
+        }
+        s = warp_reduce(s, [](float x, float y) { return x + y; });
+        const float inv = 1.f / s;
+        // the entries of this slice, once it is here: their part of the loss
+        const int* ids = top_id + top_at * Kp;
+        const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
+        const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
+        const uint4* slice = held + b * a.slice;
+        mbar_wait_parked<false>(smem_u32(&full[b]), uint32_t(n / ring) & 1u, a.status);
+        float top = -INFINITY;
+        for (int k = lane; k < a.K; k += 32) {
+          const float pk = p[k] * inv;
+          p[k] = pk;
+          if (ids[k] >= lo && ids[k] < hi && pk != 0.f)
+            top = fmaxf(top, slice_logit<T>(slice, meta[b], parts, v0, ids[k]));
+        }
+        top = warp_reduce(top, [](float x, float y) { return fmaxf(x, y); });
+        if (!(fabsf(top) < INFINITY)) top = 0.f;
+        const float inv_tau = 1.f / a.tau;
+        float side = 0.f, P = 0.f;
+        for (int k = lane; k < a.K; k += 32) {
+          const float pk = p[k];
+          if (ids[k] < lo || ids[k] >= hi || pk == 0.f) continue;
+          const float z = slice_logit<T>(slice, meta[b], parts, v0, ids[k]);
+          // a closed entry makes the loss infinite, also in a slice of nothing else
+          side += z == -INFINITY ? INFINITY : pk * (logf(pk) - (z - top) * inv_tau);
+          P += pk;
+        }
+        side = warp_reduce(side, [](float x, float y) { return x + y; });
+        P = warp_reduce(P, [](float x, float y) { return x + y; });
+        if (lane == 0) {
+          meta[b].side = side;
+          meta[b].P = P;
+          meta[b].top = top;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&top_full[b]));
+      if (r + step < a.N) next = look(r + step, int((n + 1) % (ring + 1)));
+    }
+    // every copy lands before the CTA goes away (also if the others gave up)
+    for (long long i = max(0LL, n - ring); i < n; ++i)
+      mbar_wait_parked<false>(smem_u32(&full[i % ring]), uint32_t(i / ring) & 1u, a.status);
+  } else {
+    // ------------------------------ the compute warps -----------------------
+    long long counted = 0;  // rows with statistics
+    int flip = 0;
+    bool ok = true;
+    // Statistics of the row in buffer b, its loss, its gradient; frees the buffer.
+    auto finish = [&](long long n, MaxSum ms, float parts_m, float side, float P) {
+      const int b = int(n % ring);
+      const RowMeta& mt = meta[b];
+      const long long r = mt.row;
+      const float l2s = log2f(ms.s);
+      if (rank == 0 && warp == 0) {
+        // lane j: slice j
+        float part_loss = 0.f;
+        if (lane < cluster) part_loss = P == 0.f ? side : side - P * Prob<T>(c, ms.m, l2s).log2q(parts_m) * kLn2;
+#pragma unroll
+        for (int o = kMaxCluster / 2; o; o >>= 1) part_loss += __shfl_xor_sync(0xffffffffu, part_loss, o);
+        side = part_loss;
+      }
+      if (rank == 0 && tid == 0) {
+        const float loss = mt.bad ? __int_as_float(0x7fc00000) : a.tau * a.tau * side;
+        a.stats[2 * r] = ms.m;
+        a.stats[2 * r + 1] = l2s;
+        if (a.reduction == kNone) a.loss[r] = mt.w * loss;
+        else a.row_loss[r] = mt.w * loss;
+      }
+      if constexpr (GRAD) {
+        const T* row = static_cast<const T*>(a.z) + r * a.ldz;
+        T* out = static_cast<T*>(a.dz) + r * a.lddz;
+        const RowParts<T> parts(row, a.V);
+        const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
+        const int count = int(v1 - v0);
+        const uint4* src = held + b * a.slice;
+        const float f = mt.bad ? __int_as_float(0x7fc00000) : mt.w * a.tau;
+        const Prob<T> q(c, ms.m, l2s);
+        T* dst = out + parts.head + v0 * E;
+        grad_slice<T>(src, dst, tid, count, kStreamWarps * 32, q, f);
+        const long long tail0 = parts.head + parts.vecs * E;
+        if (rank == 0 && tid < parts.head) store1(out + tid, f * q(mt.head[tid]));
+        if (rank == cluster - 1 && tid < parts.tail) store1(out + tail0 + tid, f * q(mt.tail[tid]));
+        compute_sync();  // the entries' elements are written again, from both terms
+        const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
+        const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
+        const int top_at = int(n % (ring + 1));
+        const TeacherSmem top{top_p + top_at * Kp, top_id + top_at * Kp, nullptr};
+        for (int k = tid; k < a.K; k += kStreamWarps * 32) {
+          const int id = top.id[k];
+          if (id < lo || id >= hi) continue;
+          store1(out + id, f * (q(slice_logit<T>(src, mt, parts, v0, id)) - teacher_p(top, a.K, k)));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty[b]));
+    };
+    long long n = 0;
+    for (long long r = first; r < a.N && ok; r += step, ++n) {
+      const int b = int(n % ring);
+      ok = mbar_wait_parked<false>(smem_u32(&full[b]), uint32_t(n / ring) & 1u, a.status);
+      if (!ok) break;
+      const RowMeta& mt = meta[b];
+      const T* row = static_cast<const T*>(a.z) + r * a.ldz;
+      const RowParts<T> parts(row, a.V);
+      const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
+      const int count = int(v1 - v0);
+      if (mt.skip) {
+        if constexpr (GRAD) {
+          T* out = static_cast<T*>(a.dz) + r * a.lddz;
+          T* dst = out + parts.head + v0 * E;
+          const bool aligned = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+          for (int i = tid; i < count; i += kStreamWarps * 32)
+            put_vec<T>(dst + (long long)i * E, make_uint4(0, 0, 0, 0), aligned);
+          if (rank == 0 && tid < parts.head) out[tid] = T(0);
+          if (rank == cluster - 1 && tid < parts.tail) out[parts.head + parts.vecs * E + tid] = T(0);
+        }
+        if (rank == 0 && tid == 0) {
+          a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
+          if (a.reduction == kNone) a.loss[r] = 0.f;
+          else a.row_loss[r] = 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&empty[b]));
+        continue;
+      }
+      const uint4* src = held + b * a.slice;
+      Running<T> run(c);
+      if (rank == 0 && tid < parts.head) run.add1(mt.head[tid]);
+      if (rank == cluster - 1 && tid < parts.tail) run.add1(mt.tail[tid]);
+      run.add_slice(src, tid, count, kStreamWarps * 32);
+      MaxSum ms = run.ms;
+      ms = warp_pair<32>(ms, c);
+      flip ^= 1;  // the last row's parts may still be read
+      if (lane == 0) {
+        part[flip][warp][0] = ms.m;
+        part[flip][warp][1] = ms.s;
+      }
+      ok = mbar_wait_parked<false>(smem_u32(&top_full[b]), uint32_t(n / ring) & 1u, a.status);
+      compute_sync();
+      ms = warp_pair<kStreamWarps>({part[flip][lane % kStreamWarps][0], part[flip][lane % kStreamWarps][1]}, c);
+      // the entries' part of the loss, now relative to the slice's maximum
+      float side = mt.side, P = mt.P, slice_m = ms.m;
+      if (P != 0.f) side -= P * (mt.top - slice_m) / a.tau;
+      if (cluster > 1) {
+        const int at = int(counted % kSlots);
+        if (warp == 0 && lane < cluster) {  // one lane per CTA of the cluster
+          const uint32_t to = mapa_shared(smem_u32(&slot[at][rank]), uint32_t(lane));
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(ms.m), "f"(ms.s), "f"(side),
+                       "f"(P)
+                       : "memory");
+          mbar_arrive_remote(mapa_shared(smem_u32(&slot_bar[at]), uint32_t(lane)));
+        }
+        __syncwarp();
+        ok = mbar_wait_parked<true>(smem_u32(&slot_bar[at]), uint32_t(counted / kSlots) & 1u, a.status) && ok;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float4 of{-INFINITY, 0.f, 0.f, 0.f};
+        if (lane % kMaxCluster < cluster) of = slot[at][lane % kMaxCluster];
+        ms = warp_pair<kMaxCluster>({of.x, of.y}, c);
+        slice_m = of.x;
+        side = of.z;
+        P = of.w;
+        ++counted;
+      }
+      finish(n, ms, slice_m, side, P);
+    }
+  }
+  __syncwarp();
+  if (cluster > 1) cluster_sync();  // no CTA leaves while another may still write its slots
+  if (a.reduction == kNone || rank != 0) return;
+  // reduction: the last cluster to arrive adds all rows, in row order
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    last_row = atomicAdd(a.counter, 1u) == unsigned(step - 1);
+  }
+  __syncthreads();
+  if (!last_row) return;
+  __threadfence();
+  float sum = 0.f;
+  if (warp < kStreamWarps)
+    for (long long i = tid; i < a.N; i += kStreamWarps * 32) sum += __ldcg(a.row_loss + i);
+  sum = warp_reduce(sum, [](float x, float y) { return x + y; });
+  if (lane == 0 && warp < kStreamWarps) final_part[warp] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    sum = 0.f;
+    for (int i = 0; i < kStreamWarps; ++i) sum += final_part[i];
+    *a.loss = sum;
+  }
+}
+
 // Backward for any upstream gradient: the gradient again from the logits and
 // the forward's statistics.  Work item: one of `pieces` pieces of a row.
 template <typename T>
@@ -486,7 +1044,7 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const Args a, int
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ float teacher_scratch[kWarps];
   float* teacher_p0 = reinterpret_cast<float*>(smem_raw);
-  const TeacherSmem teacher{teacher_p0, reinterpret_cast<int*>(teacher_p0 + a.K), teacher_scratch};
+  const TeacherSmem teacher{teacher_p0, reinterpret_cast<int*>(teacher_p0 + padded_top(a.K)), teacher_scratch};
   const int tid = int(threadIdx.x);
   if (a.skip_ones && a.reduction != kNone && *a.upstream == 1.f) return;
   for (long long item = blockIdx.x; item < a.N * pieces; item += gridDim.x) {
@@ -512,8 +1070,9 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const Args a, int
       continue;
     }
     const float c = kLog2e / a.tau;
-    const float m = a.stats[2 * r], l2s = a.stats[2 * r + 1];
+    const Prob<T> q(c, a.stats[2 * r], a.stats[2 * r + 1]);
     const float f = tch.bad ? __int_as_float(0x7fc00000) : up * w * a.tau;
+    const float off = f > 0.f ? grad_offset(q, f) : 0.f;
     const uint4* src = reinterpret_cast<const uint4*>(row + part.head);
     constexpr int U = 4;
     for (long long i0 = v0 + tid; i0 < v1; i0 += U * kThreads) {
@@ -524,12 +1083,14 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const Args a, int
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + u * kThreads < v1)
-          put_vec<T>(out + part.head + (i0 + u * kThreads) * E, grad_vec<T>(x[u], m, c, l2s, f), out_aligned);
+          put_vec<T>(out + part.head + (i0 + u * kThreads) * E,
+                     q.plain && f > 0.f ? grad_vec<T, true>(x[u], q, f, off) : grad_vec<T, false>(x[u], q, f, 0.f),
+                     out_aligned);
     }
-    if (first && tid < part.head) store1(out + tid, f * ex2((load1(row + tid) - m) * c - l2s));
+    if (first && tid < part.head) store1(out + tid, f * q(load1(row + tid)));
     if (last && tid < part.tail) {
       const long long i = part.head + part.vecs * E + tid;
-      store1(out + i, f * ex2((load1(row + i) - m) * c - l2s));
+      store1(out + i, f * q(load1(row + i)));
     }
     __syncthreads();
     const long long lo = first ? 0 : part.head + v0 * E;
@@ -537,8 +1098,7 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const Args a, int
     for (int k = tid; k < a.K; k += kThreads) {
       const int id = teacher.id[k];
       if (id < lo || id >= hi) continue;
-      const float q = ex2((load1(row + id) - m) * c - l2s);
-      store1(out + id, f * (q - teacher_p(teacher, a.K, k)));
+      store1(out + id, f * (q(load1(row + id)) - teacher_p(teacher, a.K, k)));
     }
   }
 }
@@ -547,12 +1107,15 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const Args a, int
 // host
 // ---------------------------------------------------------------------------
 
-// Shared memory a CTA holds of a row: up to 72 KB, so that three CTAs fit on an
-// SM and one's loads overlap another's arithmetic; slices of rows that are
-// longer than that times the largest cluster take up to 208 KB.
+// distill_row_kernel: shared memory a CTA holds of a row, up to 72 KB, so that
+// three CTAs fit on an SM and one's loads overlap another's arithmetic; slices
+// of rows that are longer than that times the largest cluster take up to 208 KB.
 constexpr long long kSliceVecs = 72 * 1024 / 16;
 constexpr long long kTileVecs = 208 * 1024 / 16;
 constexpr size_t kTopBytes = size_t(kMaxTop) * 8;
+// distill_stream_kernel: dynamic shared memory of a CTA, three to a SM.
+constexpr size_t kStreamSmem = 73 * 1024;
+constexpr long long kStreamMinBytes = 16 * 1024;
 
 b2_status check_args(const char* who, const Args& a, int dtype, int t_dtype, int ids_dtype) {
   if (a.N < 0 || a.V < 1 || a.K < 0) return set_error(B2_ERR_INVALID, "%s: bad shape", who);
@@ -569,41 +1132,81 @@ b2_status check_args(const char* who, const Args& a, int dtype, int t_dtype, int
   return B2_OK;
 }
 
-template <typename T, bool GRAD>
-b2_status launch_fwd(Args a, cudaStream_t st) {
-  int dev = 0;
-  B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
-  const long long vecs = (a.V * (long long)sizeof(T) + 15) / 16;
-  int cluster = 1;
-  // longer rows over more CTAs; so are few rows, down to 4 KB a CTA
-  while (cluster < kMaxCluster && ((vecs + cluster - 1) / cluster > kSliceVecs ||
-                                   (a.N * cluster < sm_count(dev) && vecs / cluster >= 512)))
-    cluster *= 2;
-  a.slice = (vecs + cluster - 1) / cluster;
-  a.tile = std::min(a.slice, a.slice <= kSliceVecs ? kSliceVecs : kTileVecs);
-  const size_t smem = size_t(a.tile) * 16 + size_t(a.K) * 8;
-  auto kern = distill_fwd_kernel<T, GRAD>;
-  static bool configured[64] = {};
+// Once per kernel and device (`done`: a static of the caller).
+template <typename F>
+b2_status allow_smem(F kern, size_t bytes, bool (&done)[64], int dev) {
   if (dev < 0 || dev >= 64) return set_error(B2_ERR_INVALID, "device index %d", dev);
-  if (!configured[dev]) {
-    B2_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           int(kTileVecs * 16 + kTopBytes)),
-                      "cudaFuncSetAttribute(distill)"));
-    configured[dev] = true;
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(a.N * cluster));
-  cfg.blockDim = dim3(kThreads);
+  if (done[dev]) return B2_OK;
+  B2_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)),
+                    "cudaFuncSetAttribute(distill)"));
+  done[dev] = true;
+  return B2_OK;
+}
+
+void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, long long clusters, int cluster, int threads,
+                    size_t smem, cudaStream_t st) {
+  cfg.gridDim = dim3(unsigned(clusters * cluster));
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = unsigned(cluster);
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, cluster), "distill forward launch");
+}
+
+template <typename K, typename... A>
+b2_status launch_clusters(K kern, long long clusters, int cluster, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cluster_config(cfg, attr, clusters, cluster, threads, smem, st);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), "distill forward launch");
+}
+
+template <typename T, bool GRAD>
+b2_status launch_fwd(Args a, cudaStream_t st) {
+  int dev = 0;
+  B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  const int sms = sm_count(dev);
+  const long long vecs = (a.V * (long long)sizeof(T) + 15) / 16;
+  int cluster = 1;
+  const size_t top = size_t(padded_top(a.K)) * 8;
+  while (cluster < kMaxCluster && size_t((vecs + cluster - 1) / cluster) * 16 + 2 * top > kStreamSmem) cluster *= 2;
+  a.slice = (vecs + cluster - 1) / cluster;
+  const size_t per_row = size_t(a.slice) * 16 + top;
+  const int ring = kStreamSmem > top ? int(std::min<size_t>(kRing, (kStreamSmem - top) / per_row)) : 0;
+  // Persistent clusters where every CTA gets several slices of a good size.
+  if (ring >= 1 && a.slice * 16 >= kStreamMinBytes && a.N * cluster >= 2LL * kStreamPerSm * sms) {
+    auto kern = distill_stream_kernel<T, GRAD>;
+    static bool configured[64] = {};
+    B2_TRY(allow_smem(kern, kStreamSmem, configured, dev));
+    // as many clusters as are resident at once: a later one would run alone at the end
+    static int resident[64][kMaxCluster + 1] = {};
+    int& clusters = resident[dev][cluster];
+    if (!clusters) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute attr{};
+      cluster_config(cfg, attr, kStreamPerSm * sms / cluster, cluster, kStreamThreads, kStreamSmem, st);
+      int n = 0;
+      B2_TRY(check_cuda(cudaOccupancyMaxActiveClusters(&n, kern, &cfg), "cudaOccupancyMaxActiveClusters"));
+      if (n < 1) return set_error(B2_ERR_CUDA, "distill: no cluster of %d fits", cluster);
+      clusters = std::min(n, kStreamPerSm * sms / cluster);
+    }
+    return launch_clusters(kern, clusters, cluster, kStreamThreads, ring * per_row + top, st, a, cluster, ring);
+  }
+  // longer rows over more CTAs; so are few rows, down to 4 KB a CTA
+  cluster = 1;
+  while (cluster < kMaxCluster && ((vecs + cluster - 1) / cluster > kSliceVecs ||
+                                   (a.N * cluster < sms && vecs / cluster >= 512)))
+    cluster *= 2;
+  a.slice = (vecs + cluster - 1) / cluster;
+  a.tile = std::min(a.slice, a.slice <= kSliceVecs ? kSliceVecs : kTileVecs);
+  auto kern = distill_row_kernel<T, GRAD>;
+  static bool configured[64] = {};
+  B2_TRY(allow_smem(kern, size_t(kTileVecs) * 16 + kTopBytes, configured, dev));
+  return launch_clusters(kern, a.N, cluster, kThreads, size_t(a.tile) * 16 + top, st, a, cluster);
 }
 
 template <typename T>
@@ -614,7 +1217,7 @@ b2_status launch_bwd(Args a, cudaStream_t st) {
   const int pieces = int(std::max<long long>(1, std::min<long long>(64, vecs / 2048)));
   a.slice = (vecs + pieces - 1) / pieces;
   const long long grid = std::min<long long>(a.N * pieces, (long long)sm_count(dev) * 8);
-  distill_bwd_kernel<T><<<unsigned(grid), kThreads, size_t(a.K) * 8, st>>>(a, pieces);
+  distill_bwd_kernel<T><<<unsigned(grid), kThreads, size_t(padded_top(a.K)) * 8, st>>>(a, pieces);
   return check_cuda(cudaGetLastError(), "distill backward launch");
 }
 

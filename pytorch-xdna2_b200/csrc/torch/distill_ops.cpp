@@ -39,20 +39,17 @@ Call check(const at::Tensor& logits, const at::Tensor& teacher, const at::Tensor
   TORCH_CHECK(teacher.dim() == logits.dim() &&
                   teacher.sizes().slice(0, teacher.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
               kOp, ": teacher_logits ", teacher.sizes(), " must have the rows of logits ", logits.sizes());
-  TORCH_CHECK(!(at::GradMode::is_enabled() && teacher.requires_grad()), kOp,
-              ": teacher_logits are constants of the loss; detach() them");
   TORCH_CHECK(tau > 0 && std::isfinite(tau), kOp, ": temperature must be positive, not ", tau);
   const int64_t V = logits.size(-1), K = teacher.size(-1), N = logits.numel() / V;
-  Call c{as_rows(logits.detach(), N, V), as_rows(teacher.detach(), N, K), as_rows(ids, N, K), at::Tensor(), tau,
+  Call c{as_rows(logits, N, V), as_rows(teacher, N, K), as_rows(ids, N, K), at::Tensor(), tau,
          reduction};
   if (weight.has_value() && weight->defined()) {
     check_device(kOp, *weight, "row_weight", dev);
     TORCH_CHECK(weight->scalar_type() == at::kFloat, kOp, ": row_weight must be float32, not ", weight->scalar_type());
     TORCH_CHECK(weight->sizes() == logits.sizes().slice(0, logits.dim() - 1), kOp, ": row_weight ", weight->sizes(),
                 " must have one value for each row of logits ", logits.sizes());
-    TORCH_CHECK(!(at::GradMode::is_enabled() && weight->requires_grad()), kOp,
-                ": row_weight is a constant of the loss; detach() it");
-    c.weight = weight->detach().reshape({N}).contiguous();
+    at::NoGradGuard no_grad;
+    c.weight = weight->dim() == 1 && weight->is_contiguous() ? *weight : weight->reshape({N}).contiguous();
   }
   for (const at::Tensor* t : {&c.z, &c.t, &c.ids, &c.weight})
     if (t->defined()) materialize(*t);
@@ -73,22 +70,24 @@ std::vector<int64_t> loss_sizes(const at::Tensor& logits, int64_t reduction) {
   return logits.sizes().slice(0, logits.dim() - 1).vec();
 }
 
-// loss and stats; dz may be undefined
+// the loss, and the buffer whose last 2N + 1 values are its statistics; dz may be undefined
 std::pair<at::Tensor, at::Tensor> run_fwd(const Call& c, at::IntArrayRef loss_shape, const at::Tensor& dz) {
   const c10::Device dev = c.z.device();
   c10::cuda::CUDAGuard g(dev.index());
   const int64_t N = c.z.size(0), V = c.z.size(1), K = c.t.size(1);
   at::Tensor loss = empty(loss_shape, at::kFloat, dev.index());
-  at::Tensor stats = empty({2 * N + 1}, at::kFloat, dev.index());
-  at::Tensor ws = empty({int64_t(b2_distill_workspace_bytes(N))}, at::kByte, dev.index());
+  // one allocation: the workspace, then what the backward needs
+  const int64_t scratch = (int64_t(b2_distill_workspace_bytes(N)) + 15) / 16 * 4;
+  at::Tensor stats = empty({scratch + 2 * N + 1}, at::kFloat, dev.index());
   const cudaStream_t st = stream(dev.index());
   KernelTimer kt("lm.distill", double(N) * double(V) * double(c.z.element_size()) * (dz.defined() ? 2.0 : 1.0), st);
   XDNA_B2(b2_distill_loss_fwd(c.z.data_ptr(), row_stride(c.z), float_code(c.z.scalar_type()), N, V, c.t.data_ptr(),
                               row_stride(c.t), float_code(c.t.scalar_type()), c.ids.data_ptr(), row_stride(c.ids),
                               index_code(c.ids.scalar_type()), K, float(c.tau),
                               c.weight.defined() ? c.weight.data_ptr<float>() : nullptr, int(c.reduction),
-                              loss.data_ptr<float>(), stats.data_ptr<float>(), dz.defined() ? dz.data_ptr() : nullptr,
-                              dz.defined() ? row_stride(dz) : V, ws.data_ptr(), size_t(ws.numel()), st));
+                              loss.data_ptr<float>(), stats.data_ptr<float>() + scratch,
+                              dz.defined() ? dz.data_ptr() : nullptr, dz.defined() ? row_stride(dz) : V,
+                              stats.data_ptr(), size_t(scratch) * 4, st));
   count_launch("lm.distill");
   return {loss, stats};
 }
@@ -132,16 +131,16 @@ class Distill : public torch::autograd::Function<Distill> {
       }
       const int64_t N = c.z.size(0), V = c.z.size(1), K = c.t.size(1);
       materialize(grads[0]);
-      const at::Tensor up = grads[0].reshape({-1}).contiguous();
+      const at::Tensor up = grads[0].contiguous();
       const cudaStream_t st = stream(dev.index());
       XDNA_B2(b2_distill_loss_bwd(c.z.data_ptr(), row_stride(c.z), float_code(c.z.scalar_type()), N, V,
                                   c.t.data_ptr(), row_stride(c.t), float_code(c.t.scalar_type()), c.ids.data_ptr(),
                                   row_stride(c.ids), index_code(c.ids.scalar_type()), K, float(c.tau),
                                   c.weight.defined() ? c.weight.data_ptr<float>() : nullptr, int(c.reduction),
-                                  stats.data_ptr<float>(), up.data_ptr<float>(), first ? 1 : 0, dz.data_ptr(),
+                                  stats.data_ptr<float>() + (stats.numel() - (2 * N + 1)), up.data_ptr<float>(), first ? 1 : 0, dz.data_ptr(),
                                   row_stride(dz), st));
       count_launch("lm.distill_bwd");
-      out = dz.reshape(saved[0].sizes());
+      out = dz.sizes() == saved[0].sizes() ? dz : dz.reshape(saved[0].sizes());
     }
     return {out, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
@@ -149,9 +148,12 @@ class Distill : public torch::autograd::Function<Distill> {
 
 at::Tensor distill_loss(const at::Tensor& logits, const at::Tensor& teacher, const at::Tensor& ids, double tau,
                         const std::optional<at::Tensor>& weight, int64_t reduction) {
-  if (at::GradMode::is_enabled() && logits.requires_grad()) {
-    check(logits, teacher, ids, weight, tau, reduction);  // refusals of teacher and weight gradients need grad mode
-    return Distill::apply(logits, teacher, ids, weight, tau, reduction);
+  // (the refusals below need grad mode, which is off inside apply)
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK(!teacher.requires_grad(), kOp, ": teacher_logits are constants of the loss; detach() them");
+    TORCH_CHECK(!weight.has_value() || !weight->requires_grad(), kOp,
+                ": row_weight is a constant of the loss; detach() it");
+    if (logits.requires_grad()) return Distill::apply(logits, teacher, ids, weight, tau, reduction);
   }
   const Call c = check(logits, teacher, ids, weight, tau, reduction);
   return run_fwd(c, loss_sizes(logits, reduction), at::Tensor()).first;

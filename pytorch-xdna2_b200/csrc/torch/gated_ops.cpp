@@ -33,10 +33,10 @@ Call check(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, cons
               wg.sizes(), ", w_up ", wu.sizes(), " and w_down ", wd.sizes(),
               " do not fit: [..., D], [F, D], [F, D] and [E, F] are wanted");
   for (const at::Tensor* t : {&x, &wg, &wu, &wd}) materialize(*t);
-  c.x = as_rows(x.detach(), c.M, c.D);
-  c.wg = as_rows(wg.detach(), c.F, c.D);
-  c.wu = as_rows(wu.detach(), c.F, c.D);
-  c.wd = as_rows(wd.detach(), c.E, c.F);
+  c.x = as_rows(x, c.M, c.D);
+  c.wg = as_rows(wg, c.F, c.D);
+  c.wu = as_rows(wu, c.F, c.D);
+  c.wd = as_rows(wd, c.E, c.F);
   return c;
 }
 

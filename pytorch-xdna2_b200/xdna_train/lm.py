@@ -24,13 +24,19 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
+_C = None
+
+
 def _native(t: torch.Tensor):
     """The extension when ``t`` runs on its kernels, else None (plain path)."""
-    if t.device.type == "cpu":
+    global _C
+    if t.is_cpu:
         return None
-    from . import device
-    device.register_xdna_device()
-    return device._C if device._C.npu_mode() > 0 else None
+    if _C is None:
+        from . import device
+        device.register_xdna_device()
+        _C = device._C
+    return _C if _C.npu_mode() > 0 else None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,

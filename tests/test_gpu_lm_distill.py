@@ -28,11 +28,11 @@ UNIT = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -22}
 def reference(z, t, ids, tau, w, reduction):
     """(loss, gradient for an upstream gradient of 1, per-element bound of its error before the last rounding)"""
     N, V = z.shape
-    z, t = z.double() / tau, t.double() / tau
+    z, t, ids = z.cuda().double() / tau, t.cuda().double() / tau, ids.cuda()
     q = torch.softmax(z, 1)
     logq = torch.log_softmax(z, 1)
     t = t.masked_fill(ids < 0, -math.inf)
-    has = (t > -math.inf).any(1) | t.isnan().any(1) if t.shape[1] else torch.zeros(N, dtype=torch.bool)
+    has = (t > -math.inf).any(1) | t.isnan().any(1) if t.shape[1] else torch.zeros(N, dtype=torch.bool, device="cuda")
     p = torch.zeros_like(t)
     if t.shape[1]:
         p[has] = torch.softmax(t[has], 1)
@@ -40,7 +40,7 @@ def reference(z, t, ids, tau, w, reduction):
     terms = torch.where(p == 0, 0.0, p * (torch.log(p) - logq.gather(1, at)))
     rows = tau ** 2 * terms.sum(1)
     target = torch.zeros_like(q).scatter_add_(1, at, p)
-    w = torch.ones(N, dtype=torch.float64) if w is None else w.double()
+    w = torch.ones(N, dtype=torch.float64, device="cuda") if w is None else w.cuda().double()
     on = has & (w != 0)
     rows = torch.where(on, rows * w, 0.0)
     f = w if reduction != "mean" else w / w.sum() if w.sum() != 0 else torch.zeros_like(w)
@@ -79,16 +79,16 @@ def check(z, t, ids, tau, w, reduction, dev, upstream=None, lo=0, hi=None):
     wsum = float(len(z)) if w is None else w.double().sum().item()
     bound = (tau ** 2 * 2e-5 * (1.0 if reduction == "none" else wsum) + 2e-6 * (ref_rows if reduction == "none"
              else ref_rows.sum())) * scale + 1e-30
-    got = loss.detach().double().cpu()
+    got = xdna_train.as_cuda(loss.detach()).double()
     fine = ref.isfinite()
     assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.isinf(), ref.isinf())
     assert ((got - ref).abs() <= bound)[fine].all() if ref.dim() else (not fine or abs(got - ref) <= bound)
     up = torch.ones_like(loss) if upstream is None else upstream.to(dev)
     (dz,) = torch.autograd.grad(loss, [zd], up)
-    upc = up.double().cpu()
+    upc = xdna_train.as_cuda(up).double()
     upc = upc[:, None] if upc.dim() else upc
     ref = grad * upc
-    got = dz.double().cpu()
+    got = xdna_train.as_cuda(dz).double()
     assert dz.dtype == dtype and dz.shape == zd.shape
     fine = ref.isfinite()
     assert torch.equal(got.isnan(), ref.isnan())
@@ -108,6 +108,36 @@ SHAPES = [  # rows, vocabulary, entries
 def test_loss_and_gradient(dev, N, V, K, dtype, reduction, tau):
     z, t, ids, w = make(N, V, K, dtype, N + V + K)
     check(z, t, ids, tau, w if reduction != "sum" else None, reduction, dev)
+
+
+# many long rows: the persistent kernel, alone and in clusters of 2, 4 and 8, aligned rows and rows of any alignment
+MANY = [(1000, 9001, 7), (950, 20000, 9), (900, 32768, 33), (460, 40001, 17), (250, 131072, 64), (131, 262139, 5),
+        (450, 36000, 1024)]
+
+
+@pytest.mark.parametrize("N,V,K", MANY)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows(dev, N, V, K, dtype):
+    g = torch.Generator().manual_seed(N)
+    z = (torch.randn(N, V, generator=g) * 3).to(dtype)
+    ids = (torch.randint(0, V, (N, 1), generator=g) + torch.arange(K) * (V // K)) % V  # distinct
+    t = (torch.randn(N, K, generator=g) * 3).to(dtype)
+    ids[torch.rand(N, K, generator=g) < 0.1] = -1
+    ids[5:8] = -1
+    t[torch.rand(N, K, generator=g) < 0.1] = -math.inf
+    w = torch.rand(N, generator=g) * (torch.rand(N, generator=g) > 0.3)
+    w[-3:] = 0
+    z[0, 3] = z[1, V - 1] = -math.inf
+    z[w == 0] = math.nan
+    if K > 4:
+        ids[2, 3] = ids[2, 0]              # a repeated entry
+    check(z, t, ids, 1.0, w, "mean", dev)
+    w[:] = 1
+    z = z.nan_to_num(nan=1.0, neginf=-math.inf)
+    z[9, 4] = math.nan
+    z[10] = -math.inf
+    z[11, V - 2] = math.inf
+    check(z, t, ids, 2.0, None, "none", dev)
 
 
 @pytest.mark.parametrize("reduction", ["mean", "none"])
