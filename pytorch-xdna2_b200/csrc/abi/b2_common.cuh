@@ -84,6 +84,35 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 }
 
 // ---------------------------------------------------------------------------
+// programmatic dependence between the kernels of one call
+// ---------------------------------------------------------------------------
+// `chain_wait` returns when the kernels before this one in the stream have
+// ended and their writes are visible; `chain_release` lets the next one be set
+// up on SMs that have room.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launches with programmatic dependence: the kernel may be set up while the one
+// before it in the stream still runs, and waits for that one's end at its own
+// chain_wait, which stands before its first access to memory that an earlier
+// kernel may write or still read.
+template <typename... P, typename... A>
+b2_status launch_chained(void (*kern)(P...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, const char* what,
+                         const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, P(args)...), what);
+}
+
+// ---------------------------------------------------------------------------
 // mbarrier
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {

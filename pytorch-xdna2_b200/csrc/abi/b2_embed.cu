@@ -181,57 +181,48 @@ __device__ __forceinline__ void rank_items(SortSmem& s, const uint32_t (&key)[I]
   __syncthreads();
 }
 
-// Whole sort in one CTA (T <= 1024 * I): every pass goes through shared memory.
-template <int I>
-__global__ void __launch_bounds__(kSortThreads, 1)
-    embed_sort_one_kernel(const void* __restrict__ ids, int is64, int tokens, long long V, long long pad, int passes,
-                          int bits, uint32_t* __restrict__ key_out, uint32_t* __restrict__ tok_out) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
-  uint32_t* skey = reinterpret_cast<uint32_t*>(smem_raw + sizeof(SortSmem));
-  uint32_t* stok = skey + kSortThreads * I;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t key[I], tok[I], rank[I];
-  bool valid[I];
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const int pos = warp * 32 * I + i * 32 + lane;
-    valid[i] = pos < tokens;
-    tok[i] = uint32_t(pos);
-    key[i] = valid[i] ? key_of(ids, is64, pos, V, pad) : 0;
+// Up to kRankTokens tokens: a token's place is the number of smaller keys and of
+// equal keys before it, counted over all keys in shared memory by kRankSplit
+// threads a token.  Quadratic, but one launch over all SMs: 8192 tokens are 67 M
+// comparisons, about 4 us, where a radix sort in one CTA took 10 us for 3000.
+constexpr int kRankTokens = 8192;
+constexpr int kRankThreads = 256;
+constexpr int kRankSplit = 8;
+constexpr int kRankPerBlock = kRankThreads / kRankSplit;
+__global__ void __launch_bounds__(kRankThreads)
+    embed_rank_kernel(const void* __restrict__ ids, int is64, int tokens, long long V, long long pad,
+                      uint32_t* __restrict__ key_out, uint32_t* __restrict__ tok_out) {
+  __shared__ __align__(16) uint32_t keys[kRankTokens];
+  chain_release();
+  const int quads = (tokens + 3) / 4;
+  for (int i = threadIdx.x; i < quads * 4; i += kRankThreads)
+    keys[i] = i < tokens ? key_of(ids, is64, i, V, pad) : 0xffffffffu;
+  __syncthreads();
+  const int part = threadIdx.x % kRankSplit;
+  const int first = blockIdx.x * kRankPerBlock;          // this CTA's tokens, a multiple of 4
+  const int t = first + threadIdx.x / kRankSplit;
+  const uint32_t mine = t < tokens ? keys[t] : 0;
+  unsigned rank = 0;
+  const uint4* q = reinterpret_cast<const uint4*>(keys);
+  // keys before this CTA's tokens count when equal, keys behind them do not
+  const int before = first / 4, behind = (first + kRankPerBlock) / 4;
+#pragma unroll 4
+  for (int i = part; i < before; i += kRankSplit) {
+    const uint4 v = q[i];
+    rank += unsigned(v.x <= mine) + unsigned(v.y <= mine) + unsigned(v.z <= mine) + unsigned(v.w <= mine);
   }
-  const uint32_t mask = (1u << bits) - 1;
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * bits;
-    rank_items<I>(s, key, valid, shift, mask, rank);
-    const uint32_t total = threadIdx.x <= mask ? s.digit[threadIdx.x] : 0;
-    const uint32_t base = scan512(total, s.scan);
-    if (threadIdx.x <= mask) s.digit[threadIdx.x] = base;
-    __syncthreads();
-    const bool last = p + 1 == passes;
+#pragma unroll 4
+  for (int i = behind + part; i < quads; i += kRankSplit) {
+    const uint4 v = q[i];
+    rank += unsigned(v.x < mine) + unsigned(v.y < mine) + unsigned(v.z < mine) + unsigned(v.w < mine);
+  }
+  for (int i = first + part; i < min(first + kRankPerBlock, tokens); i += kRankSplit)
+    rank += unsigned(keys[i] < mine || (keys[i] == mine && i < t));
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      if (!valid[i]) continue;
-      const uint32_t d = (key[i] >> shift) & mask;
-      const uint32_t pos = s.digit[d] + s.count[warp][d] + rank[i];
-      if (last) {
-        key_out[pos] = key[i];
-        tok_out[pos] = tok[i];
-      } else {
-        skey[pos] = key[i];
-        stok[pos] = tok[i];
-      }
-    }
-    if (last) break;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const int pos = warp * 32 * I + i * 32 + lane;
-      if (valid[i]) {
-        key[i] = skey[pos];
-        tok[i] = stok[pos];
-      }
-    }
+  for (int o = 1; o < kRankSplit; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+  if (part == 0 && t < tokens) {
+    key_out[rank] = mine;
+    tok_out[rank] = uint32_t(t);
   }
 }
 
@@ -242,6 +233,7 @@ __global__ void __launch_bounds__(kSortThreads)
     embed_hist_kernel(const void* __restrict__ ids, int is64, long long tokens, long long V, long long pad, int passes,
                       int bits, int chunk, uint32_t* __restrict__ table) {
   __shared__ uint32_t h[kDigits];
+  chain_release();
   const uint32_t mask = (1u << bits) - 1;
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) h[d] = 0;
   __syncthreads();
@@ -264,6 +256,8 @@ __global__ void __launch_bounds__(kSortThreads)
                       uint32_t* __restrict__ tok_out) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
+  chain_wait();
+  chain_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int shift = pass * bits;
   const uint32_t mask = (1u << bits) - 1;
@@ -355,6 +349,7 @@ __global__ void __launch_bounds__(kAccThreads)
                      const T* __restrict__ dy, long long lddy, int vecs, int log_lanes, long long D, float scale,
                      T* __restrict__ dw, float* __restrict__ partial, long long pieces, int slabs,
                      long long acc_blocks, int zero_rows) {
+  chain_wait();
   if ((long long)blockIdx.x >= acc_blocks) {
     __shared__ uint8_t present[512];
     const long long r0 = ((long long)blockIdx.x - acc_blocks) * zero_rows;
@@ -367,17 +362,28 @@ __global__ void __launch_bounds__(kAccThreads)
       if (in) present[key[p] - r0] = 1;
       if (!__syncthreads_or(in)) break;
     }
-    const int lane = threadIdx.x & ((1 << log_lanes) - 1);
-    for (int r = threadIdx.x >> log_lanes; r < rows; r += kAccThreads >> log_lanes) {
-      if (present[r]) continue;
-      auto* out = reinterpret_cast<typename Pack<T, N>::V*>(dw + (r0 + r) * D);
-      for (int c = lane; c < vecs; c += 1 << log_lanes) {
-        Pack<T, N> z;
+    __syncthreads();
+    // the rows' elements as one range: its whole 16-byte vectors, whatever the
+    // row length (a vector over two rows goes element by element)
+    constexpr int E = 16 / sizeof(T);
+    T* base = dw + r0 * D;
+    const unsigned total = unsigned(rows * D), width = unsigned(D);  // about 64 KB, or one row
+    const unsigned head = min(total, unsigned((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / unsigned(sizeof(T)));
+    const unsigned whole = (total - head) / E;
+    for (unsigned v = threadIdx.x; v < whole; v += kAccThreads) {
+      const unsigned e0 = head + v * E;
+      const unsigned first_row = e0 / width, last_row = (e0 + E - 1) / width;
+      if (first_row == last_row) {
+        if (!present[first_row]) *reinterpret_cast<uint4*>(base + e0) = make_uint4(0, 0, 0, 0);
+      } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z.e[i] = T(0);
-        out[c] = z.v;
+        for (int i = 0; i < E; ++i)
+          if (!present[(e0 + i) / width]) base[e0 + i] = T(0);
       }
     }
+    const unsigned tail = head + whole * E;
+    if (threadIdx.x < head && !present[threadIdx.x / width]) base[threadIdx.x] = T(0);
+    if (threadIdx.x < total - tail && !present[(tail + threadIdx.x) / width]) base[tail + threadIdx.x] = T(0);
     return;
   }
   const int per_block = kAccThreads >> log_lanes;
@@ -433,12 +439,17 @@ __global__ void __launch_bounds__(kAccThreads)
   }
 }
 
-// Adds the partial rows of every run that crosses pieces, in piece order.  The
-// CTA of the piece in which the run starts does it.
+// Adds the partial rows of every run that crosses pieces.  The CTA of the piece
+// in which the run starts does it, for 32 vectors of columns: its warps take
+// every eighth piece each (a frequent token's run crosses hundreds), four rows'
+// loads in flight, and their sums are added in warp order.
 template <typename T, int N>
 __global__ void __launch_bounds__(kAccThreads)
     embed_join_kernel(const uint32_t* __restrict__ key, long long tokens, long long V, int vecs, long long D,
                       float scale, T* __restrict__ dw, const float* __restrict__ partial, long long pieces) {
+  constexpr int kJoinWarps = kAccThreads / 32;
+  __shared__ float sums[kJoinWarps][N][32];
+  chain_wait();
   const long long piece = blockIdx.x;
   const long long p0 = piece * kPiece, p1 = p0 + kPiece;
   if (p1 >= tokens) return;  // the last piece's runs all end in it
@@ -453,19 +464,29 @@ __global__ void __launch_bounds__(kAccThreads)
     else hi = mid;
   }
   const long long last = lo;
-  for (int c = blockIdx.y * kAccThreads + threadIdx.x; c < vecs; c += gridDim.y * kAccThreads) {
-    float acc[N];
-    const float* own_part = partial + (2 * piece + 1) * D + (long long)c * N;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = blockIdx.y * 32 + lane;
+  float acc[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = own_part[i];
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  if (c < vecs) {
+    // slot 1 of the piece where the run starts, slot 0 of the others
 #pragma unroll 4
-    for (long long q = piece + 1; q <= last; ++q) {
-      const float* pp = partial + (2 * q) * D + (long long)c * N;
+    for (long long q = piece + warp; q <= last; q += kJoinWarps) {
+      const float* pp = partial + (2 * q + (q == piece ? 1 : 0)) * D + (long long)c * N;
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] += pp[i];
     }
-    store_row<T, N>(dw + (long long)k * D, c, acc, scale);
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) sums[warp][i][lane] = acc[i];
+  __syncthreads();
+  if (warp != 0 || c >= vecs) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += sums[w][i][lane];
+  store_row<T, N>(dw + (long long)k * D, c, acc, scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -490,7 +511,7 @@ int log_lanes_for(int vecs) {
 
 struct SortPlan {
   int passes, bits;
-  bool one;      // whole sort in one CTA
+  bool one;      // by counting ranks, in one launch
   int items;     // tokens per thread
   int64_t blocks;
 };
@@ -501,14 +522,9 @@ SortPlan sort_plan(int64_t T, int64_t V) {
   while (bits < 32 && (int64_t(1) << bits) <= V) ++bits;  // keys 0 .. V
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.one = T <= 8 * kSortThreads;
-  if (p.one) {
-    p.items = T <= kSortThreads ? 1 : T <= 2 * kSortThreads ? 2 : T <= 4 * kSortThreads ? 4 : 8;
-    p.blocks = 1;
-  } else {
-    p.items = T <= 128 * 2 * kSortThreads ? 2 : 8;
-    p.blocks = (T + int64_t(p.items) * kSortThreads - 1) / (int64_t(p.items) * kSortThreads);
-  }
+  p.one = T <= kRankTokens;
+  p.items = T <= 128 * 2 * kSortThreads ? 2 : 8;
+  p.blocks = (T + int64_t(p.items) * kSortThreads - 1) / (int64_t(p.items) * kSortThreads);
   return p;
 }
 
@@ -552,17 +568,6 @@ b2_status allow_smem(F kern, size_t bytes, bool (&done)[64]) {
 }
 
 template <int I>
-b2_status sort_one(const void* ids, int is64, int64_t T, int64_t V, int64_t pad, const SortPlan& p, uint32_t* key,
-                   uint32_t* tok, cudaStream_t st) {
-  const size_t smem = sizeof(SortSmem) + size_t(kSortThreads) * I * 8;
-  auto kern = embed_sort_one_kernel<I>;
-  static bool configured[64] = {};
-  B2_TRY(allow_smem(kern, smem, configured));
-  kern<<<1, kSortThreads, smem, st>>>(ids, is64, int(T), V, pad, p.passes, p.bits, key, tok);
-  return check_cuda(cudaGetLastError(), "embedding sort launch");
-}
-
-template <int I>
 b2_status sort_pass(const void* ids, int is64, int64_t T, int64_t V, int64_t pad, const SortPlan& p, int pass,
                     uint32_t* table, const uint32_t* ki, const uint32_t* ti, uint32_t* ko, uint32_t* to,
                     cudaStream_t st) {
@@ -570,9 +575,8 @@ b2_status sort_pass(const void* ids, int is64, int64_t T, int64_t V, int64_t pad
   auto kern = embed_pass_kernel<I>;
   static bool configured[64] = {};
   B2_TRY(allow_smem(kern, smem, configured));
-  kern<<<unsigned(p.blocks), kSortThreads, smem, st>>>(ids, is64, T, V, pad, pass, p.passes, p.bits, table, ki, ti, ko,
-                                                       to);
-  return check_cuda(cudaGetLastError(), "embedding sort pass launch");
+  return launch_chained(kern, dim3(unsigned(p.blocks)), kSortThreads, smem, st, "embedding sort pass launch", ids, is64, T,
+                        V, pad, pass, p.passes, p.bits, table, ki, ti, ko, to);
 }
 
 template <typename T, int N>
@@ -605,15 +609,13 @@ b2_status run_acc(const uint32_t* key, const uint32_t* tok, int64_t tokens, int6
   const int zr = int(std::max<int64_t>(1, std::min<int64_t>(512, 65536 / (D * int64_t(sizeof(T))))));
   const int64_t blocks = acc_blocks + (V + zr - 1) / zr;
   if (blocks > INT32_MAX) return set_error(B2_ERR_UNSUPPORTED, "b2_embedding_bwd: too many rows");
-  embed_acc_kernel<T, N><<<unsigned(blocks), kAccThreads, 0, st>>>(
-      key, tok, tokens, V, static_cast<const T*>(dy), lddy, vecs, ll, D, scale, static_cast<T*>(dw), partial, pieces,
-      slabs, acc_blocks, zr);
-  B2_TRY(check_cuda(cudaGetLastError(), "embedding gradient launch"));
+  B2_TRY(launch_chained(embed_acc_kernel<T, N>, dim3(unsigned(blocks)), kAccThreads, 0, st, "embedding gradient launch",
+                        key, tok, tokens, V, static_cast<const T*>(dy), lddy, vecs, ll, D, scale, static_cast<T*>(dw),
+                        partial, pieces, slabs, acc_blocks, zr));
   if (pieces > 1) {
-    const int by = std::max(1, std::min((vecs + kAccThreads - 1) / kAccThreads, 16));
-    embed_join_kernel<T, N><<<dim3(unsigned(pieces), unsigned(by)), kAccThreads, 0, st>>>(
-        key, tokens, V, vecs, D, scale, static_cast<T*>(dw), partial, pieces);
-    B2_TRY(check_cuda(cudaGetLastError(), "embedding gradient join launch"));
+    B2_TRY(launch_chained(embed_join_kernel<T, N>, dim3(unsigned(pieces), unsigned((vecs + 31) / 32)), kAccThreads, 0,
+                          st, "embedding gradient join launch", key, tokens, V, vecs, D, scale, static_cast<T*>(dw),
+                          static_cast<const float*>(partial), pieces));
   }
   return B2_OK;
 }
@@ -682,12 +684,9 @@ b2_status b2_embedding_bwd(const void* ids, int ids_dtype, int64_t T, const void
   const SortPlan p = sort_plan(T, V);
   uint32_t *key = u32(w.key0), *tok = u32(w.tok0);
   if (p.one) {
-    switch (p.items) {
-      case 1: B2_TRY(sort_one<1>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
-      case 2: B2_TRY(sort_one<2>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
-      case 4: B2_TRY(sort_one<4>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
-      default: B2_TRY(sort_one<8>(ids, is64, T, V, padding_idx, p, key, tok, st)); break;
-    }
+    embed_rank_kernel<<<unsigned((T + kRankPerBlock - 1) / kRankPerBlock), kRankThreads, 0, st>>>(
+        ids, is64, int(T), V, padding_idx, key, tok);
+    B2_TRY(check_cuda(cudaGetLastError(), "embedding rank launch"));
   } else {
     uint32_t* table = u32(w.table);
     embed_hist_kernel<<<unsigned(p.blocks), kSortThreads, 0, st>>>(ids, is64, T, V, padding_idx, p.passes, p.bits,

@@ -151,12 +151,6 @@ __device__ __forceinline__ float4* partial_at(const Problem& q, int tile, int sp
          ((((long long)tile * q.splits + split) * 16 + region) * (PBN / 64) + j) * 256 + lane;
 }
 
-// Programmatic dependence: `wait` returns when the kernels before this one in
-// the stream have ended and their writes are visible, `release` lets the next
-// one be set up.
-__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // A staged 32 x 64 box (128-byte rows, chunk c of row r at c ^ (r & 7)) to output
 // rows that no TMA store can address: the warp writes row after row, 4-byte
 // words in consecutive lanes where the row's parity allows, so that a row's 128
@@ -376,7 +370,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item it = decode(p, t);
       const Problem& q = p.p[it.prob];
       const int row0 = it.mt * 256 + int(rank) * 128 + quarter * 32;
-      const int row = row0 + lane;
       // kGateBwd: this warp's 32-column chunks of the tile; the first one's
       // factors travel while its product is still running
       int chunks = 0;
@@ -1038,26 +1031,6 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int pairs, bool gate, int sms
   return best;
 }
 
-// Launches with programmatic dependence: the kernel may be set up on SMs that
-// the kernel before it in the stream has left while that one still runs, and
-// waits for its end (and its writes) at its own griddepcontrol.wait, which
-// stands before every access to global memory.
-template <typename K, typename... A>
-b2_status launch_chained(K kern, unsigned grid, unsigned block, size_t smem, cudaStream_t st, const char* what,
-                         const A&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
-}
-
 template <int EPI, int PBN, bool A_MN, bool B_MN, int ACT>
 b2_status launch_gemm(const Maps& maps, const Params& p, cudaStream_t st) {
   using C = Config<EPI, PBN>;
@@ -1072,7 +1045,7 @@ b2_status launch_gemm(const Maps& maps, const Params& p, cudaStream_t st) {
     configured[dev] = true;
   }
   const int clusters = std::min(p.items, sm_count(dev) / 2);
-  return launch_chained(kern, 2 * clusters, kThreads, C::kSmem, st, "gated product launch", maps, p);
+  return launch_chained(kern, dim3(2 * clusters), kThreads, C::kSmem, st, "gated product launch", maps, p);
 }
 
 // The gate epilogues' tensors.
@@ -1155,8 +1128,8 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
     }
     const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * ((EPI == kGate ? pbn / 2 : pbn) / 8);
     const unsigned blocks = unsigned(std::min<long long>((units + 7) / 8, 148 * 16));
-    B2_TRY((pbn == 256 ? launch_chained(gated_reduce_kernel<EPI, 256, ACT>, blocks, 256, 0, st, "gated reduce launch", r)
-                       : launch_chained(gated_reduce_kernel<EPI, 128, ACT>, blocks, 256, 0, st, "gated reduce launch", r)));
+    B2_TRY((pbn == 256 ? launch_chained(gated_reduce_kernel<EPI, 256, ACT>, dim3(blocks), 256, 0, st, "gated reduce launch", r)
+                       : launch_chained(gated_reduce_kernel<EPI, 128, ACT>, dim3(blocks), 256, 0, st, "gated reduce launch", r)));
   }
   return B2_OK;
 }
@@ -1276,7 +1249,7 @@ struct Padder {
       if (a.begin[i + 1] - a.begin[i] > UINT32_MAX)
         return set_error(B2_ERR_UNSUPPORTED, "gated_mlp: an operand of unaligned rows is too large to copy");
     const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 255) / 256, 148 * 16));
-    return launch_chained(gated_pad_kernel, blocks, 256, 0, st, "gated pad launch", a);
+    return launch_chained(gated_pad_kernel, dim3(blocks), 256, 0, st, "gated pad launch", a);
   }
 };
 
