@@ -183,9 +183,9 @@ __device__ __forceinline__ void rank_items(SortSmem& s, const uint32_t (&key)[I]
 
 // Up to kRankTokens tokens: a token's place is the number of smaller keys and of
 // equal keys before it, counted over all keys in shared memory by kRankSplit
-// threads a token.  Quadratic, but one launch over all SMs: 8192 tokens are 67 M
-// comparisons, about 4 us, where a radix sort in one CTA took 10 us for 3000.
-constexpr int kRankTokens = 8192;
+// threads a token.  Quadratic, but one launch over all SMs: 3000 tokens take 5 us,
+// where a radix sort in one CTA took 10; 8192 tokens 16 us, the passes below 13.
+constexpr int kRankTokens = 4096;
 constexpr int kRankThreads = 256;
 constexpr int kRankSplit = 8;
 constexpr int kRankPerBlock = kRankThreads / kRankSplit;
@@ -195,6 +195,7 @@ __global__ void __launch_bounds__(kRankThreads)
   __shared__ __align__(16) uint32_t keys[kRankTokens];
   chain_release();
   const int quads = (tokens + 3) / 4;
+#pragma unroll 8
   for (int i = threadIdx.x; i < quads * 4; i += kRankThreads)
     keys[i] = i < tokens ? key_of(ids, is64, i, V, pad) : 0xffffffffu;
   __syncthreads();
@@ -439,54 +440,85 @@ __global__ void __launch_bounds__(kAccThreads)
   }
 }
 
-// Adds the partial rows of every run that crosses pieces.  The CTA of the piece
-// in which the run starts does it, for 32 vectors of columns: its warps take
-// every eighth piece each (a frequent token's run crosses hundreds), four rows'
-// loads in flight, and their sums are added in warp order.
+// Adds the partial rows of every run that crosses pieces, for 32 vectors of
+// columns.  A warp looks after one piece: it finds the end of a run that starts
+// there and goes on (32 pieces a look) and adds a short one's rows by itself, in
+// piece order; a run over more than kShortRun pieces (a frequent token's has
+// hundreds) is shared by the CTA's warps, every eighth piece each, and their
+// sums are added in warp order.
+constexpr int kJoinWarps = kAccThreads / 32;
+constexpr int kShortRun = 16;
 template <typename T, int N>
 __global__ void __launch_bounds__(kAccThreads)
     embed_join_kernel(const uint32_t* __restrict__ key, long long tokens, long long V, int vecs, long long D,
                       float scale, T* __restrict__ dw, const float* __restrict__ partial, long long pieces) {
-  constexpr int kJoinWarps = kAccThreads / 32;
   __shared__ float sums[kJoinWarps][N][32];
+  __shared__ uint32_t long_key[kJoinWarps];
+  __shared__ long long long_last[kJoinWarps];
   chain_wait();
-  const long long piece = blockIdx.x;
-  const long long p0 = piece * kPiece, p1 = p0 + kPiece;
-  if (p1 >= tokens) return;  // the last piece's runs all end in it
-  const uint32_t k = key[p1 - 1];
-  if (k >= V || key[p1] != k) return;                                    // no run goes on
-  if (key[p0] == k && p0 > 0 && key[p0 - 1] == k) return;                // it started earlier
-  // the pieces after this one that start with k are its continuation
-  long long lo = piece + 1, hi = pieces;  // key[lo * kPiece] == k; find the first piece that does not start with k
-  while (lo + 1 < hi) {
-    const long long mid = (lo + hi) / 2;
-    if (key[mid * kPiece] == k) lo = mid;
-    else hi = mid;
-  }
-  const long long last = lo;
+  const uint32_t none = 0xffffffffu;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.y * 32 + lane;
-  float acc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  if (c < vecs) {
-    // slot 1 of the piece where the run starts, slot 0 of the others
-#pragma unroll 4
-    for (long long q = piece + warp; q <= last; q += kJoinWarps) {
-      const float* pp = partial + (2 * q + (q == piece ? 1 : 0)) * D + (long long)c * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += pp[i];
+  const long long first = (long long)blockIdx.x * kJoinWarps, piece = first + warp;
+  const long long p0 = piece * kPiece, p1 = p0 + kPiece;
+  uint32_t k = none;
+  long long last = piece;  // the last piece of the run
+  if (p1 < tokens) {  // the last piece's runs all end in it
+    k = key[p1 - 1];
+    const uint32_t next = key[p1], begin = key[p0], before = p0 > 0 ? key[p0 - 1] : none;
+    if (k >= V || next != k || (begin == k && before == k)) k = none;  // none goes on, or it started earlier
+  }
+  if (k != none) {
+    for (;;) {
+      const long long q = last + 1 + lane;
+      const unsigned same = __ballot_sync(0xffffffffu, q < pieces && key[q * kPiece] == k);
+      const int more = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+      last += more;
+      if (more < 32) break;
     }
   }
+  // slot 1 of the piece where the run starts, slot 0 of the others
+  auto add = [&](float (&acc)[N], long long q, long long start) {
+    const float* pp = partial + (2 * q + (q == start ? 1 : 0)) * D + (long long)c * N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sums[warp][i][lane] = acc[i];
-  __syncthreads();
-  if (warp != 0 || c >= vecs) return;
+    for (int i = 0; i < N; ++i) acc[i] += pp[i];
+  };
+  const bool is_long = k != none && last - piece >= kShortRun;
+  if (k != none && !is_long && c < vecs) {
+    float acc[N];
 #pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w)
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (long long q = piece; q <= last; ++q) add(acc, q, piece);
+    store_row<T, N>(dw + (long long)k * D, c, acc, scale);
+  }
+  if (lane == 0) {
+    long_key[warp] = is_long ? k : none;
+    long_last[warp] = last;
+  }
+  if (!__syncthreads_or(is_long)) return;
+  for (int j = 0; j < kJoinWarps; ++j) {
+    const uint32_t kj = long_key[j];
+    if (kj == none) continue;
+    const long long start = first + j, end = long_last[j];
+    float acc[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += sums[w][i][lane];
-  store_row<T, N>(dw + (long long)k * D, c, acc, scale);
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    if (c < vecs)
+#pragma unroll 4
+      for (long long q = start + warp; q <= end; q += kJoinWarps) add(acc, q, start);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sums[warp][i][lane] = acc[i];
+    __syncthreads();
+    if (warp == 0 && c < vecs) {
+#pragma unroll
+      for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += sums[w][i][lane];
+      store_row<T, N>(dw + (long long)kj * D, c, acc, scale);
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -613,7 +645,8 @@ b2_status run_acc(const uint32_t* key, const uint32_t* tok, int64_t tokens, int6
                         key, tok, tokens, V, static_cast<const T*>(dy), lddy, vecs, ll, D, scale, static_cast<T*>(dw),
                         partial, pieces, slabs, acc_blocks, zr));
   if (pieces > 1) {
-    B2_TRY(launch_chained(embed_join_kernel<T, N>, dim3(unsigned(pieces), unsigned((vecs + 31) / 32)), kAccThreads, 0,
+    B2_TRY(launch_chained(embed_join_kernel<T, N>, dim3(unsigned((pieces + kJoinWarps - 1) / kJoinWarps), unsigned((vecs + 31) / 32)),
+                          kAccThreads, 0,
                           st, "embedding gradient join launch", key, tokens, V, vecs, D, scale, static_cast<T*>(dw),
                           static_cast<const float*>(partial), pieces));
   }

@@ -565,8 +565,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // Adds a problem's partial tiles in split order and finishes them with its
-// epilogue.  A thread takes 8 columns of one row (kGate: of g and of u); the
-// lanes of a warp are 32 rows, so its partial reads are contiguous.
+// epilogue.  Gate epilogues: a thread takes 8 columns of one row (kGate: of g and
+// of u).  kStore: a warp takes 32 rows x 32 columns and writes them, staged,
+// in whole rows (elements of unaligned rows straight from the threads that own
+// the rows took 26 us for 777 x 1001 where this takes 6).  The lanes of a warp
+// are 32 rows, so its partial reads are contiguous.
 struct ReduceArgs {
   Problem q;
   int train;
@@ -602,6 +605,70 @@ __device__ __forceinline__ void put8(uint16_t* dst, const float (&v)[8], int col
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < cols) dst[i] = cvt1(v[i]);
+}
+
+template <int PBN>
+__global__ void __launch_bounds__(256) gated_reduce_store_kernel(const __grid_constant__ ReduceArgs a) {
+  __shared__ __align__(16) uint8_t boxes[8][32 * 64];
+  chain_wait();
+  const Problem& q = a.q;
+  constexpr int kChunks = PBN / 32;
+  const int lane = threadIdx.x & 31;
+  uint8_t* box = boxes[threadIdx.x >> 5];
+  const long long units = (long long)q.tiles_m * q.tiles_n * 8 * kChunks;  // (tile, 32-row block, 32 columns)
+  for (long long w = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5; w < units; w += (long long)gridDim.x * 8) {
+    const int chunk = int(w % kChunks);
+    const long long rest = w / kChunks;
+    const int rows = int(rest % 8);  // rank * 4 + quarter
+    const int tile = int(rest / 8);
+    const int group = tile / (kGroupM * q.tiles_n), first = group * kGroupM;
+    const int gm = min(kGroupM, q.tiles_m - first), in = tile - first * q.tiles_n;
+    const int row0 = (first + in % gm) * 256 + rows * 32, col0 = (in / gm) * PBN + chunk * 32;
+    if (row0 >= q.M || col0 >= q.N) continue;
+    const int half = chunk / (PBN / 64), j = chunk % (PBN / 64);
+    const int region = (rows >> 2) * 8 + half * 4 + (rows & 3);
+    float4 v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int s = 0; s < q.splits; ++s) {
+      const float4* src = partial_at<PBN>(q, tile, s, region, j, lane);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float4 x = __ldcg(src + c * 32);
+        v[c].x += x.x;
+        v[c].y += x.y;
+        v[c].z += x.z;
+        v[c].w += x.w;
+      }
+    }
+    __syncwarp();
+    // 64-byte rows, 16-byte chunk c of row r at c ^ ((r >> 1) & 3)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(cvt2(v[2 * c].x, v[2 * c].y), cvt2(v[2 * c].z, v[2 * c].w),
+                     cvt2(v[2 * c + 1].x, v[2 * c + 1].y), cvt2(v[2 * c + 1].z, v[2 * c + 1].w));
+    __syncwarp();
+    const int nrows = min(32, q.M - row0), cols = min(32, q.N - col0);
+    uint16_t* out = q.out + (long long)row0 * q.ldo + col0;
+    if (q.tma_out && cols == 32) {
+      // aligned rows: four lanes of 16 bytes a row, eight rows at once
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2), c = lane & 3;
+        if (r < nrows)
+          *reinterpret_cast<uint4*>(out + (long long)r * q.ldo + c * 8) =
+              *reinterpret_cast<const uint4*>(box + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+      }
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < nrows; ++r)
+        if (lane < cols)
+          out[(long long)r * q.ldo + lane] = *reinterpret_cast<const uint16_t*>(
+              box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+    }
+  }
 }
 
 template <int EPI, int PBN, int ACT>
@@ -647,23 +714,18 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(const __grid_constant
     } else {
       const int half = oc / (PBN / 16), o = oc % (PBN / 16);
       sum8<PBN>(q, tile, rank * 8 + half * 4 + quarter, o / 4, o & 3, lane, v);
-      if constexpr (EPI == kStore) {
-        uint16_t* dst = q.out + (long long)row * q.ldo + col;
-        put8(dst, v, cols, (reinterpret_cast<uintptr_t>(dst) & 15) == 0);
-      } else {
-        const uint4 pv = *reinterpret_cast<const uint4*>(a.fp + (long long)row * a.ldf + col);
-        const uint4 av = *reinterpret_cast<const uint4*>(a.fa + (long long)row * a.ldf + col);
-        const uint16_t* pe = reinterpret_cast<const uint16_t*>(&pv);
-        const uint16_t* ae = reinterpret_cast<const uint16_t*>(&av);
-        float dg[8], du[8];
+      const uint4 pv = *reinterpret_cast<const uint4*>(a.fp + (long long)row * a.ldf + col);
+      const uint4 av = *reinterpret_cast<const uint4*>(a.fa + (long long)row * a.ldf + col);
+      const uint16_t* pe = reinterpret_cast<const uint16_t*>(&pv);
+      const uint16_t* ae = reinterpret_cast<const uint16_t*>(&av);
+      float dg[8], du[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dg[i] = v[i] * bf2f(pe[i]);
-          du[i] = v[i] * bf2f(ae[i]);
-        }
-        put8(a.o1 + (long long)row * a.ldo + col, dg, cols, true);
-        put8(a.o2 + (long long)row * a.ldo + col, du, cols, true);
+      for (int i = 0; i < 8; ++i) {
+        dg[i] = v[i] * bf2f(pe[i]);
+        du[i] = v[i] * bf2f(ae[i]);
       }
+      put8(a.o1 + (long long)row * a.ldo + col, dg, cols, true);
+      put8(a.o2 + (long long)row * a.ldo + col, du, cols, true);
     }
   }
 }
@@ -694,30 +756,53 @@ struct PadArgs {
 };
 __global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ PadArgs a) {
   chain_wait();
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.begin[a.n]; i += (long long)gridDim.x * 256) {
-    int m = 0;
-    while (i >= a.begin[m + 1]) ++m;
-    const unsigned at = unsigned(i - a.begin[m]);  // below 2^31 groups of a matrix (checked by the host)
-    const unsigned groups = unsigned(a.ldd[m]) / 8;
-    const long long row = at / groups;
-    const int col = int(at - unsigned(row) * groups) * 8;
-    const uint16_t* s = a.src[m] + row * a.lds[m] + col;
-    const uintptr_t addr = reinterpret_cast<uintptr_t>(s);
-    const int shift = int(addr & 15) * 8;  // bits
-    uint4 out;
-    // the two aligned 16-byte words around the 8 elements, where both lie inside this row
-    if (col >= 8 && col + 16 <= a.cols[m]) {
-      const uint4* w = reinterpret_cast<const uint4*>(addr & ~uintptr_t(15));
-      const uint4 lo = w[0];
-      const uint4 hi = shift ? w[1] : lo;
-      out = shift_words(lo, hi, shift);
-    } else {
-      uint16_t v[8];
+  constexpr int U = 4;  // 16-byte groups a thread has in flight
+  const long long total = a.begin[a.n], step = (long long)gridDim.x * 256;
+  for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += U * step) {
+    const uint16_t* src[U];
+    uint4* dst[U];
+    int left[U];  // columns from the group's first
+    bool inner[U];
+    uint4 lo[U], hi[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = col + e < a.cols[m] ? s[e] : uint16_t(0);
-      out = *reinterpret_cast<uint4*>(v);
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * step;
+      left[u] = -1;
+      inner[u] = false;
+      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+      if (i >= total) continue;
+      int m = 0;
+      while (i >= a.begin[m + 1]) ++m;
+      const unsigned at = unsigned(i - a.begin[m]);  // below 2^32 groups of a matrix (checked by the host)
+      const unsigned groups = unsigned(a.ldd[m]) / 8;
+      const unsigned row = at / groups;
+      const int col = int(at - row * groups) * 8;
+      src[u] = a.src[m] + (long long)row * a.lds[m] + col;
+      dst[u] = reinterpret_cast<uint4*>(a.dst[m] + (long long)row * a.ldd[m] + col);
+      left[u] = a.cols[m] - col;
+      // the two aligned 16-byte words around the 8 elements, where both lie inside this row
+      inner[u] = col >= 8 && left[u] >= 16;
+      if (inner[u]) {
+        const uint4* w = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src[u]) & ~uintptr_t(15));
+        lo[u] = __ldg(w);
+        hi[u] = __ldg(w + 1);
+      }
     }
-    *reinterpret_cast<uint4*>(a.dst[m] + row * a.ldd[m] + col) = out;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (left[u] < 0) continue;
+      if (inner[u]) {
+        *dst[u] = shift_words(lo[u], hi[u], int(reinterpret_cast<uintptr_t>(src[u]) & 15) * 8);
+      } else {
+        union {
+          uint4 v;
+          uint16_t e[8];
+        } r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.e[e] = e < left[u] ? src[u][e] : uint16_t(0);
+        *dst[u] = r.v;
+      }
+    }
   }
 }
 
@@ -1126,10 +1211,15 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
       r.ldo = gate->o1.ld;
       r.ldf = gate->ldf;
     }
-    const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * ((EPI == kGate ? pbn / 2 : pbn) / 8);
-    const unsigned blocks = unsigned(std::min<long long>((units + 7) / 8, 148 * 16));
-    B2_TRY((pbn == 256 ? launch_chained(gated_reduce_kernel<EPI, 256, ACT>, dim3(blocks), 256, 0, st, "gated reduce launch", r)
-                       : launch_chained(gated_reduce_kernel<EPI, 128, ACT>, dim3(blocks), 256, 0, st, "gated reduce launch", r)));
+    const long long cols = EPI == kStore ? pbn / 32 : (EPI == kGate ? pbn / 2 : pbn) / 8;  // a warp's unit of columns
+    const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * cols;
+    const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
+    if constexpr (EPI == kStore)
+      B2_TRY((pbn == 256 ? launch_chained(gated_reduce_store_kernel<256>, blocks, 256, 0, st, "gated reduce launch", r)
+                         : launch_chained(gated_reduce_store_kernel<128>, blocks, 256, 0, st, "gated reduce launch", r)));
+    else
+      B2_TRY((pbn == 256 ? launch_chained(gated_reduce_kernel<EPI, 256, ACT>, blocks, 256, 0, st, "gated reduce launch", r)
+                         : launch_chained(gated_reduce_kernel<EPI, 128, ACT>, blocks, 256, 0, st, "gated reduce launch", r)));
   }
   return B2_OK;
 }
