@@ -712,7 +712,8 @@ b2_status b2_distill_loss_bwd(const void* z, int64_t ldz, int dtype, int64_t N,
  * row stride in elements (any; rows that are not 16-byte aligned are copied to
  * the workspace first).  act 0: silu, 1: gelu (erf), 2: relu.  fp32 sums; h is
  * rounded to bf16 as an operand of the second product.  saved (may be NULL): what
- * the backward needs, bf16 [M][3][F rounded up to 8] (h, u act'(g), act(g)),
+ * the backward needs, 16-bit words [M][4][F rounded up to 8] (h as bf16, the
+ * upper halves of u act'(g) and of act(g) as fp32, and the next 8 bits of both),
  * 16-byte aligned.  Workspace: b2_gated_mlp_fwd_workspace_bytes(), 256-byte aligned. */
 size_t b2_gated_mlp_fwd_workspace_bytes(int64_t M, int64_t D, int64_t F,
                                         int64_t E);

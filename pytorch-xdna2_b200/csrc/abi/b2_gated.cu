@@ -21,11 +21,14 @@
 //   kStore     a plain product, up to three of them in one launch; the two
 //              halves of dx are one reduction over 2F whose operands change in
 //              the middle
-// h, P, A, dg and du are rounded to bf16 once each, from fp32: a relative error
-// of at most 2^-8, that of the tensors themselves.  Keeping the factors P and A rather
-// than g and u costs no more room beside h, leaves the backward's epilogue two
-// products instead of an exponential, and is more exact (a rounded g moves
-// act'(g) and with it h, dg and du: 1.8 against 1.2 roundings in dWd).
+// h, dg and du are rounded to bf16 once each, from fp32, as operands of the next
+// product: a relative error of at most 2^-8, that of the tensors themselves.  P
+// and A keep 16 bits of significand -- their upper halves as bf16 patterns, the
+// next 8 bits of both in one 16-bit word R -- so that the backward adds no
+// rounding of its own: with both as bf16 the errors of dx, dWg and dWu were 1.7
+// times those of one rounding at the end, with g and u as bf16 (act' of a
+// rounded g) those of dWd too.  Keeping the factors rather than g and u also
+// leaves the backward's epilogue two products instead of an exponential.
 //
 // Everything is bound by the tensor pipe or, for few tokens, by reading the
 // weights.  Reductions whose tiles would leave most SM pairs idle are split;
@@ -61,13 +64,13 @@ struct Problem {
 };
 
 struct Maps {
-  CUtensorMap a[kMaxProblems], b[kMaxProblems], o[kMaxProblems];
+  CUtensorMap a[kMaxProblems], b[kMaxProblems], o[kMaxProblems + 1];
 };
 
 struct Params {
   Problem p[kMaxProblems];
   int problems, items;
-  int train;  // kGate: write the factors P and A (kGateBwd reads them through maps.a[1] and maps.b[1])
+  int train;  // kGate: write the factors (kGateBwd reads P, A and R through maps.a[1], maps.b[1] and maps.o[0])
   int* status;
 };
 
@@ -106,13 +109,36 @@ __device__ __forceinline__ float act_value(float g) {
   return a;
 }
 
+// The factors P and A as stored: their upper halves (bf16 patterns, truncated)
+// and the next 8 bits of each, P's above A's: 16 bits of significand, truncated
+// (2^-15; rounding would cost the epilogue more instructions than the factors
+// themselves).  A NaN stays one: results of arithmetic carry it in the upper half.
+struct Factors2 {  // of two neighbouring columns
+  uint32_t p, a, r;
+};
+__device__ __forceinline__ Factors2 pack_factors(float p0, float p1, float a0, float a1) {
+  const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1), y0 = __float_as_uint(a0), y1 = __float_as_uint(a1);
+  Factors2 f;
+  f.p = __byte_perm(x0, x1, 0x7632);
+  f.a = __byte_perm(y0, y1, 0x7632);
+  // bytes: A0, P0, A1, P1 (byte 1 of each word)
+  f.r = __byte_perm(__byte_perm(y0, x0, 0x0051), __byte_perm(y1, x1, 0x0051), 0x5410);
+  return f;
+}
+__device__ __forceinline__ float factor_lo(uint32_t upper, uint32_t r, int byte) {  // column 0: upper's low half
+  return __uint_as_float((upper << 16) | (((r >> (8 * byte)) & 0xffu) << 8));
+}
+__device__ __forceinline__ float factor_hi(uint32_t upper, uint32_t r, int byte) {  // column 1: upper's high half
+  return __uint_as_float((upper & 0xffff0000u) | (((r >> (8 * byte)) & 0xffu) << 8));
+}
+
 template <int EPI, int PBN>
 struct Config {
   static constexpr int kBHalf = PBN / 2;
   static constexpr int kStage = kABytes + kBHalf * BK * 2;
-  // per epilogue warp: kStore two 32 x 64 boxes, kGate three 32 x 32 boxes, kGateBwd two pairs of 32 x 32 boxes
-  static constexpr int kEpiBytes = EPI == kGate ? 3 * 2048 : 2 * 4096;
-  static constexpr int kStages = PBN == 256 ? 5 : (EPI == kGate ? 7 : 6);
+  // per epilogue warp: kStore two 32 x 64 boxes, kGate four 32 x 32 boxes, kGateBwd two triples of 32 x 32 boxes
+  static constexpr int kEpiBytes = EPI == kGateBwd ? 2 * 6144 : 2 * 4096;
+  static constexpr int kStages = PBN == 256 ? (EPI == kGateBwd ? 4 : 5) : (EPI == kGateBwd ? 5 : 6);
   static constexpr size_t kSmem = size_t(kStages) * kStage + kEpiWarps * kEpiBytes + 1024 + 512;
 };
 
@@ -349,16 +375,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
     uint8_t* buf = epi_stage + (warp - 2) * C::kEpiBytes;
     int sel = 0;
-    uint64_t* factor_bar = factor_bars + (warp - 2) * 2;  // one per box pair
+    uint64_t* factor_bar = factor_bars + (warp - 2) * 2;  // one per box triple
     int factor_phase = 0;
-    // loads a 32 x 32 box of P and one of A into box pair `which`, once the last store from it has read it
+    // loads a 32 x 32 box of each of P, A and R into box triple `which`, once the last store from it has read it
     auto fetch_factors = [&](int c0, int row, int which) {
       if (lane == 0) {
         bulk_wait_read<0>();
         const uint32_t bar = smem_u32(&factor_bar[which]);
-        mbar_arrive_expect_tx(bar, 4096);
-        tma_load_3d(smem_u32(buf + which * 4096), &maps.a[1], bar, c0, row, 0);
-        tma_load_3d(smem_u32(buf + which * 4096 + 2048), &maps.b[1], bar, c0, row, 0);
+        mbar_arrive_expect_tx(bar, 6144);
+        tma_load_3d(smem_u32(buf + which * 6144), &maps.a[1], bar, c0, row, 0);
+        tma_load_3d(smem_u32(buf + which * 6144 + 2048), &maps.b[1], bar, c0, row, 0);
+        tma_load_3d(smem_u32(buf + which * 6144 + 4096), &maps.o[0], bar, c0, row, 0);
       }
       __syncwarp();
     };
@@ -473,7 +500,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
             uint32_t h[16];
             if (p.train) {
-              uint32_t fp[16], fa[16];
+              uint32_t fp[16], fa[16], fr[16];
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
                 const float u0 = __uint_as_float(u[2 * c]), u1 = __uint_as_float(u[2 * c + 1]);
@@ -481,11 +508,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 act_both<ACT>(__uint_as_float(g[2 * c]), a0, s0);
                 act_both<ACT>(__uint_as_float(g[2 * c + 1]), a1, s1);
                 h[c] = cvt2(a0 * u0, a1 * u1);
-                fp[c] = cvt2(s0 * u0, s1 * u1);
-                fa[c] = cvt2(a0, a1);
+                const Factors2 f = pack_factors(s0 * u0, s1 * u1, a0, a1);
+                fp[c] = f.p;
+                fa[c] = f.a;
+                fr[c] = f.r;
               }
               fill(buf + 2048, fp);
               fill(buf + 4096, fa);
+              fill(buf + 6144, fr);
             } else {
 #pragma unroll
               for (int c = 0; c < 16; ++c)
@@ -500,6 +530,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               if (p.train) {
                 tma_store_3d(&maps.o[1], smem_u32(buf + 2048), c0, row0, 0);
                 tma_store_3d(&maps.o[2], smem_u32(buf + 4096), c0, row0, 0);
+                tma_store_3d(&maps.o[3], smem_u32(buf + 6144), c0, row0, 0);
               }
               bulk_commit();
             }
@@ -509,22 +540,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int j = 0; j < chunks; ++j) {
             const int c0 = f0 + j * 32;
-            // the other box pair takes the next chunk's factors
+            // the other boxes take the next chunk's factors
             if (j + 1 < chunks) fetch_factors(c0 + 32, row0, sel ^ 1);
             ok = mbar_wait(smem_u32(&factor_bar[sel]), uint32_t(factor_phase >> sel) & 1u, p.status, abort_flag);
             factor_phase ^= 1 << sel;
             uint32_t d[32];
             tmem_ld32(thalf + j * 32, d);
             tc_wait_ld();
-            uint8_t* box = buf + sel * 4096;
-            uint32_t pv[16], av[16];
+            uint8_t* box = buf + sel * 6144;
+            uint32_t pv[16], av[16], rv[16];
             read(box, pv);
             read(box + 2048, av);
+            read(box + 4096, rv);
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               const float d0 = __uint_as_float(d[2 * c]), d1 = __uint_as_float(d[2 * c + 1]);
-              pv[c] = cvt2(d0 * __uint_as_float(pv[c] << 16), d1 * __uint_as_float(pv[c] & 0xffff0000u));
-              av[c] = cvt2(d0 * __uint_as_float(av[c] << 16), d1 * __uint_as_float(av[c] & 0xffff0000u));
+              pv[c] = cvt2(d0 * factor_lo(pv[c], rv[c], 1), d1 * factor_hi(pv[c], rv[c], 3));
+              av[c] = cvt2(d0 * factor_lo(av[c], rv[c], 0), d1 * factor_hi(av[c], rv[c], 2));
             }
             // a lane writes its results over the factors that it read
             fill(box, pv);
@@ -573,8 +605,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 struct ReduceArgs {
   Problem q;
   int train;
-  uint16_t *h, *o1, *o2;           // kGate: h, P, A; kGateBwd: -, dg, du
-  const uint16_t *fp, *fa;
+  uint16_t *h, *o1, *o2, *o3;      // kGate: h, P, A, R; kGateBwd: -, dg, du, -
+  const uint16_t *fp, *fa, *fr;
   long long ldh, ldo, ldf;
 };
 
@@ -708,21 +740,35 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(const __grid_constant
       }
       put8(a.h + (long long)row * a.ldh + col, h, cols, true);
       if (a.train) {
-        put8(a.o1 + (long long)row * a.ldo + col, v, cols, true);
-        put8(a.o2 + (long long)row * a.ldo + col, g, cols, true);
+        // rows of the factors hold a multiple of 8 columns: whole vectors fit
+        uint32_t fp[4], fa[4], fr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Factors2 f = pack_factors(v[2 * i], v[2 * i + 1], g[2 * i], g[2 * i + 1]);
+          fp[i] = f.p;
+          fa[i] = f.a;
+          fr[i] = f.r;
+        }
+        const long long at = (long long)row * a.ldo + col;
+        *reinterpret_cast<uint4*>(a.o1 + at) = make_uint4(fp[0], fp[1], fp[2], fp[3]);
+        *reinterpret_cast<uint4*>(a.o2 + at) = make_uint4(fa[0], fa[1], fa[2], fa[3]);
+        *reinterpret_cast<uint4*>(a.o3 + at) = make_uint4(fr[0], fr[1], fr[2], fr[3]);
       }
     } else {
       const int half = oc / (PBN / 16), o = oc % (PBN / 16);
       sum8<PBN>(q, tile, rank * 8 + half * 4 + quarter, o / 4, o & 3, lane, v);
-      const uint4 pv = *reinterpret_cast<const uint4*>(a.fp + (long long)row * a.ldf + col);
-      const uint4 av = *reinterpret_cast<const uint4*>(a.fa + (long long)row * a.ldf + col);
-      const uint16_t* pe = reinterpret_cast<const uint16_t*>(&pv);
-      const uint16_t* ae = reinterpret_cast<const uint16_t*>(&av);
+      const long long at = (long long)row * a.ldf + col;
+      const uint4 pv = *reinterpret_cast<const uint4*>(a.fp + at);
+      const uint4 av = *reinterpret_cast<const uint4*>(a.fa + at);
+      const uint4 rv = *reinterpret_cast<const uint4*>(a.fr + at);
+      const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w}, aw[4] = {av.x, av.y, av.z, av.w}, rw[4] = {rv.x, rv.y, rv.z, rv.w};
       float dg[8], du[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dg[i] = v[i] * bf2f(pe[i]);
-        du[i] = v[i] * bf2f(ae[i]);
+      for (int i = 0; i < 4; ++i) {
+        dg[2 * i] = v[2 * i] * factor_lo(pw[i], rw[i], 1);
+        dg[2 * i + 1] = v[2 * i + 1] * factor_hi(pw[i], rw[i], 3);
+        du[2 * i] = v[2 * i] * factor_lo(aw[i], rw[i], 0);
+        du[2 * i + 1] = v[2 * i + 1] * factor_hi(aw[i], rw[i], 2);
       }
       put8(a.o1 + (long long)row * a.ldo + col, dg, cols, true);
       put8(a.o2 + (long long)row * a.ldo + col, du, cols, true);
@@ -834,7 +880,7 @@ struct FewArgs {
   FewMat x;      // [M][K]
   int M, rows, K;
   int early;     // the weights were not written by the kernel before this one
-  uint16_t *out, *o1, *o2;  // kGate: h, P, A (or null); kStore: y
+  uint16_t *out, *o1, *o2, *o3;  // kGate: h, P, A, R (or null); kStore: y
   long long ldo;            // of all of them
 };
 
@@ -1034,8 +1080,10 @@ __global__ void __launch_bounds__(kFewThreads, kFewPerSm) gated_few_kernel(const
         act_both<ACT>(v[0], act, slope);
         a.out[at] = cvt1(act * v[1]);
         if (a.o1) {
-          a.o1[at] = cvt1(slope * v[1]);
-          a.o2[at] = cvt1(act);
+          const Factors2 f = pack_factors(slope * v[1], 0.f, act, 0.f);
+          a.o1[at] = uint16_t(f.p);
+          a.o2[at] = uint16_t(f.a);
+          a.o3[at] = uint16_t(f.r);
         }
       } else {
         a.out[at] = cvt1(v[0]);
@@ -1136,8 +1184,8 @@ b2_status launch_gemm(const Maps& maps, const Params& p, cudaStream_t st) {
 // The gate epilogues' tensors.
 struct Gate {
   int train = 0;
-  Mat h, o1, o2;                 // written: h, P, A (kGate) or dg, du (kGateBwd)
-  const uint16_t *fp = nullptr, *fa = nullptr;
+  Mat h, o1, o2, o3;             // written: h, P, A, R (kGate) or dg, du (kGateBwd)
+  const uint16_t *fp = nullptr, *fa = nullptr, *fr = nullptr;
   int64_t ldf = 0;
 };
 
@@ -1188,11 +1236,13 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
     } else {
       B2_TRY(map2d(&maps.a[1], {gate->fp, pr[0].M, pr[0].N, gate->ldf}, 32, 32, 64));
       B2_TRY(map2d(&maps.b[1], {gate->fa, pr[0].M, pr[0].N, gate->ldf}, 32, 32, 64));
+      B2_TRY(map2d(&maps.o[0], {gate->fr, pr[0].M, pr[0].N, gate->ldf}, 32, 32, 64));
     }
     if (EPI == kGateBwd || gate->train) {
       B2_TRY(map2d(&maps.o[1], gate->o1, 32, 32, 64));
       B2_TRY(map2d(&maps.o[2], gate->o2, 32, 32, 64));
     }
+    if (EPI == kGate && gate->train) B2_TRY(map2d(&maps.o[3], gate->o3, 32, 32, 64));
   }
   B2_TRY((pbn == 256 ? launch_gemm<EPI, 256, A_MN, B_MN, ACT>(maps, p, st)
                      : launch_gemm<EPI, 128, A_MN, B_MN, ACT>(maps, p, st)));
@@ -1205,8 +1255,10 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
       r.h = static_cast<uint16_t*>(const_cast<void*>(gate->h.p));
       r.o1 = static_cast<uint16_t*>(const_cast<void*>(gate->o1.p));
       r.o2 = static_cast<uint16_t*>(const_cast<void*>(gate->o2.p));
+      r.o3 = static_cast<uint16_t*>(const_cast<void*>(gate->o3.p));
       r.fp = gate->fp;
       r.fa = gate->fa;
+      r.fr = gate->fr;
       r.ldh = gate->h.ld;
       r.ldo = gate->o1.ld;
       r.ldf = gate->ldf;
@@ -1269,8 +1321,8 @@ b2_status launch_few(const FewArgs& a, cudaStream_t st) {
 }
 
 // The forward of few tokens: two launches, no padded copies.
-b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd, int act, const Mat& h, uint16_t* fp,
-                      uint16_t* fa, void* y, int64_t ldy, cudaStream_t st) {
+b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd, int act, const Mat& h,
+                      uint16_t* factors, int64_t apart, void* y, int64_t ldy, cudaStream_t st) {
   FewArgs a{};
   a.w[0] = few_mat(wg);
   a.w[1] = few_mat(wu);
@@ -1279,8 +1331,11 @@ b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd,
   a.rows = int(wg.rows);
   a.K = int(x.cols);
   a.out = static_cast<uint16_t*>(const_cast<void*>(h.p));
-  a.o1 = fp;
-  a.o2 = fa;
+  if (factors) {
+    a.o1 = factors;
+    a.o2 = factors + apart;
+    a.o3 = factors + 2 * apart;
+  }
   a.ldo = h.ld;
   B2_TRY((act == kSilu   ? launch_few<kGate, kSilu>(a, st)
           : act == kGelu ? launch_few<kGate, kGelu>(a, st)
@@ -1419,11 +1474,11 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   const FwdPlan plan = fwd_plan({M, D, F, E}, sms);
   Carve ws(workspace);
   const int64_t Fp = up8(F);
-  const Mat h = saved ? Mat{saved, M, F, 3 * Fp} : Mat{ws.take(size_t(M) * Fp * 2), M, F, Fp};
+  const Mat h = saved ? Mat{saved, M, F, 4 * Fp} : Mat{ws.take(size_t(M) * Fp * 2), M, F, Fp};
   Mat mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
   if (M <= kFewTokens) {
     uint16_t* keep = static_cast<uint16_t*>(saved);
-    return few_forward(mx, mg, mu, md, act, h, keep ? keep + Fp : nullptr, keep ? keep + 2 * Fp : nullptr, y, ldy, st);
+    return few_forward(mx, mg, mu, md, act, h, keep ? keep + Fp : nullptr, Fp, y, ldy, st);
   }
   Padder pad;
   pad.add(mx, ws);
@@ -1436,8 +1491,9 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   gate.train = saved != nullptr;
   gate.h = h;
   if (saved) {
-    gate.o1 = {static_cast<uint16_t*>(saved) + Fp, M, F, 3 * Fp};
-    gate.o2 = {static_cast<uint16_t*>(saved) + 2 * Fp, M, F, 3 * Fp};
+    gate.o1 = {static_cast<uint16_t*>(saved) + Fp, M, F, 4 * Fp};
+    gate.o2 = {static_cast<uint16_t*>(saved) + 2 * Fp, M, F, 4 * Fp};
+    gate.o3 = {static_cast<uint16_t*>(saved) + 3 * Fp, M, F, 4 * Fp};
   }
   Product up;
   up.a[0] = mx;
@@ -1495,7 +1551,7 @@ b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int
   const BwdPlan plan = bwd_plan(s, current_sms());
   Carve ws(workspace);
   const int64_t Fp = up8(F);
-  const Mat h{saved, M, F, 3 * Fp};
+  const Mat h{saved, M, F, 4 * Fp};
   uint16_t* dgu = static_cast<uint16_t*>(ws.take(size_t(M) * Fp * 4));
   const Mat dg{dgu, M, F, 2 * Fp}, du{dgu + Fp, M, F, 2 * Fp};
   Mat mdy{dy, M, E, lddy}, mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
@@ -1515,7 +1571,8 @@ b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int
   gate.o2 = du;
   gate.fp = static_cast<const uint16_t*>(saved) + Fp;
   gate.fa = gate.fp + Fp;
-  gate.ldf = 3 * Fp;
+  gate.fr = gate.fa + Fp;
+  gate.ldf = 4 * Fp;
   Product t;
   t.a[0] = mdy;
   t.b[0] = md;

@@ -40,7 +40,7 @@ Call check(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, cons
   return c;
 }
 
-int64_t saved_width(int64_t F) { return 3 * ((F + 7) / 8 * 8); }
+int64_t saved_width(int64_t F) { return 4 * ((F + 7) / 8 * 8); }
 
 // kept: room for what the backward needs; may be undefined
 at::Tensor run_fwd(const Call& c, at::IntArrayRef x_sizes, int64_t act, const at::Tensor& kept) {

@@ -65,7 +65,8 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     ``[..., E]``.  ``activation``: ``"silu"``, ``"gelu"`` (erf form) or
     ``"relu"``.  Sums are fp32; the hidden tensor is rounded to bfloat16
     between the products, and the backward keeps it and the two factors
-    ``act(gate)`` and ``up * act'(gate)`` in bfloat16.  Inside ``torch.autocast("xdna")`` other
+    ``act(gate)`` and ``up * act'(gate)`` (16 bits of significand): eight bytes
+    a hidden element.  Inside ``torch.autocast("xdna")`` other
     floating-point arguments are cast first, as for a matrix product."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"gated_mlp: activation must be one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
