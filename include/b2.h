@@ -662,7 +662,8 @@ b2_status b2_embedding_fwd(const void* ids, int ids_dtype, int64_t T,
  * for padding_idx; -1: none; ids outside [0, V) add to no row).  dy has row
  * stride lddy >= D.  fp32 sums in a fixed order over tokens sorted by id
  * (bit-reproducible), rounded once.  Workspace: at least
- * b2_embedding_bwd_workspace_bytes(T, V, D) bytes, 16-byte aligned. */
+ * b2_embedding_bwd_workspace_bytes(T, V, D) bytes, 16-byte aligned (0 for few
+ * tokens; may then be NULL). */
 size_t b2_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D);
 b2_status b2_embedding_bwd(const void* ids, int ids_dtype, int64_t T,
                            const void* dy, int64_t lddy, int dtype, int64_t V,

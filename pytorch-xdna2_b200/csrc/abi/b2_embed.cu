@@ -344,6 +344,98 @@ __device__ __forceinline__ void store_row(T* row, int c, const float (&acc)[N], 
   reinterpret_cast<typename Pack<T, N>::V*>(row)[c] = p.v;
 }
 
+// Zeros to the rows of `base` (rows x width) that are not present (all threads of
+// the CTA call).  The rows' elements are taken as one range: its whole 16-byte
+// vectors, whatever the row length (a vector over two rows goes element by
+// element).
+template <typename T>
+__device__ __forceinline__ void zero_absent(T* base, int rows, unsigned width, const uint8_t* present) {
+  constexpr int E = 16 / sizeof(T);
+  const unsigned total = unsigned(rows) * width;  // about 64 KB, or one row
+  const unsigned head = min(total, unsigned((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / unsigned(sizeof(T)));
+  const unsigned whole = (total - head) / E;
+  for (unsigned v = threadIdx.x; v < whole; v += kAccThreads) {
+    const unsigned e0 = head + v * E;
+    const unsigned first_row = e0 / width, last_row = (e0 + E - 1) / width;
+    if (first_row == last_row) {
+      if (!present[first_row]) *reinterpret_cast<uint4*>(base + e0) = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (!present[(e0 + i) / width]) base[e0 + i] = T(0);
+    }
+  }
+  const unsigned tail = head + whole * E;
+  if (threadIdx.x < head && !present[threadIdx.x / width]) base[threadIdx.x] = T(0);
+  if (threadIdx.x < total - tail && !present[(tail + threadIdx.x) / width]) base[tail + threadIdx.x] = T(0);
+}
+
+// The whole gradient in one launch for few tokens: CTAs [0, token_blocks) give
+// every token 1 << log_warps warps (a warp for up to 32 vectors of columns); the
+// first token of an id adds the rows of all tokens that have it, in token order,
+// eight loads in flight.  The CTAs behind them zero the absent rows.  A frequent
+// id's rows are added by one group of warps one batch after the other, which is
+// why this ends at kSmallTokens (512 tokens of one id: 45 us).
+constexpr int kSmallTokens = 512;
+template <typename T, int N>
+__global__ void __launch_bounds__(kAccThreads)
+    embed_small_kernel(const void* __restrict__ ids, int is64, int tokens, long long V, long long pad,
+                       const T* __restrict__ dy, long long lddy, int vecs, int log_warps, long long D, float scale,
+                       T* __restrict__ dw, int slabs, long long token_blocks, int zero_rows) {
+  if ((long long)blockIdx.x >= token_blocks) {
+    __shared__ uint8_t present[512];
+    const long long r0 = ((long long)blockIdx.x - token_blocks) * zero_rows;
+    const int rows = int(min((long long)zero_rows, V - r0));
+    for (int i = threadIdx.x; i < rows; i += kAccThreads) present[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens; i += kAccThreads) {
+      const long long k = (long long)key_of(ids, is64, i, V, pad) - r0;
+      if (k >= 0 && k < rows) present[k] = 1;  // (a token without a row has key V, behind every row)
+    }
+    __syncthreads();
+    zero_absent(dw + r0 * D, rows, unsigned(D), present);
+    return;
+  }
+  __shared__ uint32_t keys[kSmallTokens];
+  const int padded = (tokens + 31) / 32 * 32;
+  for (int i = threadIdx.x; i < padded; i += kAccThreads)
+    keys[i] = i < tokens ? key_of(ids, is64, i, V, pad) : 0xffffffffu;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = int(blockIdx.x / slabs) * ((kAccThreads / 32) >> log_warps) + (warp >> log_warps);
+  if (t >= tokens) return;
+  const uint32_t mine = keys[t];
+  if (mine >= V) return;
+  for (int base = 0; base < t; base += 32)
+    if (__any_sync(0xffffffffu, base + lane < t && keys[base + lane] == mine)) return;  // not the id's first token
+  const int c = ((int(blockIdx.x % slabs) << log_warps) + (warp & ((1 << log_warps) - 1))) * 32 + lane;
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  constexpr int U = 8;
+  for (int base = t / 32 * 32; base < padded; base += 32) {
+    unsigned found = __ballot_sync(0xffffffffu, keys[base + lane] == mine);
+    while (found) {
+      Pack<T, N> v[U];
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (found == 0) break;
+        const int j = base + __ffs(found) - 1;
+        found &= found - 1;
+        n = u + 1;
+        if (c < vecs) v[u].v = reinterpret_cast<const typename Pack<T, N>::V*>(dy + (long long)j * lddy)[c];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < n)
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] += v[u].get(i);
+    }
+  }
+  if (c < vecs) store_row<T, N>(dw + (long long)mine * D, c, acc, scale);
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kAccThreads)
     embed_acc_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ tok, long long tokens, long long V,
@@ -364,27 +456,7 @@ __global__ void __launch_bounds__(kAccThreads)
       if (!__syncthreads_or(in)) break;
     }
     __syncthreads();
-    // the rows' elements as one range: its whole 16-byte vectors, whatever the
-    // row length (a vector over two rows goes element by element)
-    constexpr int E = 16 / sizeof(T);
-    T* base = dw + r0 * D;
-    const unsigned total = unsigned(rows * D), width = unsigned(D);  // about 64 KB, or one row
-    const unsigned head = min(total, unsigned((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / unsigned(sizeof(T)));
-    const unsigned whole = (total - head) / E;
-    for (unsigned v = threadIdx.x; v < whole; v += kAccThreads) {
-      const unsigned e0 = head + v * E;
-      const unsigned first_row = e0 / width, last_row = (e0 + E - 1) / width;
-      if (first_row == last_row) {
-        if (!present[first_row]) *reinterpret_cast<uint4*>(base + e0) = make_uint4(0, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (!present[(e0 + i) / width]) base[e0 + i] = T(0);
-      }
-    }
-    const unsigned tail = head + whole * E;
-    if (threadIdx.x < head && !present[threadIdx.x / width]) base[threadIdx.x] = T(0);
-    if (threadIdx.x < total - tail && !present[(tail + threadIdx.x) / width]) base[tail + threadIdx.x] = T(0);
+    zero_absent(dw + r0 * D, rows, unsigned(D), present);
     return;
   }
   const int per_block = kAccThreads >> log_lanes;
@@ -541,6 +613,11 @@ int log_lanes_for(int vecs) {
   return l;
 }
 
+// rows of dW a zeroing CTA looks after: about 64 KB
+int zero_rows_for(int64_t D, size_t size) {
+  return int(std::max<int64_t>(1, std::min<int64_t>(512, 65536 / (D * int64_t(size)))));
+}
+
 struct SortPlan {
   int passes, bits;
   bool one;      // by counting ranks, in one launch
@@ -637,8 +714,7 @@ b2_status run_acc(const uint32_t* key, const uint32_t* tok, int64_t tokens, int6
   const int64_t pieces = (tokens + kPiece - 1) / kPiece;
   const int per_block = kAccThreads >> ll;
   const int64_t acc_blocks = (pieces + per_block - 1) / per_block * slabs;
-  // rows per zeroing CTA: about 64 KB of dW
-  const int zr = int(std::max<int64_t>(1, std::min<int64_t>(512, 65536 / (D * int64_t(sizeof(T))))));
+  const int zr = zero_rows_for(D, sizeof(T));
   const int64_t blocks = acc_blocks + (V + zr - 1) / zr;
   if (blocks > INT32_MAX) return set_error(B2_ERR_UNSUPPORTED, "b2_embedding_bwd: too many rows");
   B2_TRY(launch_chained(embed_acc_kernel<T, N>, dim3(unsigned(blocks)), kAccThreads, 0, st, "embedding gradient launch",
@@ -651,6 +727,24 @@ b2_status run_acc(const uint32_t* key, const uint32_t* tok, int64_t tokens, int6
                           static_cast<const float*>(partial), pieces));
   }
   return B2_OK;
+}
+
+template <typename T, int N>
+b2_status run_small(const void* ids, int is64, int64_t tokens, int64_t V, int64_t pad, const void* dy, int64_t lddy,
+                    int64_t D, float scale, void* dw, cudaStream_t st) {
+  const int vecs = int(D / N);
+  int lw = 0;
+  while (lw < 3 && (32 << lw) < vecs) ++lw;
+  const int slabs = (vecs + (32 << lw) - 1) / (32 << lw);
+  const int per_block = (kAccThreads / 32) >> lw;
+  const int64_t token_blocks = (tokens + per_block - 1) / per_block * slabs;
+  const int zr = zero_rows_for(D, sizeof(T));
+  const int64_t blocks = token_blocks + (V + zr - 1) / zr;
+  if (blocks > INT32_MAX) return set_error(B2_ERR_UNSUPPORTED, "b2_embedding_bwd: too many rows");
+  embed_small_kernel<T, N><<<unsigned(blocks), kAccThreads, 0, st>>>(ids, is64, int(tokens), V, pad,
+                                                                      static_cast<const T*>(dy), lddy, vecs, lw, D,
+                                                                      scale, static_cast<T*>(dw), slabs, token_blocks, zr);
+  return check_cuda(cudaGetLastError(), "embedding gradient launch");
 }
 
 b2_status check_common(const char* who, int ids_dtype, int dtype, int64_t T, int64_t V, int64_t D, int64_t ld) {
@@ -692,7 +786,7 @@ b2_status b2_embedding_fwd(const void* ids, int ids_dtype, int64_t T, const void
 }
 
 size_t b2_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) {
-  if (T <= 0 || V <= 0 || D <= 0 || T >= INT32_MAX || V >= INT32_MAX) return 0;
+  if (T <= kSmallTokens || V <= 0 || D <= 0 || T >= INT32_MAX || V >= INT32_MAX) return 0;
   return embed_ws(T, V, D).total;
 }
 
@@ -706,7 +800,24 @@ b2_status b2_embedding_bwd(const void* ids, int ids_dtype, int64_t T, const void
   if (T == 0)
     return check_cuda(cudaMemsetAsync(dw, 0, size_t(V) * size_t(D) * (dtype == B2_BF16 ? 2 : 4), st),
                       "embedding gradient memset");
-  if (!ids || !dy || !workspace) return set_error(B2_ERR_INVALID, "b2_embedding_bwd: null pointer");
+  if (!ids || !dy) return set_error(B2_ERR_INVALID, "b2_embedding_bwd: null pointer");
+  if (T <= kSmallTokens) {
+    const int wide = ids_dtype == B2_I64;
+    if (dtype == B2_BF16) {
+      switch (vec_elems(2, D, lddy, dy, dw)) {
+        case 8: return run_small<uint16_t, 8>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+        case 4: return run_small<uint16_t, 4>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+        case 2: return run_small<uint16_t, 2>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+        default: return run_small<uint16_t, 1>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+      }
+    }
+    switch (vec_elems(4, D, lddy, dy, dw)) {
+      case 4: return run_small<float, 4>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+      case 2: return run_small<float, 2>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+      default: return run_small<float, 1>(ids, wide, T, V, padding_idx, dy, lddy, D, scale, dw, st);
+    }
+  }
+  if (!workspace) return set_error(B2_ERR_INVALID, "b2_embedding_bwd: null pointer");
   const EmbedWs w = embed_ws(T, V, D);
   if (workspace_bytes < w.total || reinterpret_cast<uintptr_t>(workspace) % 16)
     return set_error(B2_ERR_WORKSPACE, "b2_embedding_bwd: workspace of %zu bytes (16-byte aligned) needed, got %zu",

@@ -55,12 +55,13 @@ at::Tensor backward_impl(const at::Tensor& ids_in, const at::Tensor& dy_in, int6
   const at::Tensor ids = ids_in.contiguous();
   const at::Tensor dy = as_rows(dy_in, T, D);
   const int64_t bytes = int64_t(b2_embedding_bwd_workspace_bytes(T, V, D));
-  at::Tensor ws = empty({std::max<int64_t>(bytes, 16)}, at::kByte, dev.index());
+  at::Tensor ws;  // few tokens need none
+  if (bytes) ws = empty({bytes}, at::kByte, dev.index());
   const cudaStream_t st = stream(dev.index());
   KernelTimer kt("lm.embedding_bwd", double(dw.numel() + dy.numel()) * double(dw.element_size()), st);
   XDNA_B2(b2_embedding_bwd(ids.data_ptr(), index_code(ids.scalar_type()), T, dy.data_ptr(), row_stride(dy),
-                           float_code(dy.scalar_type()), V, D, float(scale), padding_idx, dw.data_ptr(), ws.data_ptr(),
-                           size_t(ws.numel()), st));
+                           float_code(dy.scalar_type()), V, D, float(scale), padding_idx, dw.data_ptr(),
+                           bytes ? ws.data_ptr() : nullptr, size_t(bytes), st));
   count_launch("lm.embedding_bwd");
   return dw;
 }

@@ -57,7 +57,7 @@ def _check(ids, w, scale, pad, dev, dy=None, ids_dtype=torch.int64):
 CASES = [
     # tokens, vocabulary, width
     (1, 1, 1), (1, 5, 8), (2, 3, 7), (31, 40, 16), (33, 40, 33), (64, 7, 9), (257, 1000, 130), (1024, 513, 64),
-    (1025, 511, 72), (2500, 262145, 12), (4097, 3000, 40), (8192, 20000, 24), (8193, 30000, 24), (20011, 100, 18),
+    (512, 300, 40), (513, 300, 40), (500, 90000, 264), (1025, 511, 72), (4096, 700, 12), (2500, 262145, 12), (4097, 3000, 40), (8192, 20000, 24), (8193, 30000, 24), (20011, 100, 18),
     (300000, 50000, 4), (700, 300, 2056), (70, 5000, 3001),
 ]
 
@@ -160,8 +160,8 @@ def test_refusals(dev):
     dy = torch.ones(3, 8, device=dev, requires_grad=True)
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(lm.embedding(ids, wg), [wg], dy, create_graph=True)
-    need = _abi.lib().b2_embedding_bwd_workspace_bytes(3, 5, 8)
-    st = _abi.lib().b2_embedding_bwd(ids.data_ptr(), _abi.B2_I64, 3, w.data_ptr(), 8, _abi.B2_F32, 5, 8, 1.0, -1,
+    need = _abi.lib().b2_embedding_bwd_workspace_bytes(3000, 5, 8)
+    st = _abi.lib().b2_embedding_bwd(ids.data_ptr(), _abi.B2_I64, 3000, w.data_ptr(), 8, _abi.B2_F32, 5, 8, 1.0, -1,
                                      w.data_ptr(), w.data_ptr(), need - 1, None)
     assert st == 5 and b"workspace" in _abi.lib().b2_last_error()
 
