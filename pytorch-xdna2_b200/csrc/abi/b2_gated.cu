@@ -855,19 +855,27 @@ __global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------
 // Few tokens (M <= kFewTokens): reading the weights once is everything, and a
 // 256-row tile per token would idle most of the machine.  A CTA takes 16 weight
-// rows (kGate: of Wg and of Wu), its 4 warps interleave the reduction in steps
-// of 32, and a cluster of up to 8 CTAs shares a reduction where there are few
-// rows.  The products run on mma.sync m16n8k16 with the weights as the 16-row
-// operand and the tokens as the columns: a lane's 16-byte load of a weight row
-// holds 8 consecutive k, which two instructions take in an order of their own
-// (the same for both operands, so the sum is the same); weights go from memory
-// straight to registers, a batch of U steps ahead of the products.  Partial
-// sums are added in warp and CTA order.
+// rows (kGate: of Wg and of Wu), its 8 warps interleave the reduction in steps
+// of 32, and a cluster of up to 8 CTAs shares a reduction of Wd.  The products
+// run on mma.sync m16n8k16 with the weights as the 16-row operand and the tokens
+// as the columns: a lane's 16 bytes of a weight row hold 8 consecutive k, which
+// two instructions take in an order of their own (the same for both operands, so
+// the sum is the same).  What bounds it is how much is on its way from memory:
+// every lane copies its own 16 bytes ahead into a ring of 3 to 6 steps in shared
+// memory (asynchronously, and read back by the same lane, so nothing has to be
+// synchronized).  Partial sums are added in warp and CTA order.
+//
+// One token, D 1024, F 4096 (25 MB of weights): 9.7 us; 4096 x 12288 (302 MB):
+// 57 us, 5.3 TB/s.  Loads straight to registers took 13 and 68 us; one
+// cooperative kernel over both products with TMA boxes 18 and 67 us.
 // ---------------------------------------------------------------------------
-constexpr int kFewThreads = 128;
+constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kFewPerSm = 4;   // resident CTAs a SM
-constexpr int kFewTokens = 32;
+constexpr int kFewStages = 6;
+// 16 tokens take 12 us (1024 x 4096), 27 us (2048 x 5464) and 73 us (4096 x 12288)
+// here, 22, 30 and 78 us on the tensor-memory path; a third column block for 24
+// would add a fifth to each, and the other path does not grow with the tokens.
+constexpr int kFewTokens = 16;
 
 struct FewMat {
   const uint16_t* p;
@@ -884,63 +892,54 @@ struct FewArgs {
   long long ldo;            // of all of them
 };
 
-// 8 consecutive elements of a weight row from k, zeros from K on: in one
-// aligned word, or (ALIGNED false) in the two aligned words around them, to be
-// shifted together when they are used -- a shift at the load would wait for it.
-template <bool ALIGNED>
-struct RowWord;
-template <>
-struct RowWord<true> {
-  uint4 lo;
-  __device__ __forceinline__ void clear() { lo = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const FewMat&, const uint16_t* row, int k, int K) {
-    if (k + 8 <= K) {
-      lo = __ldg(reinterpret_cast<const uint4*>(row + k));
-    } else {
-      clear();
-      uint16_t* e = reinterpret_cast<uint16_t*>(&lo);
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Waits for the oldest of the S - 1 steps under way.
+__device__ __forceinline__ void copy_wait_step(int S) {
+  if (S == 3)
+    copy_wait<1>();
+  else if (S == 4)
+    copy_wait<2>();
+  else if (S == 5)
+    copy_wait<3>();
+  else
+    copy_wait<4>();
+}
+
+// Starts this lane's copy of 8 consecutive elements of a row from k (zeros from K
+// on) to its 16 bytes at `at`; rows at any alignment (WORDS 2): the two aligned
+// words around them, 512 bytes apart, to be shifted when they are used.
+template <int WORDS>
+__device__ __forceinline__ void fetch8(const FewMat& m, const uint16_t* row, int k, int K, uint4* at) {
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(row + k);
+  const uint16_t* first = reinterpret_cast<const uint16_t*>(WORDS == 2 ? addr & ~uintptr_t(15) : addr);
+  const bool whole = k + 8 <= K && (WORDS == 2 ? first >= m.p && first + 16 <= m.end : m.aligned != 0);
+  if (whole) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < K) e[i] = row[k + i];
-    }
-  }
-  __device__ __forceinline__ uint4 get(int) const { return lo; }
-};
-template <>
-struct RowWord<false> {
-  uint4 lo, hi;
-  __device__ __forceinline__ void clear() { lo = hi = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const FewMat& m, const uint16_t* row, int k, int K) {
-    const uintptr_t addr = reinterpret_cast<uintptr_t>(row + k);
-    const uint4* w = reinterpret_cast<const uint4*>(addr & ~uintptr_t(15));
-    const uint16_t* first = reinterpret_cast<const uint16_t*>(w);
-    if (k + 8 <= K && first >= m.p && first + 16 <= m.end) {
-      lo = __ldg(w);
-      hi = __ldg(w + 1);
-    } else {  // at the ends of the row or the matrix: what is inside, element by element
-      clear();
-      uint16_t *l = reinterpret_cast<uint16_t*>(&lo), *h = reinterpret_cast<uint16_t*>(&hi);
+    for (int w = 0; w < WORDS; ++w) copy16_async(smem_u32(at + w * 32), first + w * 8);
+  } else {
+    // at the ends of the row or the matrix: what is inside, element by element
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      union {
+        uint4 v;
+        uint16_t e[8];
+      } r;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (first + i >= row + k && first + i < row + K) l[i] = first[i];
-        if (first + 8 + i < row + K) h[i] = first[8 + i];
+        const uint16_t* p = first + w * 8 + i;
+        r.e[i] = p >= row + k && p < row + K ? __ldcg(p) : uint16_t(0);
       }
+      at[w * 32] = r.v;
     }
   }
-  __device__ __forceinline__ uint4 get(int shift) const { return shift_words(lo, hi, shift); }
-};
-
-// The tokens' operand is read from L2: until chain_wait the kernel before may
-// be writing it.
-__device__ __forceinline__ uint4 load_tokens(const FewMat& m, const uint16_t* row, int k, int K) {
-  if (m.aligned && k + 8 <= K) return __ldcg(reinterpret_cast<const uint4*>(row + k));
-  union {
-    uint4 v;
-    uint16_t e[8];
-  } r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r.e[i] = k + i < K ? __ldcg(row + k + i) : uint16_t(0);
-  return r.v;
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -951,30 +950,43 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16-byte slots of one step: weights, then tokens; 32 lanes each.
+template <int EPI, int NT, bool ALIGNED>
+struct FewConfig {
+  static constexpr int kMats = EPI == kGate ? 2 : 1;
+  static constexpr int kWords = ALIGNED ? 1 : 2;
+  static constexpr int kSlots = kMats * 2 * kWords + NT;
+  static constexpr size_t kStep = size_t(kFewWarps) * kSlots * 512;  // bytes of a stage
+  static constexpr size_t kStatic = size_t(kFewWarps + 1) * kMats * 16 * 8 * NT * 4;  // red and total
+  static constexpr int kMost = int((227 * 1024 - kStatic) / kStep) < kFewStages ? int((227 * 1024 - kStatic) / kStep) : kFewStages;
+  static_assert(kMost >= 3, "a ring of three steps");
+};
+
 template <int EPI, int NT, int ACT, bool ALIGNED>
-__global__ void __launch_bounds__(kFewThreads, kFewPerSm) gated_few_kernel(const __grid_constant__ FewArgs a,
-                                                                           int cluster) {
-  constexpr int kMats = EPI == kGate ? 2 : 1;
-  // steps whose loads are in flight together
-  constexpr int U = (NT <= 2 ? 4 : 2) / (ALIGNED || EPI == kStore ? 1 : 2);
+__global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_constant__ FewArgs a, int cluster,
+                                                                int S) {
+  using C = FewConfig<EPI, NT, ALIGNED>;
+  constexpr int kMats = C::kMats, kWords = C::kWords;
   constexpr int kOut = 16 * 8 * NT;   // sums per matrix
+  extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ float red[kFewWarps][kMats][kOut];
   __shared__ float total[kMats][kOut];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
   const int rank = cluster > 1 ? int(cluster_ctarank()) : 0;
   const int row0 = (blockIdx.x / cluster) * 16;
+  uint4* ring = reinterpret_cast<uint4*>(smem_raw) + warp * S * C::kSlots * 32 + lane;
   const uint16_t* wrow[kMats][2];
   bool live[2];
   int shift[kMats][2];
-  int k0 = (rank * kFewWarps + warp) * 32 + q * 8;
+  const int k_first = (rank * kFewWarps + warp) * 32 + q * 8;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     live[i] = row0 + g + 8 * i < a.rows;
 #pragma unroll
     for (int m = 0; m < kMats; ++m) {
       wrow[m][i] = a.w[m].p + (long long)(live[i] ? row0 + g + 8 * i : row0) * a.w[m].ld;
-      shift[m][i] = int(reinterpret_cast<uintptr_t>(wrow[m][i] + k0) & 15) * 8;  // the same at every step
+      shift[m][i] = int(reinterpret_cast<uintptr_t>(wrow[m][i] + k_first) & 15) * 8;  // the same at every step
     }
   }
   const uint16_t* xrow[NT];
@@ -992,52 +1004,74 @@ __global__ void __launch_bounds__(kFewThreads, kFewPerSm) gated_few_kernel(const
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[m][n][i] = 0.f;
   const int stride = kFewWarps * cluster * 32;
-  RowWord<ALIGNED> wv[U][kMats][2];
-  uint4 xv[U][NT];
-  auto load_w = [&](int k) {
+  const int steps = (a.K - (k_first - q * 8) + stride - 1) / stride;  // of this warp; may be <= 0
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  // the copies of step t into stage `at`
+  auto fetch_w = [&](int t, int at) {
+    const int k = k_first + t * stride;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int m = 0; m < kMats; ++m)
 #pragma unroll
-      for (int m = 0; m < kMats; ++m)
+      for (int i = 0; i < 2; ++i) {
+        uint4* slot = ring + (at * C::kSlots + (m * 2 + i) * kWords) * 32;
+        if (k < a.K && live[i])
+          fetch8<kWords>(a.w[m], wrow[m][i], k, a.K, slot);
+        else
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int at = k + u * stride;
-          if (at < a.K && live[i])
-            wv[u][m][i].load(a.w[m], wrow[m][i], at, a.K);
-          else
-            wv[u][m][i].clear();
-        }
-  };
-  auto load_x = [&](int k) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int at = k + u * stride;
-        xv[u][n] = make_uint4(0, 0, 0, 0);
-        if (at < a.K && xlive[n]) xv[u][n] = load_tokens(a.x, xrow[n], at, a.K);
+          for (int w = 0; w < kWords; ++w) slot[w * 32] = zero;
       }
+  };
+  auto fetch_x = [&](int t, int at) {
+    const int k = k_first + t * stride;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint4* slot = ring + (at * C::kSlots + kMats * 2 * kWords + n) * 32;
+      if (k < a.K && xlive[n])
+        fetch8<1>(a.x, xrow[n], k, a.K, slot);
+      else
+        *slot = zero;
+    }
   };
   if (!a.early) chain_wait();
   chain_release();
-  load_w(k0);
+  for (int t = 0; t < S - 1; ++t)
+    if (t < steps) fetch_w(t, t);
   if (a.early) chain_wait();  // the tokens' operand comes from the kernel before
-  load_x(k0);
-  for (; k0 - q * 8 < a.K; k0 += U * stride) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int m = 0; m < kMats; ++m) {
-        const uint4 w0 = wv[u][m][0].get(shift[m][0]), w1 = wv[u][m][1].get(shift[m][1]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma16816(c[m][n], w0.x, w1.x, w0.y, w1.y, xv[u][n].x, xv[u][n].y);
-          mma16816(c[m][n], w0.z, w1.z, w0.w, w1.w, xv[u][n].z, xv[u][n].w);
-        }
-      }
-    load_w(k0 + U * stride);
-    load_x(k0 + U * stride);
+  for (int t = 0; t < S - 1; ++t) {
+    if (t < steps) fetch_x(t, t);
+    copy_commit();
   }
+  int at = 0;
+  for (int t = 0; t < steps; ++t) {
+    copy_wait_step(S);
+    const uint4* slot = ring + at * C::kSlots * 32;
+    uint4 xv[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xv[n] = slot[(kMats * 2 * kWords + n) * 32];
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) {
+      uint4 w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4* p = slot + (m * 2 + i) * kWords * 32;
+        w[i] = ALIGNED ? p[0] : shift_words(p[0], p[(kWords - 1) * 32], shift[m][i]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma16816(c[m][n], w[0].x, w[1].x, w[0].y, w[1].y, xv[n].x, xv[n].y);
+        mma16816(c[m][n], w[0].z, w[1].z, w[0].w, w[1].w, xv[n].z, xv[n].w);
+      }
+    }
+    // the stage of the step before is free
+    const int next = at == 0 ? S - 1 : at - 1;
+    if (t + S - 1 < steps) {
+      fetch_w(t + S - 1, next);
+      fetch_x(t + S - 1, next);
+    }
+    copy_commit();
+    if (++at == S) at = 0;
+  }
+  copy_wait<0>();
 #pragma unroll
   for (int m = 0; m < kMats; ++m)
 #pragma unroll
@@ -1285,15 +1319,38 @@ template <int EPI, int NT, int ACT, bool ALIGNED>
 b2_status launch_few_nt(const FewArgs& a, cudaStream_t st) {
   int dev = 0;
   B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  using C = FewConfig<EPI, NT, ALIGNED>;
+  auto kern = gated_few_kernel<EPI, NT, ACT, ALIGNED>;
+  static bool configured[64] = {};
+  if (dev < 0 || dev >= 64) return set_error(B2_ERR_INVALID, "device index %d", dev);
+  if (!configured[dev]) {
+    B2_TRY(check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(C::kStep * C::kMost)),
+                      "cudaFuncSetAttribute(gated few)"));
+    configured[dev] = true;
+  }
   const int groups = (a.rows + 15) / 16;
   const int steps = (a.K + 31) / 32;
-  // a reduction is shared by as many CTAs as stay resident together, while every warp has two steps or more
-  int cluster = 1;
-  while (cluster < 8 && groups * cluster * 2 <= kFewPerSm * sm_count(dev) && steps >= 4 * kFewWarps * cluster)
-    cluster *= 2;
+  // The most steps on their way with every CTA resident; where not even the
+  // smallest choice is resident, that one (more CTAs a SM leave less of the
+  // machine idle in the last wave).  Only Wd's reductions are shared, whose rows
+  // are few and whose copies start while h is still being computed; every warp
+  // keeps three steps.
+  int S = 3, cluster = 1;
+  long long most = 0;
+  for (int c = 1; c <= (EPI == kGate ? 1 : 8) && (c == 1 || steps >= 3 * kFewWarps * c); c *= 2)
+    for (int n = 3; n <= C::kMost; ++n) {
+      const long long resident = 228 * 1024 / (C::kStep * n + C::kStatic + 1024) * sm_count(dev);
+      const long long under_way = (long long)groups * c * (n - 1);
+      if ((long long)groups * c <= resident && under_way > most) {
+        most = under_way;
+        S = n;
+        cluster = c;
+      }
+    }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(groups * cluster));
   cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = C::kStep * S;
   cfg.stream = st;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1304,15 +1361,13 @@ b2_status launch_few_nt(const FewArgs& a, cudaStream_t st) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return check_cuda(cudaLaunchKernelEx(&cfg, gated_few_kernel<EPI, NT, ACT, ALIGNED>, a, cluster),
-                    "gated few-token launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, cluster, S), "gated few-token launch");
 }
 
 template <int EPI, int ACT, bool ALIGNED>
 b2_status launch_few_rows(const FewArgs& a, cudaStream_t st) {
   if (a.M <= 8) return launch_few_nt<EPI, 1, ACT, ALIGNED>(a, st);
-  if (a.M <= 16) return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
-  return launch_few_nt<EPI, 4, ACT, ALIGNED>(a, st);
+  return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
 }
 template <int EPI, int ACT>
 b2_status launch_few(const FewArgs& a, cudaStream_t st) {
