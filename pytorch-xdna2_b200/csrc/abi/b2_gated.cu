@@ -598,7 +598,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // Adds a problem's partial tiles in split order and finishes them with its
 // epilogue.  Gate epilogues: a thread takes 8 columns of one row (kGate: of g and
-// of u).  kStore: a warp takes 32 rows x 32 columns and writes them, staged,
+// of u).  kStore: a warp takes 32 rows x COLS columns and writes them, staged,
 // in whole rows (elements of unaligned rows straight from the threads that own
 // the rows took 26 us for 777 x 1001 where this takes 6).  The lanes of a warp
 // are 32 rows, so its partial reads are contiguous.
@@ -639,34 +639,36 @@ __device__ __forceinline__ void put8(uint16_t* dst, const float (&v)[8], int col
     if (i < cols) dst[i] = cvt1(v[i]);
 }
 
-template <int PBN>
+template <int PBN, int COLS>
 __global__ void __launch_bounds__(256) gated_reduce_store_kernel(const __grid_constant__ ReduceArgs a) {
-  __shared__ __align__(16) uint8_t boxes[8][32 * 64];
+  __shared__ __align__(16) uint8_t boxes[8][32 * COLS * 2];
   chain_wait();
   const Problem& q = a.q;
-  constexpr int kChunks = PBN / 32;
+  constexpr int kUnits = PBN / COLS, kVecs = COLS / 8;
   const int lane = threadIdx.x & 31;
   uint8_t* box = boxes[threadIdx.x >> 5];
-  const long long units = (long long)q.tiles_m * q.tiles_n * 8 * kChunks;  // (tile, 32-row block, 32 columns)
+  const long long units = (long long)q.tiles_m * q.tiles_n * 8 * kUnits;  // (tile, 32-row block, COLS columns)
   for (long long w = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5; w < units; w += (long long)gridDim.x * 8) {
-    const int chunk = int(w % kChunks);
-    const long long rest = w / kChunks;
+    const int unit = int(w % kUnits);
+    const long long rest = w / kUnits;
     const int rows = int(rest % 8);  // rank * 4 + quarter
     const int tile = int(rest / 8);
     const int group = tile / (kGroupM * q.tiles_n), first = group * kGroupM;
     const int gm = min(kGroupM, q.tiles_m - first), in = tile - first * q.tiles_n;
-    const int row0 = (first + in % gm) * 256 + rows * 32, col0 = (in / gm) * PBN + chunk * 32;
+    const int row0 = (first + in % gm) * 256 + rows * 32, col0 = (in / gm) * PBN + unit * COLS;
     if (row0 >= q.M || col0 >= q.N) continue;
+    const int chunk = unit * COLS / 32;
     const int half = chunk / (PBN / 64), j = chunk % (PBN / 64);
     const int region = (rows >> 2) * 8 + half * 4 + (rows & 3);
-    float4 v[8];
+    const int skip = unit * COLS % 32 / 4 * 32;
+    float4 v[2 * kVecs];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+    for (int c = 0; c < 2 * kVecs; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll(COLS == 32 ? 2 : 8)
     for (int s = 0; s < q.splits; ++s) {
-      const float4* src = partial_at<PBN>(q, tile, s, region, j, lane);
+      const float4* src = partial_at<PBN>(q, tile, s, region, j, lane) + skip;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < 2 * kVecs; ++c) {
         const float4 x = __ldcg(src + c * 32);
         v[c].x += x.x;
         v[c].y += x.y;
@@ -674,31 +676,31 @@ __global__ void __launch_bounds__(256) gated_reduce_store_kernel(const __grid_co
         v[c].w += x.w;
       }
     }
+    // 16-byte vector c of row r at c ^ ((r >> 1) & 3) of its 64 bytes
+    const auto slot = [&](int r, int c) { return box + r * (COLS * 2) + ((kVecs == 4 ? c ^ ((r >> 1) & 3) : c) << 4); };
     __syncwarp();
-    // 64-byte rows, 16-byte chunk c of row r at c ^ ((r >> 1) & 3)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+    for (int c = 0; c < kVecs; ++c)
+      *reinterpret_cast<uint4*>(slot(lane, c)) =
           make_uint4(cvt2(v[2 * c].x, v[2 * c].y), cvt2(v[2 * c].z, v[2 * c].w),
                      cvt2(v[2 * c + 1].x, v[2 * c + 1].y), cvt2(v[2 * c + 1].z, v[2 * c + 1].w));
     __syncwarp();
-    const int nrows = min(32, q.M - row0), cols = min(32, q.N - col0);
+    const int nrows = min(32, q.M - row0), cols = min(COLS, q.N - col0);
     uint16_t* out = q.out + (long long)row0 * q.ldo + col0;
-    if (q.tma_out && cols == 32) {
-      // aligned rows: four lanes of 16 bytes a row, eight rows at once
+    if (q.tma_out && cols == COLS) {
+      // aligned rows: a lane a vector
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2), c = lane & 3;
+      for (int i = 0; i < kVecs; ++i) {
+        const int r = i * (32 / kVecs) + lane / kVecs, c = lane % kVecs;
         if (r < nrows)
-          *reinterpret_cast<uint4*>(out + (long long)r * q.ldo + c * 8) =
-              *reinterpret_cast<const uint4*>(box + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+          *reinterpret_cast<uint4*>(out + (long long)r * q.ldo + c * 8) = *reinterpret_cast<const uint4*>(slot(r, c));
       }
     } else {
+      const int c = lane % COLS;
 #pragma unroll 4
-      for (int r = 0; r < nrows; ++r)
-        if (lane < cols)
-          out[(long long)r * q.ldo + lane] = *reinterpret_cast<const uint16_t*>(
-              box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+      for (int r = lane / COLS; r < nrows; r += 32 / COLS)
+        if (c < cols)
+          out[(long long)r * q.ldo + c] = *reinterpret_cast<const uint16_t*>(slot(r, c >> 3) + (c & 7) * 2);
     }
   }
 }
@@ -865,17 +867,15 @@ __global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ 
 // memory (asynchronously, and read back by the same lane, so nothing has to be
 // synchronized).  Partial sums are added in warp and CTA order.
 //
-// One token, D 1024, F 4096 (25 MB of weights): 9.7 us; 4096 x 12288 (302 MB):
+// One token, D 1024, F 4096 (25 MB of weights): 9.6 us; 4096 x 12288 (302 MB):
 // 57 us, 5.3 TB/s.  Loads straight to registers took 13 and 68 us; one
-// cooperative kernel over both products with TMA boxes 18 and 67 us.
+// cooperative kernel over both products with TMA boxes 18 and 67 us; 64 k a
+// step, copied in whole 128-byte lines, 14 and 66 us.
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kFewStages = 6;
-// 16 tokens take 12 us (1024 x 4096), 27 us (2048 x 5464) and 73 us (4096 x 12288)
-// here, 22, 30 and 78 us on the tensor-memory path; a third column block for 24
-// would add a fifth to each, and the other path does not grow with the tokens.
-constexpr int kFewTokens = 16;
+constexpr int kFewTokens = 32;
 
 struct FewMat {
   const uint16_t* p;
@@ -1223,6 +1223,53 @@ struct Gate {
   int64_t ldf = 0;
 };
 
+// Carves a workspace; with a null base it only counts.
+struct Carve {
+  uint8_t* base;
+  size_t at = 0;
+  explicit Carve(void* b) : base(static_cast<uint8_t*>(b)) {}
+  void* take(size_t bytes) {
+    void* r = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  }
+};
+
+// Brings operands into TMA-addressable rows where they are not, in one launch.
+struct Padder {
+  PadArgs a{};
+  void add(Mat& m, Carve& ws) {
+    if (!m.p || m.rows == 0 || m.cols == 0) return;
+    // room is reserved by the shape alone, so that the workspace size does not depend on the pointers
+    if (tma_rows(m.p, m.ld)) return;
+    const int64_t ld = up8(m.cols);
+    void* d = ws.take(size_t(m.rows) * size_t(ld) * 2);
+    const int i = a.n++;
+    a.src[i] = static_cast<const uint16_t*>(m.p);
+    a.dst[i] = static_cast<uint16_t*>(d);
+    a.lds[i] = m.ld;
+    a.rows[i] = int(m.rows);
+    a.cols[i] = int(m.cols);
+    a.ldd[i] = int(ld);
+    a.begin[i + 1] = a.begin[i] + m.rows * (ld / 8);
+    m.p = d;
+    m.ld = ld;
+  }
+  b2_status run(cudaStream_t st) {
+    if (a.n == 0) return B2_OK;
+    for (int i = 0; i < a.n; ++i)
+      if (a.begin[i + 1] - a.begin[i] > UINT32_MAX)
+        return set_error(B2_ERR_UNSUPPORTED, "gated_mlp: an operand of unaligned rows is too large to copy");
+    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 255) / 256, 148 * 16));
+    return launch_chained(gated_pad_kernel, dim3(blocks), 256, 0, st, "gated pad launch", a);
+  }
+};
+
+int current_sms() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
+}
+
 template <int EPI, bool A_MN, bool B_MN, int ACT = kSilu>
 b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial, const Gate* gate, cudaStream_t st) {
   Maps maps;
@@ -1297,15 +1344,22 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
       r.ldo = gate->o1.ld;
       r.ldf = gate->ldf;
     }
-    const long long cols = EPI == kStore ? pbn / 32 : (EPI == kGate ? pbn / 2 : pbn) / 8;  // a warp's unit of columns
+    // kStore: units of 8 columns where those of 32 would be fewer than 8 warps a SM
+    // (19 tokens, 1024 x 4096: a forward of 22 us against 27; 512 tokens, 4096 x 12288:
+    // 131 us against 129 with the wide ones)
+    const long long blocks32 = (long long)(r.q.M + 31) / 32 * r.q.tiles_n * (pbn / 32);
+    const bool narrow = EPI != kStore || blocks32 < 8LL * current_sms();
+    const long long cols = narrow ? (EPI == kGate ? pbn / 2 : pbn) / 8 : pbn / 32;  // a warp's units of a tile's columns
     const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * cols;
     const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
-    if constexpr (EPI == kStore)
-      B2_TRY((pbn == 256 ? launch_chained(gated_reduce_store_kernel<256>, blocks, 256, 0, st, "gated reduce launch", r)
-                         : launch_chained(gated_reduce_store_kernel<128>, blocks, 256, 0, st, "gated reduce launch", r)));
-    else
-      B2_TRY((pbn == 256 ? launch_chained(gated_reduce_kernel<EPI, 256, ACT>, blocks, 256, 0, st, "gated reduce launch", r)
-                         : launch_chained(gated_reduce_kernel<EPI, 128, ACT>, blocks, 256, 0, st, "gated reduce launch", r)));
+    if constexpr (EPI == kStore) {
+      auto kern = pbn == 256 ? (narrow ? gated_reduce_store_kernel<256, 8> : gated_reduce_store_kernel<256, 32>)
+                             : (narrow ? gated_reduce_store_kernel<128, 8> : gated_reduce_store_kernel<128, 32>);
+      B2_TRY(launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r));
+    } else {
+      auto kern = pbn == 256 ? gated_reduce_kernel<EPI, 256, ACT> : gated_reduce_kernel<EPI, 128, ACT>;
+      B2_TRY(launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r));
+    }
   }
   return B2_OK;
 }
@@ -1367,12 +1421,36 @@ b2_status launch_few_nt(const FewArgs& a, cudaStream_t st) {
 template <int EPI, int ACT, bool ALIGNED>
 b2_status launch_few_rows(const FewArgs& a, cudaStream_t st) {
   if (a.M <= 8) return launch_few_nt<EPI, 1, ACT, ALIGNED>(a, st);
-  return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
+  if (a.M <= 16) return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
+  if (a.M <= 24) return launch_few_nt<EPI, 3, ACT, ALIGNED>(a, st);
+  return launch_few_nt<EPI, 4, ACT, ALIGNED>(a, st);
 }
 template <int EPI, int ACT>
 b2_status launch_few(const FewArgs& a, cudaStream_t st) {
-  const bool aligned = a.w[0].aligned && (EPI == kStore || a.w[1].aligned);
-  return aligned ? launch_few_rows<EPI, ACT, true>(a, st) : launch_few_rows<EPI, ACT, false>(a, st);
+  if constexpr (EPI == kGate)  // (takes_few)
+    return launch_few_rows<EPI, ACT, true>(a, st);
+  else
+    return a.w[0].aligned ? launch_few_rows<EPI, ACT, true>(a, st) : launch_few_rows<EPI, ACT, false>(a, st);
+}
+
+// Which forwards take the few-token kernels.  Up to 16 tokens: 16 take 12 us
+// (1024 x 4096), 27 us (2048 x 5464) and 74 us (4096 x 12288) there, 22, 30 and
+// 78 us on the tensor-memory path, which does not grow with the tokens.  Up to
+// 32 where the projections' CTAs are resident at once: 24 tokens 13 against 22 us
+// (1024 x 4096), 32 tokens 8.4 against 14.7 us (512 x 1536); where they are
+// not, 24 tokens take 33 against 31 us (2048 x 5464).  Rows of Wd at any
+// alignment: one token 27 against 45 us with a padded copy (2048 x 5461), 16
+// tokens 34 against 39.  Where x, Wg and Wu have them too, copies pay: 80 against
+// 61 us (2045 x 5461).
+template <int NT>
+bool few_resident(int64_t rows) {
+  using C = FewConfig<kGate, NT, true>;
+  return (rows + 15) / 16 <= int64_t(228 * 1024 / (C::kStep * 3 + C::kStatic + 1024)) * current_sms();
+}
+bool takes_few(const Mat& x, const Mat& wg, const Mat& wu) {
+  if (!tma_rows(x.p, x.ld) || !tma_rows(wg.p, wg.ld) || !tma_rows(wu.p, wu.ld)) return false;
+  return x.rows <= 16 || (x.rows <= 24 && few_resident<3>(wg.rows)) ||
+         (x.rows <= kFewTokens && few_resident<4>(wg.rows));
 }
 
 // The forward of few tokens: two launches, no padded copies.
@@ -1407,56 +1485,9 @@ b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd,
   return launch_few<kStore, kSilu>(d, st);
 }
 
-// Carves a workspace; with a null base it only counts.
-struct Carve {
-  uint8_t* base;
-  size_t at = 0;
-  explicit Carve(void* b) : base(static_cast<uint8_t*>(b)) {}
-  void* take(size_t bytes) {
-    void* r = base ? base + at : nullptr;
-    at += (bytes + 255) / 256 * 256;
-    return r;
-  }
-};
-
 struct Shape {
   int64_t M, D, F, E;
 };
-
-// Brings operands into TMA-addressable rows where they are not, in one launch.
-struct Padder {
-  PadArgs a{};
-  void add(Mat& m, Carve& ws) {
-    if (!m.p || m.rows == 0 || m.cols == 0) return;
-    // room is reserved by the shape alone, so that the workspace size does not depend on the pointers
-    if (tma_rows(m.p, m.ld)) return;
-    const int64_t ld = up8(m.cols);
-    void* d = ws.take(size_t(m.rows) * size_t(ld) * 2);
-    const int i = a.n++;
-    a.src[i] = static_cast<const uint16_t*>(m.p);
-    a.dst[i] = static_cast<uint16_t*>(d);
-    a.lds[i] = m.ld;
-    a.rows[i] = int(m.rows);
-    a.cols[i] = int(m.cols);
-    a.ldd[i] = int(ld);
-    a.begin[i + 1] = a.begin[i] + m.rows * (ld / 8);
-    m.p = d;
-    m.ld = ld;
-  }
-  b2_status run(cudaStream_t st) {
-    if (a.n == 0) return B2_OK;
-    for (int i = 0; i < a.n; ++i)
-      if (a.begin[i + 1] - a.begin[i] > UINT32_MAX)
-        return set_error(B2_ERR_UNSUPPORTED, "gated_mlp: an operand of unaligned rows is too large to copy");
-    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 255) / 256, 148 * 16));
-    return launch_chained(gated_pad_kernel, dim3(blocks), 256, 0, st, "gated pad launch", a);
-  }
-};
-
-int current_sms() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
-}
 
 struct FwdPlan {
   Plan gate, down;
@@ -1531,7 +1562,7 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   const int64_t Fp = up8(F);
   const Mat h = saved ? Mat{saved, M, F, 4 * Fp} : Mat{ws.take(size_t(M) * Fp * 2), M, F, Fp};
   Mat mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
-  if (M <= kFewTokens) {
+  if (takes_few(mx, mg, mu)) {
     uint16_t* keep = static_cast<uint16_t*>(saved);
     return few_forward(mx, mg, mu, md, act, h, keep ? keep + Fp : nullptr, Fp, y, ldy, st);
   }
