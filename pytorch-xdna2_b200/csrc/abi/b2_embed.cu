@@ -373,12 +373,19 @@ __device__ __forceinline__ void zero_absent(T* base, int rows, unsigned width, c
 // The whole gradient in one launch for few tokens: CTAs [0, token_blocks) give
 // every token 1 << log_warps warps (a warp for up to 32 vectors of columns); the
 // first token of an id adds the rows of all tokens that have it, in token order,
-// eight loads in flight.  The CTAs behind them zero the absent rows.  A frequent
-// id's rows are added by one group of warps one batch after the other, which is
-// why this ends at kSmallTokens (512 tokens of one id: 45 us).
+// eight loads in flight.  The CTAs behind them zero the absent rows.  512 tokens,
+// 20000 x 256 bf16: 5.2 us, 12 with the sort below, and two launches less on the
+// host.  A frequent id's rows are added by one group of warps one batch after
+// the other, which is why this ends at kSmallTokens: 512 tokens of one id take
+// 26 us here, 14 there.
 constexpr int kSmallTokens = 512;
+template <int U>
+struct Batch {
+  static constexpr int value = U;
+};
+
 template <typename T, int N>
-__global__ void __launch_bounds__(kAccThreads)
+__global__ void __launch_bounds__(kAccThreads, 4)
     embed_small_kernel(const void* __restrict__ ids, int is64, int tokens, long long V, long long pad,
                        const T* __restrict__ dy, long long lddy, int vecs, int log_warps, long long D, float scale,
                        T* __restrict__ dw, int slabs, long long token_blocks, int zero_rows) {
@@ -408,31 +415,37 @@ __global__ void __launch_bounds__(kAccThreads)
   if (mine >= V) return;
   for (int base = 0; base < t; base += 32)
     if (__any_sync(0xffffffffu, base + lane < t && keys[base + lane] == mine)) return;  // not the id's first token
+  // the id's tokens, in order
+  __shared__ uint16_t lists[kAccThreads / 32][kSmallTokens];
+  uint16_t* list = lists[warp];
+  int count = 0;
+  for (int base = t / 32 * 32; base < padded; base += 32) {
+    const unsigned found = __ballot_sync(0xffffffffu, keys[base + lane] == mine);
+    if (found >> lane & 1) list[count + __popc(found & ((1u << lane) - 1))] = uint16_t(base + lane);
+    count += __popc(found);
+  }
+  __syncwarp();
   const int c = ((int(blockIdx.x % slabs) << log_warps) + (warp & ((1 << log_warps) - 1))) * 32 + lane;
+  const int at = min(c, vecs - 1);
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  constexpr int U = 8;
-  for (int base = t / 32 * 32; base < padded; base += 32) {
-    unsigned found = __ballot_sync(0xffffffffu, keys[base + lane] == mine);
-    while (found) {
-      Pack<T, N> v[U];
-      int n = 0;
+  auto add = [&](int first, auto batch) {
+    constexpr int U = decltype(batch)::value;
+    Pack<T, N> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (found == 0) break;
-        const int j = base + __ffs(found) - 1;
-        found &= found - 1;
-        n = u + 1;
-        if (c < vecs) v[u].v = reinterpret_cast<const typename Pack<T, N>::V*>(dy + (long long)j * lddy)[c];
-      }
+    for (int u = 0; u < U; ++u)
+      v[u].v = reinterpret_cast<const typename Pack<T, N>::V*>(dy + (long long)list[first + u] * lddy)[at];
+    __syncwarp();  // keeps the batch's loads together: the compiler otherwise takes them one by one to save registers
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < n)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int i = 0; i < N; ++i) acc[i] += v[u].get(i);
-    }
-  }
+      for (int i = 0; i < N; ++i) acc[i] += v[u].get(i);
+  };
+  int n = 0;
+  for (; n + 8 <= count; n += 8) add(n, Batch<8>{});
+  for (; n + 4 <= count; n += 4) add(n, Batch<4>{});
+  for (; n < count; ++n) add(n, Batch<1>{});
   if (c < vecs) store_row<T, N>(dw + (long long)mine * D, c, acc, scale);
 }
 
