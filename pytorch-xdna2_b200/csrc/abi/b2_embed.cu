@@ -71,6 +71,9 @@ __device__ __forceinline__ long long load_id(const void* ids, int is64, long lon
 // forward: `lanes` threads (a power of two) walk one row, 256 / lanes rows per
 // CTA, U rows' loads in flight per thread.  An id outside [0, V) gives a row of
 // NaN and B2_ERR_INVALID in the device status word; nothing out of range is read.
+// Bound by HBM: 65536 tokens of 131072 x 2048 bf16 rows 76 us (one row in flight a
+// thread 87, eight 76), 0.54 GB with repeated rows; few tokens by latency, so
+// their columns are spread over CTAs.
 // ---------------------------------------------------------------------------
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(256) embed_fwd_kernel(const void* __restrict__ ids, int is64, long long tokens,
@@ -229,7 +232,8 @@ __global__ void __launch_bounds__(kRankThreads)
 
 // Many CTAs, one launch per digit.  table[p][b][d]: tokens of chunk b with
 // digit d at the start of pass p.  This kernel fills pass 0's table and zeroes
-// the later ones; each pass adds up the next one's while it scatters.
+// the later ones; each pass adds up the next one's while it scatters.  65536
+// tokens, 131072 ids: 3 us here and 8 a pass, two of them.
 __global__ void __launch_bounds__(kSortThreads)
     embed_hist_kernel(const void* __restrict__ ids, int is64, long long tokens, long long V, long long pad, int passes,
                       int bits, int chunk, uint32_t* __restrict__ table) {
@@ -449,6 +453,11 @@ __global__ void __launch_bounds__(kAccThreads, 4)
   if (c < vecs) store_row<T, N>(dw + (long long)mine * D, c, acc, scale);
 }
 
+// Sums of the sorted tokens' rows, a piece of kPiece tokens and up to 256 vectors
+// of columns per group of threads, four rows in flight a thread; the CTAs behind
+// the pieces' zero the absent rows meanwhile.  Bound by HBM: 65536 tokens of
+// 131072 x 2048 bf16 133 us for the 0.8 GB read and written, 6.1 TB/s; 3000 x 997
+// of 50257 fp32 37 us, 5.7 TB/s.
 template <typename T, int N>
 __global__ void __launch_bounds__(kAccThreads)
     embed_acc_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ tok, long long tokens, long long V,
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(kAccThreads)
 // there and goes on (32 pieces a look) and adds a short one's rows by itself, in
 // piece order; a run over more than kShortRun pieces (a frequent token's has
 // hundreds) is shared by the CTA's warps, every eighth piece each, and their
-// sums are added in warp order.
+// sums are added in warp order.  65536 tokens of a Zipf-like draw: 17 us.
 constexpr int kJoinWarps = kAccThreads / 32;
 constexpr int kShortRun = 16;
 template <typename T, int N>
