@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(kAccThreads, 4)
 // Sums of the sorted tokens' rows, a piece of kPiece tokens and up to 256 vectors
 // of columns per group of threads, four rows in flight a thread; the CTAs behind
 // the pieces' zero the absent rows meanwhile.  Bound by HBM: 65536 tokens of
-// 131072 x 2048 bf16 133 us for the 0.8 GB read and written, 6.1 TB/s; 3000 x 997
-// of 50257 fp32 37 us, 5.7 TB/s.
+// 131072 x 2048 bf16 133 us for the 0.8 GB read and written, 6.1 TB/s; 3001 of
+// 50001 x 1001 fp32 37 us, 5.7 TB/s.
 template <typename T, int N>
 __global__ void __launch_bounds__(kAccThreads)
     embed_acc_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ tok, long long tokens, long long V,
