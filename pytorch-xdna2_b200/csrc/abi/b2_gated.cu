@@ -136,9 +136,12 @@ template <int EPI, int PBN>
 struct Config {
   static constexpr int kBHalf = PBN / 2;
   static constexpr int kStage = kABytes + kBHalf * BK * 2;
-  // per epilogue warp: kStore two 32 x 64 boxes, kGate four 32 x 32 boxes, kGateBwd two triples of 32 x 32 boxes
-  static constexpr int kEpiBytes = EPI == kGateBwd ? 2 * 6144 : 2 * 4096;
-  static constexpr int kStages = PBN == 256 ? (EPI == kGateBwd ? 4 : 5) : (EPI == kGateBwd ? 5 : 6);
+  // per epilogue warp: kStore two 32 x 64 boxes, kGate four 32 x 32 boxes, kGateBwd triples of 32 x 32 boxes.
+  // Of these one beside a fifth stage at PBN 256 (dh of 8192 tokens, 4096 x 12288: 700 us, 750 with two triples and
+  // four stages, 886 with three), two at 128 (512 tokens, 1024 x 4096: 13.3 us, 13.8 with one).
+  static constexpr int kTriples = PBN == 256 ? 1 : 2;
+  static constexpr int kEpiBytes = EPI == kGateBwd ? kTriples * 6144 : 2 * 4096;
+  static constexpr int kStages = PBN == 256 ? 5 : (EPI == kGateBwd ? 5 : 6);
   static constexpr size_t kSmem = size_t(kStages) * kStage + kEpiWarps * kEpiBytes + 1024 + 512;
 };
 
@@ -546,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int j = 0; j < chunks; ++j) {
             const int c0 = f0 + j * 32;
             // the other boxes take the next chunk's factors
-            if (j + 1 < chunks) fetch_factors(c0 + 32, row0, sel ^ 1);
+            if (C::kTriples == 2 && j + 1 < chunks) fetch_factors(c0 + 32, row0, sel ^ 1);
             ok = mbar_wait(smem_u32(&factor_bar[sel]), uint32_t(factor_phase >> sel) & 1u, p.status, abort_flag);
             factor_phase ^= 1 << sel;
             uint32_t d[32];
@@ -573,7 +576,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               tma_store_3d(&maps.o[2], smem_u32(box + 2048), c0, row0, 0);
               bulk_commit();
             }
-            sel ^= 1;
+            if (C::kTriples == 2)
+              sel ^= 1;
+            else if (j + 1 < chunks)
+              fetch_factors(c0 + 32, row0, 0);
           }
         }
       }
