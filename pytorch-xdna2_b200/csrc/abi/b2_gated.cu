@@ -619,6 +619,7 @@ struct ReduceArgs {
   uint16_t *h, *o1, *o2, *o3;      // kGate: h, P, A, R; kGateBwd: -, dg, du, -
   const uint16_t *fp, *fa, *fr;
   long long ldh, ldo, ldf;
+  int beside;
 };
 
 template <int PBN>
@@ -653,7 +654,9 @@ __device__ __forceinline__ void put8(uint16_t* dst, const float (&v)[8], int col
 template <int PBN, int COLS>
 __global__ void __launch_bounds__(256) gated_reduce_store_kernel(const __grid_constant__ ReduceArgs a) {
   __shared__ __align__(16) uint8_t boxes[8][32 * COLS * 2];
-  chain_wait();
+  // beside: what is added was complete before the kernel before this one began
+  // (its chain_release stands after its chain_wait)
+  if (!a.beside) chain_wait();
   const Problem& q = a.q;
   constexpr int kUnits = PBN / COLS, kVecs = COLS / 8;
   const int lane = threadIdx.x & 31;
@@ -714,6 +717,7 @@ __global__ void __launch_bounds__(256) gated_reduce_store_kernel(const __grid_co
           out[(long long)r * q.ldo + c] = *reinterpret_cast<const uint16_t*>(slot(r, c >> 3) + (c & 7) * 2);
     }
   }
+  if (a.beside) chain_wait();  // what waits for this kernel waits for the one before it too
 }
 
 template <int EPI, int PBN, int ACT>
@@ -1284,8 +1288,40 @@ int current_sms() {
   return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
 }
 
+b2_status launch_reduce_store(const ReduceArgs& r, int pbn, cudaStream_t st) {
+  // Units of 8 columns where those of 32 would be fewer than 8 warps a SM (19
+  // tokens, 1024 x 4096: a forward of 22 us against 27; 512 tokens, 4096 x 12288:
+  // 131 us against 129 with the wide ones).
+  const long long wide = (long long)(r.q.M + 31) / 32 * r.q.tiles_n * (pbn / 32);
+  const bool narrow = wide < 8LL * current_sms();
+  const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * (pbn / (narrow ? 8 : 32));
+  const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
+  auto kern = pbn == 256 ? (narrow ? gated_reduce_store_kernel<256, 8> : gated_reduce_store_kernel<256, 32>)
+                         : (narrow ? gated_reduce_store_kernel<128, 8> : gated_reduce_store_kernel<128, 32>);
+  return launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r);
+}
+
+// Reductions of one product's partial tiles, put off until after the next
+// product's launch, beside which they run.
+struct Pending {
+  ReduceArgs r[kMaxProblems];
+  int pbn = 0, n = 0;
+  void add(const ReduceArgs& a, int width) {
+    r[n] = a;
+    r[n].beside = 1;
+    pbn = width;
+    ++n;
+  }
+  b2_status run(cudaStream_t st) {
+    for (int i = 0; i < n; ++i) B2_TRY(launch_reduce_store(r[i], pbn, st));
+    n = 0;
+    return B2_OK;
+  }
+};
+
 template <int EPI, bool A_MN, bool B_MN, int ACT = kSilu>
-b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial, const Gate* gate, cudaStream_t st) {
+b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial, const Gate* gate, cudaStream_t st,
+                       Pending* pending = nullptr, Pending* before = nullptr) {
   Maps maps;
   Params p{};
   p.problems = n;
@@ -1341,6 +1377,7 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
   }
   B2_TRY((pbn == 256 ? launch_gemm<EPI, 256, A_MN, B_MN, ACT>(maps, p, st)
                      : launch_gemm<EPI, 128, A_MN, B_MN, ACT>(maps, p, st)));
+  if (before) B2_TRY(before->run(st));
   for (int i = 0; i < n; ++i) {
     if (p.p[i].splits <= 1) continue;
     ReduceArgs r{};
@@ -1358,19 +1395,14 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
       r.ldo = gate->o1.ld;
       r.ldf = gate->ldf;
     }
-    // kStore: units of 8 columns where those of 32 would be fewer than 8 warps a SM
-    // (19 tokens, 1024 x 4096: a forward of 22 us against 27; 512 tokens, 4096 x 12288:
-    // 131 us against 129 with the wide ones)
-    const long long blocks32 = (long long)(r.q.M + 31) / 32 * r.q.tiles_n * (pbn / 32);
-    const bool narrow = EPI != kStore || blocks32 < 8LL * current_sms();
-    const long long cols = narrow ? (EPI == kGate ? pbn / 2 : pbn) / 8 : pbn / 32;  // a warp's units of a tile's columns
-    const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * cols;
-    const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
     if constexpr (EPI == kStore) {
-      auto kern = pbn == 256 ? (narrow ? gated_reduce_store_kernel<256, 8> : gated_reduce_store_kernel<256, 32>)
-                             : (narrow ? gated_reduce_store_kernel<128, 8> : gated_reduce_store_kernel<128, 32>);
-      B2_TRY(launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r));
+      if (pending)
+        pending->add(r, pbn);
+      else
+        B2_TRY(launch_reduce_store(r, pbn, st));
     } else {
+      const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * ((EPI == kGate ? pbn / 2 : pbn) / 8);
+      const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
       auto kern = pbn == 256 ? gated_reduce_kernel<EPI, 256, ACT> : gated_reduce_kernel<EPI, 128, ACT>;
       B2_TRY(launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r));
     }
@@ -1622,7 +1654,7 @@ size_t b2_gated_mlp_bwd_workspace_bytes(int64_t M, int64_t D, int64_t F, int64_t
   const BwdPlan p = bwd_plan(s, current_sms());
   return 2 * padded_bytes(M, F) + padded_bytes(M, D) + padded_bytes(M, E) + 2 * padded_bytes(F, D) +
          padded_bytes(E, F) +
-         std::max({p.dh.partial_bytes, p.dx.partial_bytes, dw_partial_bytes(s, p.dw)}) + 256;
+         std::max(p.dh.partial_bytes, p.dx.partial_bytes) + dw_partial_bytes(s, p.dw) + 512;
 }
 
 b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_gate,
@@ -1665,7 +1697,8 @@ b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int
   pad.add(md, ws);
   B2_TRY(pad.run(st));
   void* partial =
-      ws.take(std::max({plan.dh.partial_bytes, plan.dx.partial_bytes, dw_partial_bytes(s, plan.dw)}));
+      ws.take(std::max(plan.dh.partial_bytes, plan.dx.partial_bytes));
+  void* dw_partial = ws.take(dw_partial_bytes(s, plan.dw));  // dx's are added later
   Gate gate;
   gate.o1 = dg;
   gate.o2 = du;
@@ -1680,6 +1713,8 @@ b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int
   t.N = F;
   t.K = E;
   B2_TRY((run_products<kGateBwd, false, true>(&t, 1, plan.dh, partial, &gate, st)));
+  Pending dx_sums;  // added while the weights' gradients are computed
+  const bool weights = dw_gate || dw_up || dw_down;
   if (dx) {
     Product d;
     d.a[0] = dg;
@@ -1692,7 +1727,7 @@ b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int
     d.K = F;
     d.out = dx;
     d.ldo = D;
-    B2_TRY((run_products<kStore, false, true>(&d, 1, plan.dx, partial, nullptr, st)));
+    B2_TRY((run_products<kStore, false, true>(&d, 1, plan.dx, partial, nullptr, st, weights ? &dx_sums : nullptr)));
   }
   Product w[3];
   int n = 0;
@@ -1711,7 +1746,7 @@ b2_status b2_gated_mlp_bwd_bf16(const void* dy, int64_t lddy, const void* x, int
   weight(dw_up, du, mx);
   weight(dw_down, mdy, h);
   if (n == 0) return B2_OK;
-  return run_products<kStore, true, true>(w, n, plan.dw, partial, nullptr, st);
+  return run_products<kStore, true, true>(w, n, plan.dw, dw_partial, nullptr, st, nullptr, &dx_sums);
 }
 
 }  // extern "C"
