@@ -208,7 +208,7 @@ __device__ __forceinline__ void store_box_rows(const uint8_t* box, uint16_t* dst
 // 8192 tokens, 4096 x 12288: gate 1203 us, down 580, dh 779, dx 1141, the three
 // weight gradients 1899 -- 1.32 PFLOP/s over all five under the power cap (the
 // clock falls with it), 1.45 in runs of a few milliseconds.  512 tokens, 1024 x
-// 4096, forward and backward 83 us: there each product's launch, first tiles and
+// 4096, forward and backward 78 us: there each product's launch, first tiles and
 // epilogue (2.5, 2 and 4 us) outweigh its 3 us of tensor work.
 template <int EPI, int PBN, bool A_MN, bool B_MN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -808,66 +808,71 @@ __device__ __forceinline__ uint4 shift_words(const uint4& lo, const uint4& hi, i
 }
 
 // Copies of matrices whose rows no TMA map can address (a row stride that is
-// not a multiple of 16 bytes, or a misaligned base) into rows that one can, a
-// thread four 16-byte groups at a time: 2048 x 5461 in 9 us, 22 MB in and out.
+// not a multiple of 16 bytes, or a misaligned base) into rows that one can.  A
+// warp takes a piece of a row (or several short rows, 1 << log_lanes lanes each)
+// in aligned 16-byte words, kPadBatch on their way a lane; a lane's result is its
+// word and the next one, which its neighbour has, shifted together.  What the
+// last word of a row brings of the next row lands in the copy's padding, which no
+// map covers.  2048 x 5461, 22 MB in and out: 9.3 us; a thread 16 bytes of the
+// copy at a time, with both words of its own, took 11.5, whole rows a warp 12.2.
 // (Beside the first product instead of before it: 127 -> 132 us for a training
 // pass of 777 tokens, 1001 x 2730.)
+constexpr int kPadBatch = 4;
 struct PadArgs {
   const uint16_t* src[5];
   uint16_t* dst[5];
   long long lds[5];
-  int rows[5], cols[5], ldd[5];
-  long long begin[6];  // prefix sums of 8-column groups
+  int rows[5], cols[5], ldd[5], log_lanes[5];
+  long long begin[6];  // prefix sums of warps' units
   int n;
 };
 __global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ PadArgs a) {
   chain_wait();
-  constexpr int U = 4;  // 16-byte groups a thread has in flight
-  const long long total = a.begin[a.n], step = (long long)gridDim.x * 256;
-  for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += U * step) {
-    const uint16_t* src[U];
-    uint4* dst[U];
-    int left[U];  // columns from the group's first
-    bool inner[U];
-    uint4 lo[U], hi[U];
+  constexpr int U = kPadBatch;
+  const int lane = threadIdx.x & 31;
+  for (long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5; unit < a.begin[a.n]; unit += (long long)gridDim.x * 8) {
+    int m = 0;
+    while (unit >= a.begin[m + 1]) ++m;
+    const int ll = a.log_lanes[m], L = 1 << ll, lw = lane & (L - 1);
+    const int groups = a.ldd[m] / 8, segments = (groups + U * L - 1) / (U * L);
+    const long long rows = (unit - a.begin[m]) / segments, row = rows * (32 >> ll) + (lane >> ll);
+    const int j0 = int(unit - a.begin[m] - rows * segments) * U * L;
+    const bool live = row < a.rows[m];
+    const uint16_t* first = a.src[m];
+    const uint16_t* end = first + (a.rows[m] - 1) * a.lds[m] + a.cols[m];
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(first + (live ? row : 0) * a.lds[m]);
+    const int shift = int(addr & 15) * 8;
+    const uint16_t* base = reinterpret_cast<const uint16_t*>(addr & ~uintptr_t(15));
+    uint4* out = reinterpret_cast<uint4*>(a.dst[m] + (live ? row : 0) * a.ldd[m]);
+    // the row's aligned word j; nothing outside the matrix is read
+    auto word = [&](int j) {
+      const uint16_t* p = base + (long long)j * 8;
+      if (p >= first && p + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(p));
+      union {
+        uint4 v;
+        uint16_t e[8];
+      } r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r.e[e] = p + e >= first && p + e < end ? p[e] : uint16_t(0);
+      return r.v;
+    };
+    uint4 w[U + 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      w[u] = live && j0 + u * L + lw <= groups ? word(j0 + u * L + lw) : make_uint4(0, 0, 0, 0);
+    w[U] = live && lw == 0 && j0 + U * L <= groups ? word(j0 + U * L) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long i = i0 + u * step;
-      left[u] = -1;
-      inner[u] = false;
-      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
-      if (i >= total) continue;
-      int m = 0;
-      while (i >= a.begin[m + 1]) ++m;
-      const unsigned at = unsigned(i - a.begin[m]);  // below 2^32 groups of a matrix (checked by the host)
-      const unsigned groups = unsigned(a.ldd[m]) / 8;
-      const unsigned row = at / groups;
-      const int col = int(at - row * groups) * 8;
-      src[u] = a.src[m] + (long long)row * a.lds[m] + col;
-      dst[u] = reinterpret_cast<uint4*>(a.dst[m] + (long long)row * a.ldd[m] + col);
-      left[u] = a.cols[m] - col;
-      // the two aligned 16-byte words around the 8 elements, where both lie inside this row
-      inner[u] = col >= 8 && left[u] >= 16;
-      if (inner[u]) {
-        const uint4* w = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src[u]) & ~uintptr_t(15));
-        lo[u] = __ldg(w);
-        hi[u] = __ldg(w + 1);
-      }
-    }
+      // the next word: the next lane's, or the first lane's of the next batch entry
+      uint4 hi;
+      const uint32_t* lo = &w[u].x;
+      const uint32_t* up = &w[u + 1].x;
+      uint32_t* h = &hi.x;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (left[u] < 0) continue;
-      if (inner[u]) {
-        *dst[u] = shift_words(lo[u], hi[u], int(reinterpret_cast<uintptr_t>(src[u]) & 15) * 8);
-      } else {
-        union {
-          uint4 v;
-          uint16_t e[8];
-        } r;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r.e[e] = e < left[u] ? src[u][e] : uint16_t(0);
-        *dst[u] = r.v;
-      }
+      for (int i = 0; i < 4; ++i) h[i] = __shfl_sync(0xffffffffu, lw == 0 ? up[i] : lo[i], (lw + 1) & (L - 1), L);
+      // (lane 0 offers the next entry's word to the last lane; its own next word comes from lane 1)
+      const int j = j0 + u * L + lw;
+      if (live && j < groups) out[j] = shift_words(w[u], hi, shift);
     }
   }
 }
@@ -1269,16 +1274,17 @@ struct Padder {
     a.rows[i] = int(m.rows);
     a.cols[i] = int(m.cols);
     a.ldd[i] = int(ld);
-    a.begin[i + 1] = a.begin[i] + m.rows * (ld / 8);
+    int ll = 0;
+    while (ll < 5 && (1 << ll) < ld / 8) ++ll;
+    a.log_lanes[i] = ll;
+    const int64_t words = int64_t(kPadBatch) << ll;
+    a.begin[i + 1] = a.begin[i] + (m.rows + (32 >> ll) - 1) / (32 >> ll) * ((ld / 8 + words - 1) / words);
     m.p = d;
     m.ld = ld;
   }
   b2_status run(cudaStream_t st) {
     if (a.n == 0) return B2_OK;
-    for (int i = 0; i < a.n; ++i)
-      if (a.begin[i + 1] - a.begin[i] > UINT32_MAX)
-        return set_error(B2_ERR_UNSUPPORTED, "gated_mlp: an operand of unaligned rows is too large to copy");
-    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 255) / 256, 148 * 16));
+    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 7) / 8, 148 * 16));
     return launch_chained(gated_pad_kernel, dim3(blocks), 256, 0, st, "gated pad launch", a);
   }
 };
@@ -1485,9 +1491,9 @@ b2_status launch_few(const FewArgs& a, cudaStream_t st) {
 // 32 where the projections' CTAs are resident at once: 24 tokens 13 against 22 us
 // (1024 x 4096), 32 tokens 8.4 against 14.7 us (512 x 1536); where they are
 // not, 24 tokens take 33 against 31 us (2048 x 5464).  Rows of Wd at any
-// alignment: one token 27 against 45 us with a padded copy (2048 x 5461), 16
-// tokens 34 against 39.  Where x, Wg and Wu have them too, copies pay: 80 against
-// 61 us (2045 x 5461).
+// alignment: one token 27 against 47 us with a padded copy (2048 x 5461), 16
+// tokens 34 against 39.  Where x, Wg and Wu have them too, copies pay: 81 against
+// 56 us (2045 x 5461).
 template <int NT>
 bool few_resident(int64_t rows) {
   using C = FewConfig<kGate, NT, true>;
