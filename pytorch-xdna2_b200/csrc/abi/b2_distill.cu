@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kShortThreads = 128;
 constexpr int kMaxTop = 1024;        // teacher entries per row
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -164,7 +165,7 @@ __device__ __forceinline__ float warp_reduce(float v, F f) {
   for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ float block_reduce(float v, float* scratch, F f) {
   v = warp_reduce(v, f);
   __syncthreads();
@@ -172,7 +173,7 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch, F f) {
   __syncthreads();
   v = scratch[0];
 #pragma unroll
-  for (int i = 1; i < kWarps; ++i) v = f(v, scratch[i]);
+  for (int i = 1; i < THREADS / 32; ++i) v = f(v, scratch[i]);
   return v;
 }
 
@@ -183,7 +184,7 @@ __host__ __device__ constexpr int padded_top(int K) { return (K + 3) / 4 * 4; }
 struct TeacherSmem {
   float* p;
   int* id;
-  float* scratch;  // [kWarps]
+  float* scratch;  // a float a warp
 };
 
 struct Teacher {
@@ -195,11 +196,12 @@ struct Teacher {
 
 // The row's teacher: probabilities and ids into shared memory (absent entries:
 // p = 0, id = -1).
+template <int THREADS>
 __device__ __forceinline__ Teacher load_teacher(const Args& a, long long r, const TeacherSmem& sm) {
   Teacher t;
   float m = -INFINITY;
   int bad = 0, nan = 0;
-  for (int k = threadIdx.x; k < padded_top(a.K); k += kThreads) {
+  for (int k = threadIdx.x; k < padded_top(a.K); k += THREADS) {
     long long id = -1;
     if (k < a.K)
       id = a.ids64 ? static_cast<const long long*>(a.ids)[r * a.ldi + k]
@@ -217,20 +219,20 @@ __device__ __forceinline__ Teacher load_teacher(const Args& a, long long r, cons
   }
   t.bad = __syncthreads_or(bad);
   const bool has_nan = __syncthreads_or(nan);
-  t.m = block_reduce(m, sm.scratch, [](float x, float y) { return fmaxf(x, y); });
+  t.m = block_reduce<THREADS>(m, sm.scratch, [](float x, float y) { return fmaxf(x, y); });
   t.any = t.m > -INFINITY || has_nan;
   float s = 0.f;
   const float c = kLog2e / a.tau;
-  for (int k = threadIdx.x; k < a.K; k += kThreads) {
+  for (int k = threadIdx.x; k < a.K; k += THREADS) {
     const float v = sm.p[k];
     const float e = v == -INFINITY ? 0.f : ex2((v - t.m) * c);
     sm.p[k] = e;
     s += e;
   }
-  t.mass = block_reduce(s, sm.scratch, [](float x, float y) { return x + y; });
+  t.mass = block_reduce<THREADS>(s, sm.scratch, [](float x, float y) { return x + y; });
   const float inv = 1.f / t.mass;
   if (t.any)
-    for (int k = threadIdx.x; k < a.K; k += kThreads) sm.p[k] *= inv;
+    for (int k = threadIdx.x; k < a.K; k += THREADS) sm.p[k] *= inv;
   __syncthreads();
   return t;
 }
@@ -463,17 +465,17 @@ __global__ void __launch_bounds__(1024) distill_begin_kernel(const Args a) {
 // head, the last also the tail).  Few rows are bound by the latency of one, 8 us
 // (one row of 32000 bf16 logits over 8 CTAs); 900 rows with the gradient take
 // 34 us, 3.4 TB/s, in eight CTAs a SM.
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int cluster) {
+template <typename T, bool GRAD, int THREADS>
+__global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int cluster) {
   constexpr int E = Vec16<T>::N;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint4* held = reinterpret_cast<uint4*>(smem_raw);
-  __shared__ float teacher_scratch[kWarps];
+  __shared__ float teacher_scratch[THREADS / 32];
   float* teacher_p0 = reinterpret_cast<float*>(held + a.tile);
   const TeacherSmem teacher{teacher_p0, reinterpret_cast<int*>(teacher_p0 + padded_top(a.K)), teacher_scratch};
   __shared__ uint64_t bar;
   __shared__ float share[2];          // this CTA's maximum and sum, read by the cluster
-  __shared__ float scratch[2][kWarps];
+  __shared__ float scratch[2][THREADS / 32];
   __shared__ int last_row;
   const int rank = cluster > 1 ? int(cluster_ctarank()) : 0;
   const long long r = blockIdx.x / cluster;
@@ -507,14 +509,14 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
   };
   if (!skip_weight && v1 > v0) fetch(v0);
   Teacher tch{};
-  if (!skip_weight) tch = load_teacher(a, r, teacher);
+  if (!skip_weight) tch = load_teacher<THREADS>(a, r, teacher);
   const bool skip = skip_weight || !(tch.any || tch.bad);
   float loss = 0.f;
   if (skip) {
     if (!skip_weight && v1 > v0) landed();  // no copy may be in flight when the CTA leaves
     if constexpr (GRAD) {
       const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (long long i = v0 + threadIdx.x; i < v1; i += kThreads) put_vec<T>(out + part.head + i * E, zero, out_aligned);
+      for (long long i = v0 + threadIdx.x; i < v1; i += THREADS) put_vec<T>(out + part.head + i * E, zero, out_aligned);
       if (rank == 0 && threadIdx.x < part.head) out[threadIdx.x] = T(0);
       if (rank == cluster - 1 && threadIdx.x < part.tail) out[part.head + part.vecs * E + threadIdx.x] = T(0);
     }
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
         fetch(b);
       }
       landed();
-      run.add_slice(held, int(threadIdx.x), int(min(a.tile, v1 - b)), kThreads);
+      run.add_slice(held, int(threadIdx.x), int(min(a.tile, v1 - b)), THREADS);
     }
     MaxSum ms = run.ms;
     // this CTA's pair
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
         scratch[1][threadIdx.x >> 5] = ms.s;
       }
       __syncthreads();
-      ms = warp_pair<kWarps>({scratch[0][threadIdx.x % kWarps], scratch[1][threadIdx.x % kWarps]}, c);
+      ms = warp_pair<THREADS / 32>({scratch[0][threadIdx.x % (THREADS / 32)], scratch[1][threadIdx.x % (THREADS / 32)]}, c);
     }
     if (cluster > 1) {
       if (threadIdx.x == 0) {
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
       const float ln_mass = logf(tch.mass);
       const Prob<T> qs(c, ms.m, l2s);
       float sum = 0.f;
-      for (int k = threadIdx.x; k < a.K; k += kThreads) {
+      for (int k = threadIdx.x; k < a.K; k += THREADS) {
         const float p = teacher.p[k];
         const int id = teacher.id[k];
         if (id < 0 || p == 0.f) continue;
@@ -588,7 +590,7 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
         const float logq = qs.log2q(load1(row + id)) * kLn2;
         sum += p * (logp - logq);
       }
-      loss = block_reduce(sum, scratch[0], [](float x, float y) { return x + y; }) * a.tau * a.tau;
+      loss = block_reduce<THREADS>(sum, scratch[0], [](float x, float y) { return x + y; }) * a.tau * a.tau;
       if (tch.bad) loss = __int_as_float(0x7fc00000);
       if (threadIdx.x == 0) {
         a.stats[2 * r] = ms.m;
@@ -605,14 +607,14 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
           fetch(b);
           landed();
         }
-        grad_slice<T>(held, out + part.head + b * E, int(threadIdx.x), int(min(a.tile, v1 - b)), kThreads, q, f);
+        grad_slice<T>(held, out + part.head + b * E, int(threadIdx.x), int(min(a.tile, v1 - b)), THREADS, q, f);
       }
       if (has_head) store1(out + threadIdx.x, f * q(edge));
       if (has_tail) store1(out + part.head + part.vecs * E + threadIdx.x, f * q(edge2));
       __syncthreads();  // the entries' elements are written again, from both terms
       const long long lo = rank == 0 ? 0 : part.head + v0 * E;
       const long long hi = rank == cluster - 1 ? a.V : part.head + v1 * E;
-      for (int k = threadIdx.x; k < a.K; k += kThreads) {
+      for (int k = threadIdx.x; k < a.K; k += THREADS) {
         const int id = teacher.id[k];
         if (id < lo || id >= hi) continue;
         store1(out + id, f * (q(load1(row + id)) - teacher_p(teacher, a.K, k)));
@@ -635,17 +637,18 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
   if (!last_row) return;
   __threadfence();
   float sum = 0.f;
-  for (long long i = threadIdx.x; i < a.N; i += kThreads) sum += __ldcg(a.row_loss + i);
-  sum = block_reduce(sum, scratch[1], [](float x, float y) { return x + y; });
+#pragma unroll 8
+  for (long long i = threadIdx.x; i < a.N; i += THREADS) sum += __ldcg(a.row_loss + i);
+  sum = block_reduce<THREADS>(sum, scratch[1], [](float x, float y) { return x + y; });
   if (threadIdx.x == 0) *a.loss = sum;
 }
 
 // ---------------------------------------------------------------------------
 // The persistent kernel.  Three CTAs a SM, so that one's copies, another's
 // exponentials and a third's stores overlap; clusters of them walk the rows
-// cluster by cluster, each CTA with a ring of one to kRing slices.  Warp 8 runs
-// ahead: it reads a row's weight and teacher entries, starts the copy of the
-// slice unless the row is masked, meanwhile makes the teacher's probabilities
+// cluster by cluster, each CTA with a buffer for one slice.  Warp 8 runs ahead: it
+// reads the next row's weight and teacher entries, starts the copy of its slice
+// when the buffer is free unless the row is masked, meanwhile makes the teacher's probabilities
 // and, from the slice's entries, its part of the loss.  Warps 0..7 form the
 // slice's maximum and sum, exchange all that with the cluster's CTAs (a remote
 // store and a remote arrival each) and write the gradient; then the entries'
@@ -671,10 +674,9 @@ __global__ void __launch_bounds__(kThreads) distill_row_kernel(const Args a, int
 constexpr int kStreamWarps = 8;
 constexpr int kStreamThreads = (kStreamWarps + 1) * 32;
 constexpr int kStreamPerSm = 3;
-constexpr int kRing = 4;
 constexpr int kSlots = 2;
 
-// What the forward warp knows of a row in the ring.
+// What the forward warp knows of the row in the buffer.
 struct RowMeta {
   long long row;
   int skip, bad;
@@ -730,12 +732,12 @@ __device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity, 
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_kernel(const Args a, int cluster, int ring) {
+__global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_kernel(const Args a, int cluster) {
   constexpr int E = Vec16<T>::N;
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  __shared__ uint64_t full[kRing], top_full[kRing], empty[kRing], slot_bar[kSlots];
+  __shared__ uint64_t full, top_full, empty, slot_bar[kSlots];
   __shared__ float4 slot[kSlots][kMaxCluster];  // a slice's maximum, sum, loss part and P
-  __shared__ RowMeta meta[kRing];
+  __shared__ RowMeta meta;
   __shared__ float part[2][kStreamWarps][2];
   __shared__ float final_part[kStreamWarps];
   __shared__ int last_row;
@@ -744,15 +746,13 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
   const long long first = blockIdx.x / cluster, step = gridDim.x / cluster;
   const float c = kLog2e / a.tau;
   uint4* held = reinterpret_cast<uint4*>(smem_raw);
-  float* top_p = reinterpret_cast<float*>(held + ring * a.slice);
+  float* top_p = reinterpret_cast<float*>(held + a.slice);
   const int Kp = padded_top(a.K);
-  int* top_id = reinterpret_cast<int*>(top_p + (ring + 1) * Kp);
+  int* top_id = reinterpret_cast<int*>(top_p + 2 * Kp);  // two rows' entries
   if (tid == 0) {
-    for (int b = 0; b < kRing; ++b) {
-      mbar_init(smem_u32(&full[b]), 1);
-      mbar_init(smem_u32(&top_full[b]), 1);
-      mbar_init(smem_u32(&empty[b]), kStreamWarps);
-    }
+    mbar_init(smem_u32(&full), 1);
+    mbar_init(smem_u32(&top_full), 1);
+    mbar_init(smem_u32(&empty), kStreamWarps);
     for (int b = 0; b < kSlots; ++b) mbar_init(smem_u32(&slot_bar[b]), uint32_t(cluster));
     fence_barrier_init();
   }
@@ -806,34 +806,33 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
     Ahead next{};
     if (first < a.N) next = look(first, 0);
     for (long long r = first; r < a.N; r += step, ++n) {
-      const int b = int(n % ring);
-      const int top_at = int(n % (ring + 1));
+      const int top_at = int(n & 1);
       const Ahead h = next;
       bool ok = true;
-      if (n >= ring) ok = mbar_wait_parked<false>(smem_u32(&empty[b]), uint32_t((n / ring - 1) & 1), a.status);
+      if (n > 0) ok = mbar_wait_parked<false>(smem_u32(&empty), uint32_t((n - 1) & 1), a.status);
       if (!__all_sync(0xffffffffu, ok)) break;
       const T* row = static_cast<const T*>(a.z) + r * a.ldz;
       const RowParts<T> parts(row, a.V);
       const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
-      if (lane < 8) meta[b].head[lane] = h.edge;
-      else if (lane < 16) meta[b].tail[lane - 8] = h.edge;
+      if (lane < 8) meta.head[lane] = h.edge;
+      else if (lane < 16) meta.tail[lane - 8] = h.edge;
       if (lane == 0) {
-        meta[b].row = r;
-        meta[b].skip = h.skip;
-        meta[b].bad = h.bad;
-        meta[b].w = h.w;
+        meta.row = r;
+        meta.skip = h.skip;
+        meta.bad = h.bad;
+        meta.w = h.w;
       }
       __syncwarp();
       if (lane == 0) {
         const uint32_t bytes = h.skip ? 0u : uint32_t((v1 - v0) * 16);
         if (bytes) {
-          mbar_arrive_expect_tx(smem_u32(&full[b]), bytes);
+          mbar_arrive_expect_tx(smem_u32(&full), bytes);
           const uint8_t* src = reinterpret_cast<const uint8_t*>(row + parts.head) + v0 * 16;
-          const uint32_t dst = smem_u32(held + b * a.slice);
+          const uint32_t dst = smem_u32(held);
           for (uint32_t at = 0; at < bytes; at += 16384)
-            bulk_load_1d(dst + at, src + at, min(16384u, bytes - at), smem_u32(&full[b]));
+            bulk_load_1d(dst + at, src + at, min(16384u, bytes - at), smem_u32(&full));
         } else {
-          mbar_arrive(smem_u32(&full[b]));
+          mbar_arrive(smem_u32(&full));
         }
         if (h.bad && rank == 0) record_status(a.status, B2_ERR_INVALID);
       }
@@ -852,14 +851,14 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         const int* ids = top_id + top_at * Kp;
         const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
         const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
-        const uint4* slice = held + b * a.slice;
-        mbar_wait_parked<false>(smem_u32(&full[b]), uint32_t(n / ring) & 1u, a.status);
+        const uint4* slice = held;
+        mbar_wait_parked<false>(smem_u32(&full), uint32_t(n & 1), a.status);
         float top = -INFINITY;
         for (int k = lane; k < a.K; k += 32) {
           const float pk = p[k] * inv;
           p[k] = pk;
           if (ids[k] >= lo && ids[k] < hi && pk != 0.f)
-            top = fmaxf(top, slice_logit<T>(slice, meta[b], parts, v0, ids[k]));
+            top = fmaxf(top, slice_logit<T>(slice, meta, parts, v0, ids[k]));
         }
         top = warp_reduce(top, [](float x, float y) { return fmaxf(x, y); });
         if (!(fabsf(top) < INFINITY)) top = 0.f;
@@ -868,7 +867,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         for (int k = lane; k < a.K; k += 32) {
           const float pk = p[k];
           if (ids[k] < lo || ids[k] >= hi || pk == 0.f) continue;
-          const float z = slice_logit<T>(slice, meta[b], parts, v0, ids[k]);
+          const float z = slice_logit<T>(slice, meta, parts, v0, ids[k]);
           // a closed entry makes the loss infinite, also in a slice of nothing else
           side += z == -INFINITY ? INFINITY : pk * (logf(pk) - (z - top) * inv_tau);
           P += pk;
@@ -876,18 +875,17 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         side = warp_reduce(side, [](float x, float y) { return x + y; });
         P = warp_reduce(P, [](float x, float y) { return x + y; });
         if (lane == 0) {
-          meta[b].side = side;
-          meta[b].P = P;
-          meta[b].top = top;
+          meta.side = side;
+          meta.P = P;
+          meta.top = top;
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&top_full[b]));
-      if (r + step < a.N) next = look(r + step, int((n + 1) % (ring + 1)));
+      if (lane == 0) mbar_arrive(smem_u32(&top_full));
+      if (r + step < a.N) next = look(r + step, int((n + 1) & 1));
     }
     // every copy lands before the CTA goes away (also if the others gave up)
-    for (long long i = max(0LL, n - ring); i < n; ++i)
-      mbar_wait_parked<false>(smem_u32(&full[i % ring]), uint32_t(i / ring) & 1u, a.status);
+    if (n > 0) mbar_wait_parked<false>(smem_u32(&full), uint32_t((n - 1) & 1), a.status);
   } else {
     // ------------------------------ the compute warps -----------------------
     long long counted = 0;  // rows with statistics
@@ -895,8 +893,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
     bool ok = true;
     // Statistics of the row in buffer b, its loss, its gradient; frees the buffer.
     auto finish = [&](long long n, MaxSum ms, float parts_m, float side, float P) {
-      const int b = int(n % ring);
-      const RowMeta& mt = meta[b];
+      const RowMeta& mt = meta;
       const long long r = mt.row;
       const float l2s = log2f(ms.s);
       if (rank == 0 && warp == 0) {
@@ -920,7 +917,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         const RowParts<T> parts(row, a.V);
         const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
         const int count = int(v1 - v0);
-        const uint4* src = held + b * a.slice;
+        const uint4* src = held;
         const float f = mt.bad ? __int_as_float(0x7fc00000) : mt.w * a.tau;
         const Prob<T> q(c, ms.m, l2s);
         T* dst = out + parts.head + v0 * E;
@@ -931,7 +928,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         compute_sync();  // the entries' elements are written again, from both terms
         const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
         const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
-        const int top_at = int(n % (ring + 1));
+        const int top_at = int(n & 1);
         const TeacherSmem top{top_p + top_at * Kp, top_id + top_at * Kp, nullptr};
         for (int k = tid; k < a.K; k += kStreamWarps * 32) {
           const int id = top.id[k];
@@ -940,14 +937,13 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&empty[b]));
+      if (lane == 0) mbar_arrive(smem_u32(&empty));
     };
     long long n = 0;
     for (long long r = first; r < a.N && ok; r += step, ++n) {
-      const int b = int(n % ring);
-      ok = mbar_wait_parked<false>(smem_u32(&full[b]), uint32_t(n / ring) & 1u, a.status);
+      ok = mbar_wait_parked<false>(smem_u32(&full), uint32_t(n & 1), a.status);
       if (!ok) break;
-      const RowMeta& mt = meta[b];
+      const RowMeta& mt = meta;
       const T* row = static_cast<const T*>(a.z) + r * a.ldz;
       const RowParts<T> parts(row, a.V);
       const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
@@ -968,10 +964,10 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
           else a.row_loss[r] = 0.f;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&empty[b]));
+        if (lane == 0) mbar_arrive(smem_u32(&empty));
         continue;
       }
-      const uint4* src = held + b * a.slice;
+      const uint4* src = held;
       Running<T> run(c);
       if (rank == 0 && tid < parts.head) run.add1(mt.head[tid]);
       if (rank == cluster - 1 && tid < parts.tail) run.add1(mt.tail[tid]);
@@ -983,7 +979,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         part[flip][warp][0] = ms.m;
         part[flip][warp][1] = ms.s;
       }
-      ok = mbar_wait_parked<false>(smem_u32(&top_full[b]), uint32_t(n / ring) & 1u, a.status);
+      ok = mbar_wait_parked<false>(smem_u32(&top_full), uint32_t(n & 1), a.status);
       compute_sync();
       ms = warp_pair<kStreamWarps>({part[flip][lane % kStreamWarps][0], part[flip][lane % kStreamWarps][1]}, c);
       // the entries' part of the loss, now relative to the slice's maximum
@@ -1065,7 +1061,7 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const Args a, int
     const float w = row_factor(a, r);
     __syncthreads();
     Teacher tch{};
-    if (w != 0.f) tch = load_teacher(a, r, teacher);
+    if (w != 0.f) tch = load_teacher<kThreads>(a, r, teacher);
     if (w == 0.f || !(tch.any || tch.bad)) {
       const uint4 zero = make_uint4(0, 0, 0, 0);
       for (long long i = v0 + tid; i < v1; i += kThreads) put_vec<T>(out + part.head + i * E, zero, out_aligned);
@@ -1119,7 +1115,8 @@ constexpr long long kTileVecs = 208 * 1024 / 16;
 constexpr size_t kTopBytes = size_t(kMaxTop) * 8;
 // distill_stream_kernel: dynamic shared memory of a CTA, three to a SM.
 constexpr size_t kStreamSmem = 73 * 1024;
-constexpr long long kStreamMinBytes = 4000;
+// rows that distill_row_kernel takes with kShortThreads threads
+constexpr long long kShortBytes = 48 * 1024;
 
 b2_status check_args(const char* who, const Args& a, int dtype, int t_dtype, int ids_dtype) {
   if (a.N < 0 || a.V < 1 || a.K < 0) return set_error(B2_ERR_INVALID, "%s: bad shape", who);
@@ -1179,15 +1176,25 @@ b2_status launch_fwd(Args a, cudaStream_t st) {
   const size_t top = size_t(padded_top(a.K)) * 8;
   while (cluster < kMaxCluster && size_t((vecs + cluster - 1) / cluster) * 16 + 2 * top > kStreamSmem) cluster *= 2;
   a.slice = (vecs + cluster - 1) / cluster;
-  const size_t per_row = size_t(a.slice) * 16 + top;
-  const int ring = kStreamSmem > top ? int(std::min<size_t>(kRing, (kStreamSmem - top) / per_row)) : 0;
-  // Persistent clusters where every CTA gets at least two slices of a good size,
-  // else CTAs of a row's own (bf16, with the gradient): 8192 x 131072 876 us
-  // against 958, 8192 x 8192 98 against 107, 8192 x 2000 76 against 81; 300 x
+  const size_t held = size_t(a.slice) * 16 + 2 * top;
+  const bool many = a.N * cluster >= 2LL * kStreamPerSm * sms;
+  if (many && vecs * 16 <= kShortBytes) {
+    // Many short rows: a CTA each, of half the threads, so that twice as many
+    // rows overlap their latencies (8192 rows with the gradient: 2000 bf16 logits
+    // 50 us, with all threads 81, in the persistent kernel 76; 16000 logits 119,
+    // 143 and 146; 24000 logits 173 and 185 in the persistent one, 2000 rows of
+    // 32000 68 and 64; 500 rows of 2000 11.1 us against 10.7 with all threads).
+    a.slice = a.tile = vecs;
+    auto kern = distill_row_kernel<T, GRAD, kShortThreads>;
+    static bool configured[64] = {};
+    B2_TRY(allow_smem(kern, kShortBytes + kTopBytes, configured, dev));
+    return launch_clusters(kern, a.N, 1, kShortThreads, size_t(vecs) * 16 + top, st, a, 1);
+  }
+  // Persistent clusters where every CTA gets at least two slices, else CTAs of a
+  // row's own (bf16, with the gradient): 8192 x 131072 876 us against 958; 300 x
   // 32000 18.4 against 17.1, 148 x 32000 13.3 against 12.5, where rows are too
-  // few; the same at 1800 x 32000 (59).  Rows much shorter than these cost a CTA
-  // the latency of a row, 8 us, in either.
-  if (ring >= 1 && a.slice * 16 >= kStreamMinBytes && a.N * cluster >= 2LL * kStreamPerSm * sms) {
+  // few; the same at 1800 x 32000 (59).
+  if (many && held <= kStreamSmem) {
     auto kern = distill_stream_kernel<T, GRAD>;
     static bool configured[64] = {};
     B2_TRY(allow_smem(kern, kStreamSmem, configured, dev));
@@ -1203,7 +1210,7 @@ b2_status launch_fwd(Args a, cudaStream_t st) {
       if (n < 1) return set_error(B2_ERR_CUDA, "distill: no cluster of %d fits", cluster);
       clusters = std::min(n, kStreamPerSm * sms / cluster);
     }
-    return launch_clusters(kern, clusters, cluster, kStreamThreads, ring * per_row + top, st, a, cluster, ring);
+    return launch_clusters(kern, clusters, cluster, kStreamThreads, held, st, a, cluster);
   }
   // longer rows over more CTAs; so are few rows, down to 4 KB a CTA
   cluster = 1;
@@ -1212,7 +1219,7 @@ b2_status launch_fwd(Args a, cudaStream_t st) {
     cluster *= 2;
   a.slice = (vecs + cluster - 1) / cluster;
   a.tile = std::min(a.slice, a.slice <= kSliceVecs ? kSliceVecs : kTileVecs);
-  auto kern = distill_row_kernel<T, GRAD>;
+  auto kern = distill_row_kernel<T, GRAD, kThreads>;
   static bool configured[64] = {};
   B2_TRY(allow_smem(kern, size_t(kTileVecs) * 16 + kTopBytes, configured, dev));
   return launch_clusters(kern, a.N, cluster, kThreads, size_t(a.tile) * 16 + top, st, a, cluster);
