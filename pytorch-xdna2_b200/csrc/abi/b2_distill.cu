@@ -17,8 +17,8 @@
 // longer than one CTA's share; the gradient is then written from the held row.
 // Two kernels do that: distill_stream_kernel, persistent, loads rows ahead of
 // the arithmetic and keeps the memory system busy through it (many long rows);
-// distill_row_kernel gives every row CTAs of its own (few rows, short rows, or
-// rows that no cluster holds, which it reads twice).
+// distill_row_kernel gives every row CTAs of its own (few rows; many short rows,
+// with fewer threads each; or rows that no cluster holds, which it reads twice).
 //
 // Exponents are base 2: with c = log2(e) / tau and R = max * c (rounded), a
 // thread's sum is sum 2^(z c - R), one fused multiply-add and one 2^x per logit;
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
 // whose slice sums need nothing of the other slices.
 //
 // 8192 rows of 131072 bf16 logits with 64 entries, a seventh of them masked:
-// 876 us with the gradient (4.5 TB/s of the 6.45 measured), 530 us the loss
+// 858 us with the gradient (5.0 TB/s of the 6.45 measured), 530 us the loss
 // alone; a row's 10 us in a CTA are 2.5 of copy, 2.5 of sums, 0.7 of reduction,
 // 1.6 of exchange, 2.1 of gradient and 0.9 of entries.  (One CTA of 16 warps a SM
 // with a ring of three slices took 1610 us: a row at a time leaves the SM waiting
@@ -1191,7 +1191,7 @@ b2_status launch_fwd(Args a, cudaStream_t st) {
     return launch_clusters(kern, a.N, 1, kShortThreads, size_t(vecs) * 16 + top, st, a, 1);
   }
   // Persistent clusters where every CTA gets at least two slices, else CTAs of a
-  // row's own (bf16, with the gradient): 8192 x 131072 876 us against 958; 300 x
+  // row's own (bf16, with the gradient): 8192 x 131072 858 us against 958; 300 x
   // 32000 18.4 against 17.1, 148 x 32000 13.3 against 12.5, where rows are too
   // few; the same at 1800 x 32000 (59).
   if (many && held <= kStreamSmem) {
