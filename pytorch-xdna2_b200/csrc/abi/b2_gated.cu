@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(256) gated_pad_kernel(const __grid_constant__ 
 // memory (asynchronously, and read back by the same lane, so nothing has to be
 // synchronized).  Partial sums are added in warp and CTA order.
 //
-// One token, D 1024, F 4096 (25 MB of weights): 9.6 us; 4096 x 12288 (302 MB):
+// One token, D 1024, F 4096 (25 MB of weights): 10.2 us; 4096 x 12288 (302 MB):
 // 57 us, 5.3 TB/s.  Loads straight to registers took 13 and 68 us; one
 // cooperative kernel over both products with TMA boxes 18 and 67 us; 64 k a
 // step, copied in whole 128-byte lines, 14 and 66 us.
@@ -899,6 +899,12 @@ constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kFewStages = 6;
 constexpr int kFewTokens = 32;
+// Up to this many tokens Wd's product takes h as two bf16 numbers, the rounded h
+// and what the rounding left, as columns that the instruction has free: y's error
+// is then that of its own rounding alone (1.4 times that otherwise).  One token,
+// 1024 x 4096: 10.2 us, 9.6 without; 4096 x 12288 56.6 and 56.3; eight tokens would
+// need a second column block, 64.8 and 59.4.
+constexpr int kRestTokens = 4;
 
 struct FewMat {
   const uint16_t* p;
@@ -913,6 +919,8 @@ struct FewArgs {
   int early;     // the weights were not written by the kernel before this one
   uint16_t *out, *o1, *o2, *o3;  // kGate: h, P, A, R (or null); kStore: y
   long long ldo;            // of all of them
+  uint16_t* rest;           // what rounding h left, [M][ldr], or null: kGate writes it, kStore's tokens go on with it
+  long long ldr;
 };
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -1016,8 +1024,10 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
   bool xlive[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    xlive[n] = n * 8 + g < a.M;
-    xrow[n] = a.x.p + (long long)(xlive[n] ? n * 8 + g : 0) * a.x.ld;
+    const int r = n * 8 + g;
+    const bool second = EPI == kStore && a.rest && r >= a.M;
+    xlive[n] = r < (EPI == kStore && a.rest ? 2 * a.M : a.M);
+    xrow[n] = second ? a.rest + (xlive[n] ? r - a.M : 0) * a.ldr : a.x.p + (long long)(xlive[n] ? r : 0) * a.x.ld;
   }
   float c[kMats][NT][4];
 #pragma unroll
@@ -1117,25 +1127,30 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
   if (rank == 0) {
     for (int t = threadIdx.x; t < kOut; t += kFewThreads) {
       const int row = row0 + (t & 15), token = t >> 4;
-      float v[kMats];
-#pragma unroll
-      for (int m = 0; m < kMats; ++m) {
-        v[m] = total[m][t];
+      if (row >= a.rows || token >= a.M) continue;
+      auto cluster_total = [&](int m, int at) {
+        float v = total[m][at];
         for (int r = 1; r < cluster; ++r) {
           float o;
           asm volatile("ld.shared::cluster.f32 %0, [%1];"
                        : "=f"(o)
-                       : "r"(mapa_shared(smem_u32(&total[m][t]), uint32_t(r)))
+                       : "r"(mapa_shared(smem_u32(&total[m][at]), uint32_t(r)))
                        : "memory");
-          v[m] += o;
+          v += o;
         }
-      }
-      if (row >= a.rows || token >= a.M) continue;
+        return v;
+      };
+      float v[kMats];
+#pragma unroll
+      for (int m = 0; m < kMats; ++m) v[m] = cluster_total(m, t);
       const long long at = (long long)token * a.ldo + row;
       if constexpr (EPI == kGate) {
         float act, slope;
         act_both<ACT>(v[0], act, slope);
-        a.out[at] = cvt1(act * v[1]);
+        const float h = act * v[1];
+        const uint16_t hi = cvt1(h);
+        a.out[at] = hi;
+        if (a.rest) a.rest[token * a.ldr + row] = fabsf(bf2f(hi)) < INFINITY ? cvt1(h - bf2f(hi)) : uint16_t(0);
         if (a.o1) {
           const Factors2 f = pack_factors(slope * v[1], 0.f, act, 0.f);
           a.o1[at] = uint16_t(f.p);
@@ -1143,7 +1158,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
           a.o3[at] = uint16_t(f.r);
         }
       } else {
-        a.out[at] = cvt1(v[0]);
+        a.out[at] = cvt1(a.rest ? v[0] + cluster_total(0, t + 16 * a.M) : v[0]);
       }
     }
   }
@@ -1472,9 +1487,10 @@ b2_status launch_few_nt(const FewArgs& a, cudaStream_t st) {
 
 template <int EPI, int ACT, bool ALIGNED>
 b2_status launch_few_rows(const FewArgs& a, cudaStream_t st) {
-  if (a.M <= 8) return launch_few_nt<EPI, 1, ACT, ALIGNED>(a, st);
-  if (a.M <= 16) return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
-  if (a.M <= 24) return launch_few_nt<EPI, 3, ACT, ALIGNED>(a, st);
+  const int tokens = EPI == kStore && a.rest ? 2 * a.M : a.M;
+  if (tokens <= 8) return launch_few_nt<EPI, 1, ACT, ALIGNED>(a, st);
+  if (tokens <= 16) return launch_few_nt<EPI, 2, ACT, ALIGNED>(a, st);
+  if (tokens <= 24) return launch_few_nt<EPI, 3, ACT, ALIGNED>(a, st);
   return launch_few_nt<EPI, 4, ACT, ALIGNED>(a, st);
 }
 template <int EPI, int ACT>
@@ -1507,7 +1523,7 @@ bool takes_few(const Mat& x, const Mat& wg, const Mat& wu) {
 
 // The forward of few tokens: two launches, no padded copies.
 b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd, int act, const Mat& h,
-                      uint16_t* factors, int64_t apart, void* y, int64_t ldy, cudaStream_t st) {
+                      uint16_t* factors, int64_t apart, uint16_t* rest, void* y, int64_t ldy, cudaStream_t st) {
   FewArgs a{};
   a.w[0] = few_mat(wg);
   a.w[1] = few_mat(wu);
@@ -1522,6 +1538,8 @@ b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd,
     a.o3 = factors + 2 * apart;
   }
   a.ldo = h.ld;
+  a.rest = rest;
+  a.ldr = up8(h.cols);
   B2_TRY((act == kSilu   ? launch_few<kGate, kSilu>(a, st)
           : act == kGelu ? launch_few<kGate, kGelu>(a, st)
                          : launch_few<kGate, kRelu>(a, st)));
@@ -1532,6 +1550,8 @@ b2_status few_forward(const Mat& x, const Mat& wg, const Mat& wu, const Mat& wd,
   d.rows = int(wd.rows);
   d.K = int(wd.cols);
   d.early = 1;
+  d.rest = rest;
+  d.ldr = a.ldr;
   d.out = static_cast<uint16_t*>(y);
   d.ldo = ldy;
   return launch_few<kStore, kSilu>(d, st);
@@ -1591,8 +1611,8 @@ extern "C" {
 size_t b2_gated_mlp_fwd_workspace_bytes(int64_t M, int64_t D, int64_t F, int64_t E) {
   if (M <= 0 || D <= 0 || F <= 0 || E <= 0) return 0;
   const FwdPlan p = fwd_plan({M, D, F, E}, current_sms());
-  return padded_bytes(M, F) + padded_bytes(M, D) + 2 * padded_bytes(F, D) + padded_bytes(E, F) +
-         std::max(p.gate.partial_bytes, p.down.partial_bytes) + 256;
+  return padded_bytes(M, F) + padded_bytes(std::min<int64_t>(M, kRestTokens), F) + padded_bytes(M, D) +
+         2 * padded_bytes(F, D) + padded_bytes(E, F) + std::max(p.gate.partial_bytes, p.down.partial_bytes) + 256;
 }
 
 b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up,
@@ -1616,7 +1636,8 @@ b2_status b2_gated_mlp_fwd_bf16(const void* x, int64_t ldx, const void* w_gate, 
   Mat mx{x, M, D, ldx}, mg{w_gate, F, D, ldg}, mu{w_up, F, D, ldu}, md{w_down, E, F, ldd};
   if (takes_few(mx, mg, mu)) {
     uint16_t* keep = static_cast<uint16_t*>(saved);
-    return few_forward(mx, mg, mu, md, act, h, keep ? keep + Fp : nullptr, Fp, y, ldy, st);
+    uint16_t* rest = M <= kRestTokens ? static_cast<uint16_t*>(ws.take(size_t(M) * Fp * 2)) : nullptr;
+    return few_forward(mx, mg, mu, md, act, h, keep ? keep + Fp : nullptr, Fp, rest, y, ldy, st);
   }
   Padder pad;
   pad.add(mx, ws);
