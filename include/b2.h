@@ -712,8 +712,9 @@ b2_status b2_distill_loss_bwd(const void* z, int64_t ldz, int dtype, int64_t N,
  * Wd^T.  x [M][D], w_gate and w_up [F][D], w_down [E][F], y [M][E], each with a
  * row stride in elements (any; rows that are not 16-byte aligned are copied to
  * the workspace first).  act 0: silu, 1: gelu (erf), 2: relu.  fp32 sums; h is
- * rounded to bf16 as an operand of the second product.  saved (may be NULL): what
- * the backward needs, 16-bit words [M][4][F rounded up to 8] (h as bf16, the
+ * rounded to bf16 as an operand of the second product (M <= 4 with aligned rows
+ * of x, w_gate and w_up: to two bf16 numbers).  saved (may be NULL): what the
+ * backward needs, 16-bit words [M][4][F rounded up to 8] (h as bf16, the
  * upper halves of u act'(g) and of act(g) as fp32, and the next 8 bits of both),
  * 16-byte aligned.  Workspace: b2_gated_mlp_fwd_workspace_bytes(), 256-byte aligned. */
 size_t b2_gated_mlp_fwd_workspace_bytes(int64_t M, int64_t D, int64_t F,

@@ -253,3 +253,29 @@ def test_refusals(dev):
                                  x.data_ptr(), 8, None, 4, 16, 24, 8, x.data_ptr(), need - 1, None)
     assert st == 5 and b"workspace" in L.b2_last_error()
     assert xdna_train.device_status(0) == 0
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+@pytest.mark.parametrize("D,F,E", [(64, 104, 40), (1024, 4096, 256), (512, 1531, 77)])
+def test_up_to_four_tokens_round_once(dev, M, D, F, E):
+    # h goes on as two bf16 numbers, which leave eps^2 of it; y is rounded once.  fp32 sums add less than 2^-16 of
+    # the absolute sums, as above.
+    x, wg, wu, wd, dy = make(M, D, F, E, 5)
+    with torch.no_grad():
+        y = lm.gated_mlp(*(t.to(dev) for t in (x, wg, wu, wd)))
+    ref, _ = reference(x, wg, wu, wd, dy, "silu")[0]
+    x, wg, wu, wd = (t.double().cuda() for t in (x, wg, wu, wd))
+    g, u = x @ wg.t(), x @ wu.t()
+    a = g * torch.sigmoid(g)
+    eh = 1.2 * 2.0 ** -20 * (u.abs() * (x.abs() @ wg.abs().t()) + a.abs() * (x.abs() @ wu.abs().t()))
+    inner = (EPS ** 2 + 2.0 ** -16) * ((a * u).abs() @ wd.abs().t()) + eh @ wd.abs().t()
+    err = (xdna_train.as_cuda(y).double() - ref).abs()
+    assert (err <= EPS * ref.abs() + 1.01 * inner).all()
+
+
+def test_few_tokens_keep_infinities(dev):
+    # an h beyond bf16's range is an infinity, and what its rounding left is not a NaN
+    x = torch.full((1, 8), 2.0 ** 60).bfloat16()
+    w = torch.full((8, 8), 2.0 ** 8).bfloat16()
+    y = lm.gated_mlp(x.to(dev), w.to(dev), w.to(dev), torch.ones(8, 8).bfloat16().to(dev), activation="relu")
+    assert (xdna_train.as_cuda(y) == float("inf")).all()
