@@ -982,9 +982,9 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       ok = mbar_wait_parked<false>(smem_u32(&top_full), uint32_t(n & 1), a.status);
       compute_sync();
       ms = warp_pair<kStreamWarps>({part[flip][lane % kStreamWarps][0], part[flip][lane % kStreamWarps][1]}, c);
-      // the entries' part of the loss, now relative to the slice's maximum
+      // the entries' part of the loss, now relative to the slice's maximum (in a closed slice it is infinite already)
       float side = mt.side, P = mt.P, slice_m = ms.m;
-      if (P != 0.f) side -= P * (mt.top - slice_m) / a.tau;
+      if (P != 0.f && slice_m > -INFINITY) side -= P * (mt.top - slice_m) / a.tau;
       if (cluster > 1) {
         const int at = int(counted % kSlots);
         if (warp == 0 && lane < cluster) {  // one lane per CTA of the cluster

@@ -276,3 +276,31 @@ def test_refusals(dev):
                                         ids.data_ptr(), 4, _abi.B2_I64, 4, 1.0, None, 0, z.data_ptr(), z.data_ptr(),
                                         None, 50, z.data_ptr(), 1000, None)
     assert st == 1 and b"row stride" in _abi.lib().b2_last_error()
+
+
+@pytest.mark.parametrize("N,V", [(900, 9001), (460, 40001), (250, 131072), (131, 262139)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_closed_slices(dev, N, V, dtype):
+    # a long part of a row closed (a masked range of the vocabulary), so that some CTA of the row's cluster sees
+    # nothing else: infinite loss where a live entry lies in it, as for a single closed logit, else a finite one
+    g = torch.Generator().manual_seed(V)
+    z = (torch.randn(N, V, generator=g) * 3).to(dtype)
+    t = torch.randn(N, 4, generator=g)
+    ids = torch.randint(0, V // 8, (N, 4), generator=g) + torch.arange(4) * (V // 4)  # one entry in each quarter
+    late, early = slice(V // 2 - 16, V), slice(0, V // 2 + 16)
+    z[2, late] = -math.inf                                   # entries on both sides
+    z[3, early] = -math.inf
+    z[4, late], ids[4, 2:] = -math.inf, -1                   # entries on the open side alone
+    z[5, early], ids[5, :2] = -math.inf, -1
+    z[6, late], ids[6, :2] = -math.inf, -1                   # on the closed side alone
+    z[7, late], t[7, 2:] = -math.inf, -math.inf              # those on the closed side have no probability
+    z[8, V // 8 + 16:] = -math.inf                           # all but a first part
+    z[9, late], z[9, 1] = -math.inf, math.nan
+    z[10, late], z[10, V - 1] = -math.inf, math.nan
+    loss, _ = check(z, t, ids, 2.0, None, "none", dev)
+    assert loss.isinf().nonzero().flatten().tolist() == [2, 3, 6, 8]
+    assert loss.isnan().nonzero().flatten().tolist() == [9, 10]
+    w = torch.ones(N)
+    w[9:11] = 0
+    loss, _ = check(z, t, ids, 2.0, w, "mean", dev)
+    assert loss.item() == math.inf
