@@ -20,11 +20,16 @@
 // distill_row_kernel gives every row CTAs of its own (few rows; many short rows,
 // with fewer threads each; or rows that no cluster holds, which it reads twice).
 //
+// Products that go into a sum are written as fused multiply-adds or as rounded
+// products, so that the kernels with and without the gradient round alike and
+// give the same loss.
+//
 // Exponents are base 2: with c = log2(e) / tau and R = max * c (rounded), a
 // thread's sum is sum 2^(z c - R), one fused multiply-add and one 2^x per logit;
 // since every later use refers to the same rounded R, its rounding cancels.
-// Where R is not finite (rows whose largest logit is the type's lowest value,
-// or an infinity) the difference is taken before the product.
+// Where R is large (rows far from zero, or whose largest logit is the type's
+// lowest value) or not finite, the difference is taken before the product: R's
+// rounding, 2^-24 of it, then no longer is a small exponent (kPlain).
 // The backward proper has nothing to do when the upstream gradient is 1 (a
 // loss that is differentiated directly); for any other value it writes the
 // gradient again from the logits and the row's statistics, so that each
@@ -43,6 +48,12 @@ constexpr int kMaxTop = 1024;        // teacher entries per row
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
+// Largest |R| of the plain form.  The bf16 gradient's exponent adds R to two other
+// offsets, each sum rounded at 2^-17 up to here: 10^-5 of an element, where its own
+// rounding is 2^-9; at |R| = 2^20 it would be a tenth, and from 2^31 on the rounding
+// of R alone overflows 2^x.  4096 rows of 131072 bf16 logits take 484 us with the
+// gradient in the plain form, 525 in the other (the loss alone 295 and 301).
+constexpr float kPlain = 256.f;
 
 enum Reduction : int { kMean = 0, kSum = 1, kNone = 2 };
 
@@ -130,17 +141,24 @@ __device__ __forceinline__ void cluster_wait() {
 struct MaxSum {
   float m, s;
 };
+// R = m c, rounded: never fused into what it is added to
+__device__ __forceinline__ float offset_of(float m, float c) { return __fmul_rn(m, c); }
+// What that rounding left of m c: a sum of the plain form is relative to R, others to m c itself
+__device__ __forceinline__ float left_of(float m, float c) {
+  const float r = offset_of(m, c);
+  return fabsf(r) < kPlain ? fmaf(m, c, -r) : 0.f;
+}
 // log2 of the factor that brings a sum relative to `from` to one relative to `to`
 __device__ __forceinline__ float rescale(float from, float to, float c) {
-  const float a = from * c, b = to * c;
-  return fabsf(a) < INFINITY && fabsf(b) < INFINITY ? a - b : (from - to) * c;
+  const float a = offset_of(from, c), b = offset_of(to, c);
+  return fabsf(a) < kPlain && fabsf(b) < kPlain ? a - b : fmaf(from - to, c, left_of(to, c) - left_of(from, c));
 }
 __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
   const float m = fmaxf(a.m, b.m);
   // -inf - -inf would be NaN: a side that saw nothing keeps its sum of 0 (or a NaN that it saw)
   const float fa = a.m == m ? 1.f : ex2(rescale(a.m, m, c));
   const float fb = b.m == m ? 1.f : ex2(rescale(b.m, m, c));
-  return {m, a.s * fa + b.s * fb};
+  return {m, fmaf(a.s, fa, b.s * fb)};
 }
 // The pair of W neighbouring lanes' pairs, in each of them: the maximum first,
 // then each lane's sum relative to it once, then the sum of those.
@@ -149,14 +167,14 @@ __device__ __forceinline__ MaxSum warp_pair(MaxSum v, float c) {
   float m = v.m;
 #pragma unroll
   for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float s = v.m == m ? v.s : v.s * ex2(rescale(v.m, m, c));
+  float s = v.m == m ? v.s : __fmul_rn(v.s, ex2(rescale(v.m, m, c)));
 #pragma unroll
   for (int o = W / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return {m, s};
 }
-// One value: 2^0 of the sum if it is the maximum, NaN if it is +inf (inf - inf)
-__device__ __forceinline__ MaxSum one_value(float x) {
-  return {x, x == INFINITY ? __int_as_float(0x7fc00000) : 1.f};
+// One value: 2^(x c - R) if it is the maximum, NaN if it is +inf (inf - inf)
+__device__ __forceinline__ MaxSum one_value(float x, float c) {
+  return {x, x == INFINITY ? __int_as_float(0x7fc00000) : ex2(left_of(x, c))};
 }
 
 template <typename F>
@@ -269,7 +287,7 @@ struct RowParts {
 };
 
 // A thread's running pair over 16-byte vectors of logits.  The common case --
-// its maximum so far times c is finite -- is one multiply-add, one 2^x and one
+// its maximum so far times c is below kPlain -- is one multiply-add, one 2^x and one
 // addition per logit; the test for it and for a new maximum is made once for up
 // to 8 vectors (some lane of a warp sees a new maximum nearly every time, so its
 // dozen instructions are the price of every test).
@@ -279,18 +297,18 @@ struct Running {
   float c;
   MaxSum ms;
   float ref;    // ms.m * c
-  bool plain;   // finite
+  bool plain;   // |ref| < kPlain
   __device__ __forceinline__ explicit Running(float c_) : c(c_), ms{-INFINITY, 0.f}, ref(-INFINITY), plain(false) {}
   __device__ __forceinline__ void grow(float m) {
-    ms.s *= ex2(rescale(ms.m, m, c));  // 0 * 2^-inf = 0 for the first
+    ms.s = __fmul_rn(ms.s, ex2(rescale(ms.m, m, c)));  // 0 * 2^-inf = 0 for the first
     ms.m = m;
-    ref = m * c;
-    plain = fabsf(ref) < INFINITY;
+    ref = offset_of(m, c);
+    plain = fabsf(ref) < kPlain;
   }
   __device__ __forceinline__ void add1(float x) {
-    ms = merge(ms, one_value(x), c);
-    ref = ms.m * c;
-    plain = fabsf(ref) < INFINITY;
+    ms = merge(ms, one_value(x, c), c);
+    ref = offset_of(ms.m, c);
+    plain = fabsf(ref) < kPlain;
   }
   template <int V>
   static __device__ __forceinline__ float max_of(const Vec16<T> (&x)[V]) {
@@ -329,10 +347,12 @@ struct Running {
     } else {
       // nothing above -inf yet (or only NaN): relative to 0, so that -inf gives 0 and NaN stays
       const float m = ms.m == -INFINITY ? 0.f : ms.m;
+      float sum[4] = {ms.s, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int j = 0; j < E; ++j) ms.s += ex2((x[v].get(j) - m) * c);
+        for (int j = 0; j < E; ++j) sum[j % 4] += ex2((x[v].get(j) - m) * c);
+      ms.s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
   }
   // vectors first, first + step, ... of src[0 .. n)
@@ -360,17 +380,17 @@ struct Prob {
   float c, m, l2s, ref;
   bool plain;
   __device__ __forceinline__ Prob(float c_, float m_, float l2s_)
-      : c(c_), m(m_), l2s(l2s_), ref(m_ * c_), plain(fabsf(m_ * c_) < INFINITY) {}
+      : c(c_), m(m_), l2s(l2s_), ref(offset_of(m_, c_)), plain(fabsf(ref) < kPlain) {}
   __device__ __forceinline__ float log2q(float z) const {
-    return (plain ? fmaf(z, c, -ref) : (z - m) * c) - l2s;
+    return plain ? fmaf(z, c, -ref) - l2s : fmaf(z - m, c, -l2s);
   }
   __device__ __forceinline__ float operator()(float z) const {
     if (plain) return fast(z);
     return ex2(log2q(z));
   }
   // `plain` rows.  bf16 results round at 2^-8: the two offsets are added up first
-  // (an error of 2^-24 of their size); fp32 keeps z c - R exact where it matters,
-  // near the top.
+  // (an error of 2^-24 of their size, see kPlain); fp32 keeps z c - R exact where it
+  // matters, near the top.
   __device__ __forceinline__ float fast(float z) const {
     if constexpr (sizeof(T) == 2) return ex2(fmaf(z, c, -(ref + l2s)));
     else return ex2(fmaf(z, c, -ref) - l2s);
@@ -586,9 +606,8 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
         if (id < 0 || p == 0.f) continue;
         const long long at = r * a.ldt + k;
         const float tv = a.t_f32 ? static_cast<const float*>(a.t)[at] : bf2f(static_cast<const uint16_t*>(a.t)[at]);
-        const float logp = (tv - tch.m) * inv_tau - ln_mass;
-        const float logq = qs.log2q(load1(row + id)) * kLn2;
-        sum += p * (logp - logq);
+        const float logp = fmaf(tv - tch.m, inv_tau, -ln_mass);
+        sum = fmaf(p, fmaf(-kLn2, qs.log2q(load1(row + id)), logp), sum);
       }
       loss = block_reduce<THREADS>(sum, scratch[0], [](float x, float y) { return x + y; }) * a.tau * a.tau;
       if (tch.bad) loss = __int_as_float(0x7fc00000);
@@ -869,7 +888,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
           if (ids[k] < lo || ids[k] >= hi || pk == 0.f) continue;
           const float z = slice_logit<T>(slice, meta, parts, v0, ids[k]);
           // a closed entry makes the loss infinite, also in a slice of nothing else
-          side += z == -INFINITY ? INFINITY : pk * (logf(pk) - (z - top) * inv_tau);
+          side = z == -INFINITY ? INFINITY : fmaf(pk, fmaf(top - z, inv_tau, logf(pk)), side);
           P += pk;
         }
         side = warp_reduce(side, [](float x, float y) { return x + y; });
@@ -899,7 +918,8 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       if (rank == 0 && warp == 0) {
         // lane j: slice j
         float part_loss = 0.f;
-        if (lane < cluster) part_loss = P == 0.f ? side : side - P * Prob<T>(c, ms.m, l2s).log2q(parts_m) * kLn2;
+        if (lane < cluster)
+          part_loss = P == 0.f ? side : fmaf(-P * kLn2, Prob<T>(c, ms.m, l2s).log2q(parts_m), side);
 #pragma unroll
         for (int o = kMaxCluster / 2; o; o >>= 1) part_loss += __shfl_xor_sync(0xffffffffu, part_loss, o);
         side = part_loss;

@@ -304,3 +304,26 @@ def test_closed_slices(dev, N, V, dtype):
     w[9:11] = 0
     loss, _ = check(z, t, ids, 2.0, w, "mean", dev)
     assert loss.item() == math.inf
+
+
+@pytest.mark.parametrize("N,V", [(12, 2051), (900, 9001), (460, 40001)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.05])
+def test_logits_far_from_zero(dev, N, V, dtype, tau):
+    # a row's loss and gradient depend on its logits' differences alone, wherever the row lies
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(N, V, generator=g) * 3
+    for r, at in enumerate([100.0, 500.0, 1000.0, 5000.0, 2.0 ** 20, -2.0 ** 20, 2.0 ** 30, 2.0 ** 100, -2.0 ** 126]):
+        # steps that the type still tells apart: an eighth (bf16) of `at` is many
+        z[r] = at * (1 + (z[r] / 3).clamp(-4, 4).round() * 2.0 ** (-7 if dtype == torch.bfloat16 else -22))
+    z[9] = torch.finfo(dtype).min                # all of the row at the type's lowest value: uniform
+    z[10], z[10, 7:9] = torch.finfo(dtype).min, 2.0
+    z = z.to(dtype)
+    ids = torch.randint(0, V // 8, (N, 4), generator=g) + torch.arange(4) * (V // 4)
+    t = torch.randn(N, 4, generator=g)
+    t[10] = -math.inf
+    loss, dz = check(z, t, ids, tau, None, "none", dev)
+    assert loss[9].isfinite() and dz[:11].isfinite().all()
+    w = torch.ones(N)
+    w[4:9] = 0
+    check(z, t, ids, tau, w, "sum", dev, upstream=torch.tensor(0.7))
