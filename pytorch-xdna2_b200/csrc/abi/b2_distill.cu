@@ -384,6 +384,12 @@ struct Prob {
   __device__ __forceinline__ float log2q(float z) const {
     return plain ? fmaf(z, c, -ref) - l2s : fmaf(z - m, c, -l2s);
   }
+  // tau log q.  A finite logit whose z c leaves fp32's range (one masked with the
+  // type's lowest value) has a finite one all the same: by z - m itself.
+  __device__ __forceinline__ float tau_logq(float z, float tau) const {
+    const float l = log2q(z), t = tau * kLn2;
+    return l == -INFINITY && z > -INFINITY ? fmaf(-t, l2s, z - m) : __fmul_rn(t, l);
+  }
   __device__ __forceinline__ float operator()(float z) const {
     if (plain) return fast(z);
     return ex2(log2q(z));
@@ -595,8 +601,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
     }
     const float l2s = log2f(ms.s);
     if (rank == 0) {
-      // the loss: sum over entries of p (log p - log q), in entry order per thread
-      const float inv_tau = 1.f / a.tau;
+      // the loss: sum over entries of p tau (log p - log q), in entry order per thread; times tau at the end
       const float ln_mass = logf(tch.mass);
       const Prob<T> qs(c, ms.m, l2s);
       float sum = 0.f;
@@ -606,10 +611,10 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
         if (id < 0 || p == 0.f) continue;
         const long long at = r * a.ldt + k;
         const float tv = a.t_f32 ? static_cast<const float*>(a.t)[at] : bf2f(static_cast<const uint16_t*>(a.t)[at]);
-        const float logp = fmaf(tv - tch.m, inv_tau, -ln_mass);
-        sum = fmaf(p, fmaf(-kLn2, qs.log2q(load1(row + id)), logp), sum);
+        const float tau_logp = fmaf(-a.tau, ln_mass, tv - tch.m);
+        sum = fmaf(p, tau_logp - qs.tau_logq(load1(row + id), a.tau), sum);
       }
-      loss = block_reduce<THREADS>(sum, scratch[0], [](float x, float y) { return x + y; }) * a.tau * a.tau;
+      loss = block_reduce<THREADS>(sum, scratch[0], [](float x, float y) { return x + y; }) * a.tau;
       if (tch.bad) loss = __int_as_float(0x7fc00000);
       if (threadIdx.x == 0) {
         a.stats[2 * r] = ms.m;
@@ -675,9 +680,10 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
 //
 // The loss in parts: with m_j the maximum of slice j, P_j the probability of the
 // entries in it and lse the row's log-sum-exp of z / tau,
-//   sum_k p_k (log p_k - log q_k) = sum_j [ sum_{k in j} p_k (log p_k - (z_k -
-//   m_j) / tau) + P_j (lse - m_j / tau) ]
-// whose slice sums need nothing of the other slices.
+//   sum_k p_k tau (log p_k - log q_k) = sum_j [ sum_{k in j} p_k (tau log p_k -
+//   (z_k - m_j)) + P_j (tau lse - m_j) ]
+// whose slice sums need nothing of the other slices (and whose differences of
+// logits, not divided by tau, are finite where the logits are).
 //
 // 8192 rows of 131072 bf16 logits with 64 entries, a seventh of them masked:
 // 858 us with the gradient (5.0 TB/s of the 6.45 measured), 530 us the loss
@@ -699,7 +705,7 @@ constexpr int kSlots = 2;
 struct RowMeta {
   long long row;
   int skip, bad;
-  float w, side, P, top;  // the slice's part of the loss relative to a logit of `top`, its entries' probability
+  float w, side, P, top;  // the slice's part of the loss over tau, relative to a logit of `top`; its entries' probability
   float head[8], tail[8];
 };
 
@@ -881,14 +887,13 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         }
         top = warp_reduce(top, [](float x, float y) { return fmaxf(x, y); });
         if (!(fabsf(top) < INFINITY)) top = 0.f;
-        const float inv_tau = 1.f / a.tau;
         float side = 0.f, P = 0.f;
         for (int k = lane; k < a.K; k += 32) {
           const float pk = p[k];
           if (ids[k] < lo || ids[k] >= hi || pk == 0.f) continue;
           const float z = slice_logit<T>(slice, meta, parts, v0, ids[k]);
           // a closed entry makes the loss infinite, also in a slice of nothing else
-          side = z == -INFINITY ? INFINITY : fmaf(pk, fmaf(top - z, inv_tau, logf(pk)), side);
+          side = z == -INFINITY ? INFINITY : fmaf(pk, fmaf(a.tau, logf(pk), top - z), side);
           P += pk;
         }
         side = warp_reduce(side, [](float x, float y) { return x + y; });
@@ -919,13 +924,13 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         // lane j: slice j
         float part_loss = 0.f;
         if (lane < cluster)
-          part_loss = P == 0.f ? side : fmaf(-P * kLn2, Prob<T>(c, ms.m, l2s).log2q(parts_m), side);
+          part_loss = P == 0.f ? side : fmaf(-P, Prob<T>(c, ms.m, l2s).tau_logq(parts_m, a.tau), side);
 #pragma unroll
         for (int o = kMaxCluster / 2; o; o >>= 1) part_loss += __shfl_xor_sync(0xffffffffu, part_loss, o);
         side = part_loss;
       }
       if (rank == 0 && tid == 0) {
-        const float loss = mt.bad ? __int_as_float(0x7fc00000) : a.tau * a.tau * side;
+        const float loss = mt.bad ? __int_as_float(0x7fc00000) : a.tau * side;
         a.stats[2 * r] = ms.m;
         a.stats[2 * r + 1] = l2s;
         if (a.reduction == kNone) a.loss[r] = mt.w * loss;
@@ -1004,7 +1009,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       ms = warp_pair<kStreamWarps>({part[flip][lane % kStreamWarps][0], part[flip][lane % kStreamWarps][1]}, c);
       // the entries' part of the loss, now relative to the slice's maximum (in a closed slice it is infinite already)
       float side = mt.side, P = mt.P, slice_m = ms.m;
-      if (P != 0.f && slice_m > -INFINITY) side -= P * (mt.top - slice_m) / a.tau;
+      if (P != 0.f && slice_m > -INFINITY) side = fmaf(P, slice_m - mt.top, side);
       if (cluster > 1) {
         const int at = int(counted % kSlots);
         if (warp == 0 && lane < cluster) {  // one lane per CTA of the cluster

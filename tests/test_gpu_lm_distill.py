@@ -327,3 +327,25 @@ def test_logits_far_from_zero(dev, N, V, dtype, tau):
     w = torch.ones(N)
     w[4:9] = 0
     check(z, t, ids, tau, w, "sum", dev, upstream=torch.tensor(0.7))
+
+
+@pytest.mark.parametrize("N,V", [(12, 2050), (900, 9001), (460, 40001), (250, 131072)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tau", [1.0, 0.5, 2.0])
+def test_entries_masked_with_the_lowest_value(dev, N, V, dtype, tau):
+    # a finite logit, however low, has a finite log-probability (3.4e38 / tau below the others), and the loss
+    # p tau 3.4e38 with the teacher's p of e^-4 / 2 here is well inside fp32's range.  p's exponent is exact but for
+    # c's rounding and the product's (6 * 2^-23), the other five operations round at 2^-24 to 2^-22: inside 2e-6.
+    lowest = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(V)
+    z = (torch.randn(N, V, generator=g) * 3).to(dtype)
+    t = torch.randn(N, 4, generator=g)
+    ids = torch.randint(0, V // 8, (N, 4), generator=g) + torch.arange(4) * (V // 4)
+    rows = torch.arange(2, 10)
+    t[rows] = torch.tensor([0.0, 0.0, -4.0 * tau, -4.0 * tau])
+    z[rows, ids[rows, 3]] = lowest                            # one entry (of row 4: both of the first half)
+    z[3, V // 2 - 16:] = lowest                               # a whole range, two entries in it
+    z[4, :V // 2 + 16], z[4, ids[4, 3]], t[4] = lowest, 0, t[4].flip(0)
+    z[5, 1:], ids[5, 0], t[5, 0] = lowest, 0, 6.0 * tau       # all but the first logit
+    loss, _ = check(z, t, ids, tau, None, "none", dev)
+    assert loss[2:10].isfinite().all() and (loss[2:10] > 1e33).all()
