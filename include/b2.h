@@ -687,6 +687,11 @@ b2_status b2_embedding_bwd(const void* ids, int ids_dtype, int64_t T,
  * gets the gradient for an upstream gradient of 1, in the same pass over the
  * logits.  Workspace: b2_distill_workspace_bytes(N), 16-byte aligned. */
 size_t b2_distill_workspace_bytes(int64_t N);
+/* How long the forward's kernels wait for their own copies and for the other
+ * CTAs of their cluster before they give up: the rows without a result get a
+ * loss of NaN, B2_ERR_TIMEOUT goes to the device status word and the kernel
+ * ends.  0: the library's limit of 20 s; a shorter one is for tests. */
+b2_status b2_distill_set_wait_limit(int64_t ns);
 b2_status b2_distill_loss_fwd(const void* z, int64_t ldz, int dtype, int64_t N,
                               int64_t V, const void* t, int64_t ldt,
                               int t_dtype, const void* ids, int64_t ldi,

@@ -35,6 +35,7 @@
 // gradient again from the logits and the row's statistics, so that each
 // element is rounded once whatever the factor.
 #include <algorithm>
+#include <atomic>
 
 #include "b2_common.cuh"
 
@@ -82,6 +83,7 @@ struct Args {
   long long slice;        // 16-byte vectors per CTA of the cluster
   long long tile;         // 16-byte vectors held in shared memory at once
   int* status;
+  unsigned long long wait_ns;  // limit of a wait
 };
 
 // 2^x by the hardware's approximation (relative error about 2^-22, results
@@ -175,6 +177,58 @@ __device__ __forceinline__ MaxSum warp_pair(MaxSum v, float c) {
 // One value: 2^(x c - R) if it is the maximum, NaN if it is +inf (inf - inf)
 __device__ __forceinline__ MaxSum one_value(float x, float c) {
   return {x, x == INFINITY ? __int_as_float(0x7fc00000) : ex2(left_of(x, c))};
+}
+
+// Waits of a warp (all lanes call and get the same answer): parked by the
+// hardware (a hint of 1 ms a try) instead of polling, since the pollers of one CTA
+// would take the issue slots of the others on the SM; polling where the limit is
+// shorter than that, since the hardware parks for longer than a short hint.  False,
+// with B2_ERR_TIMEOUT recorded, after `limit` ns, or when another warp of the CTA
+// has given up (*gave_up, if there is one).  CLUSTER: the phase is completed by
+// other CTAs' arrivals, whose stores become visible.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity, int* status, volatile int* gave_up,
+                                                 unsigned long long limit) {
+  constexpr uint32_t kHint = 1000000;
+  unsigned long long t0 = 0;
+  bool done = false;
+  for (;;) {
+    uint32_t ok;
+    if (limit < kHint)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity)
+          : "memory");
+    else if constexpr (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(kHint)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(kHint)
+          : "memory");
+    done = ok != 0;
+    if (done || (gave_up && *gave_up)) break;
+    const unsigned long long t = globaltimer();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > limit) {
+      record_status(status, B2_ERR_TIMEOUT);
+      if (gave_up) *gave_up = 1;
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, done);
 }
 
 template <typename F>
@@ -719,42 +773,20 @@ __device__ __forceinline__ float slice_logit(const uint4* slice, const RowMeta& 
                          : load1(reinterpret_cast<const T*>(slice) + (id - parts.head - v0 * Vec16<T>::N));
 }
 
-// Waits of the persistent kernel: the thread is parked by the hardware (a hint
-// of 1 ms a try) instead of polling, since the pollers of one CTA would take the
-// issue slots of the others on the SM.  Same limit as mbar_wait.  CLUSTER: the
-// phase is completed by other CTAs' arrivals, whose stores become visible.
-template <bool CLUSTER>
-__device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity, int* status) {
-  const uint32_t hint = 1000000;
-  unsigned long long t0 = 0;
-  for (;;) {
-    uint32_t ok;
-    if constexpr (CLUSTER)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity), "r"(hint)
-          : "memory");
-    else
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity), "r"(hint)
-          : "memory");
-    if (ok) return true;
-    const unsigned long long t = globaltimer();
-    if (t0 == 0) t0 = t;
-    if (t - t0 > kWaitLimitNs) {
-      record_status(status, B2_ERR_TIMEOUT);
-      return false;
-    }
-  }
+// A barrier of the compute warps that is a vote: true if none of them has given up.
+__device__ __forceinline__ bool compute_all(bool ok) {
+  uint32_t all;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(uint32_t(ok))
+      : "memory");
+  return all != 0;
 }
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_kernel(const Args a, int cluster) {
@@ -766,6 +798,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
   __shared__ float part[2][kStreamWarps][2];
   __shared__ float final_part[kStreamWarps];
   __shared__ int last_row;
+  __shared__ int gave_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = int(threadIdx.x);
   const int rank = cluster > 1 ? int(cluster_ctarank()) : 0;
   const long long first = blockIdx.x / cluster, step = gridDim.x / cluster;
@@ -774,7 +807,11 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
   float* top_p = reinterpret_cast<float*>(held + a.slice);
   const int Kp = padded_top(a.K);
   int* top_id = reinterpret_cast<int*>(top_p + 2 * Kp);  // two rows' entries
+  const auto wait_for = [&](uint64_t& bar, uint32_t parity) {
+    return mbar_wait_parked<false>(smem_u32(&bar), parity, a.status, &gave_up, a.wait_ns);
+  };
   if (tid == 0) {
+    gave_up = 0;
     mbar_init(smem_u32(&full), 1);
     mbar_init(smem_u32(&top_full), 1);
     mbar_init(smem_u32(&empty), kStreamWarps);
@@ -827,15 +864,13 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       h.skip = !(h.m > -INFINITY || nan || h.bad);
       return h;
     };
-    long long n = 0;
+    long long n = 0, started = 0;  // rows whose slice is on its way or here
     Ahead next{};
     if (first < a.N) next = look(first, 0);
     for (long long r = first; r < a.N; r += step, ++n) {
       const int top_at = int(n & 1);
       const Ahead h = next;
-      bool ok = true;
-      if (n > 0) ok = mbar_wait_parked<false>(smem_u32(&empty), uint32_t((n - 1) & 1), a.status);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (n > 0 && !wait_for(empty, uint32_t((n - 1) & 1))) break;
       const T* row = static_cast<const T*>(a.z) + r * a.ldz;
       const RowParts<T> parts(row, a.V);
       const long long v0 = min(parts.vecs, a.slice * rank), v1 = min(parts.vecs, v0 + a.slice);
@@ -861,6 +896,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         }
         if (h.bad && rank == 0) record_status(a.status, B2_ERR_INVALID);
       }
+      started = n + 1;
       if (!h.skip) {
         float* p = top_p + top_at * Kp;
         float s = 0.f;
@@ -877,7 +913,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
         const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
         const uint4* slice = held;
-        mbar_wait_parked<false>(smem_u32(&full), uint32_t(n & 1), a.status);
+        if (!wait_for(full, uint32_t(n & 1))) break;
         float top = -INFINITY;
         for (int k = lane; k < a.K; k += 32) {
           const float pk = p[k] * inv;
@@ -908,14 +944,14 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       if (lane == 0) mbar_arrive(smem_u32(&top_full));
       if (r + step < a.N) next = look(r + step, int((n + 1) & 1));
     }
-    // every copy lands before the CTA goes away (also if the others gave up)
-    if (n > 0) mbar_wait_parked<false>(smem_u32(&full), uint32_t((n - 1) & 1), a.status);
+    // every copy lands before the CTA goes away, also if someone gave up
+    if (started > 0)
+      mbar_wait_parked<false>(smem_u32(&full), uint32_t((started - 1) & 1), a.status, nullptr, kWaitLimitNs);
   } else {
     // ------------------------------ the compute warps -----------------------
     long long counted = 0;  // rows with statistics
     int flip = 0;
-    bool ok = true;
-    // Statistics of the row in buffer b, its loss, its gradient; frees the buffer.
+    // Statistics of the held row, its loss, its gradient; frees the buffer.  False: a warp gave up.
     auto finish = [&](long long n, MaxSum ms, float parts_m, float side, float P) {
       const RowMeta& mt = meta;
       const long long r = mt.row;
@@ -950,7 +986,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         const long long tail0 = parts.head + parts.vecs * E;
         if (rank == 0 && tid < parts.head) store1(out + tid, f * q(mt.head[tid]));
         if (rank == cluster - 1 && tid < parts.tail) store1(out + tail0 + tid, f * q(mt.tail[tid]));
-        compute_sync();  // the entries' elements are written again, from both terms
+        if (!compute_all(true)) return false;  // the entries' elements are written again, from both terms
         const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
         const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
         const int top_at = int(n & 1);
@@ -963,10 +999,15 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty));
+      return true;
     };
-    long long n = 0;
-    for (long long r = first; r < a.N && ok; r += step, ++n) {
-      ok = mbar_wait_parked<false>(smem_u32(&full), uint32_t(n & 1), a.status);
+    // Leaving early: a warp whose wait ran out goes to the vote behind the loop and
+    // meets the others at their next one (in the loop or behind it), where all of
+    // them learn of it and leave.  So every warp comes to the same number of votes.
+    bool ok = true, all = true;  // this warp's waits were well; every warp's, by the last vote
+    long long n = 0, r = first;
+    for (; r < a.N; r += step, ++n) {
+      ok = wait_for(full, uint32_t(n & 1));
       if (!ok) break;
       const RowMeta& mt = meta;
       const T* row = static_cast<const T*>(a.z) + r * a.ldz;
@@ -1004,8 +1045,9 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         part[flip][warp][0] = ms.m;
         part[flip][warp][1] = ms.s;
       }
-      ok = mbar_wait_parked<false>(smem_u32(&top_full), uint32_t(n & 1), a.status);
-      compute_sync();
+      ok = wait_for(top_full, uint32_t(n & 1));
+      all = compute_all(ok);
+      if (!all) break;
       ms = warp_pair<kStreamWarps>({part[flip][lane % kStreamWarps][0], part[flip][lane % kStreamWarps][1]}, c);
       // the entries' part of the loss, now relative to the slice's maximum (in a closed slice it is infinite already)
       float side = mt.side, P = mt.P, slice_m = ms.m;
@@ -1020,8 +1062,8 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
           mbar_arrive_remote(mapa_shared(smem_u32(&slot_bar[at]), uint32_t(lane)));
         }
         __syncwarp();
-        ok = mbar_wait_parked<true>(smem_u32(&slot_bar[at]), uint32_t(counted / kSlots) & 1u, a.status) && ok;
-        ok = __all_sync(0xffffffffu, ok);
+        ok = mbar_wait_parked<true>(smem_u32(&slot_bar[at]), uint32_t(counted / kSlots) & 1u, a.status, &gave_up,
+                                    a.wait_ns);
         if (!ok) break;
         float4 of{-INFINITY, 0.f, 0.f, 0.f};
         if (lane % kMaxCluster < cluster) of = slot[at][lane % kMaxCluster];
@@ -1031,8 +1073,12 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         P = of.w;
         ++counted;
       }
-      finish(n, ms, slice_m, side, P);
+      all = finish(n, ms, slice_m, side, P);
+      if (!all) break;
     }
+    if (all) all = compute_all(ok);
+    if (!all && rank == 0 && tid == 0)  // rows without a loss
+      for (float* to = a.reduction == kNone ? a.loss : a.row_loss; r < a.N; r += step) to[r] = __int_as_float(0x7fc00000);
   }
   __syncwarp();
   if (cluster > 1) cluster_sync();  // no CTA leaves while another may still write its slots
@@ -1142,6 +1188,9 @@ constexpr size_t kTopBytes = size_t(kMaxTop) * 8;
 constexpr size_t kStreamSmem = 73 * 1024;
 // rows that distill_row_kernel takes with kShortThreads threads
 constexpr long long kShortBytes = 48 * 1024;
+
+// b2_distill_set_wait_limit
+std::atomic<unsigned long long> g_wait_ns{kWaitLimitNs};
 
 b2_status check_args(const char* who, const Args& a, int dtype, int t_dtype, int ids_dtype) {
   if (a.N < 0 || a.V < 1 || a.K < 0) return set_error(B2_ERR_INVALID, "%s: bad shape", who);
@@ -1269,6 +1318,12 @@ using namespace b2;
 
 extern "C" {
 
+b2_status b2_distill_set_wait_limit(int64_t ns) {
+  if (ns < 0) return set_error(B2_ERR_INVALID, "b2_distill_set_wait_limit: negative limit");
+  g_wait_ns.store(ns ? (unsigned long long)ns : kWaitLimitNs, std::memory_order_relaxed);
+  return B2_OK;
+}
+
 size_t b2_distill_workspace_bytes(int64_t N) { return N > 0 ? size_t(N) * 4 + 16 : 16; }
 
 b2_status b2_distill_loss_fwd(const void* z, int64_t ldz, int dtype, int64_t N, int64_t V, const void* t, int64_t ldt,
@@ -1310,6 +1365,7 @@ b2_status b2_distill_loss_fwd(const void* z, int64_t ldz, int dtype, int64_t N, 
   a.counter = static_cast<unsigned*>(workspace);
   a.row_loss = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 16);
   a.status = device_status_ptr();
+  a.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   if (reduction != kNone) {
     distill_begin_kernel<<<1, 1024, 0, st>>>(a);
     B2_TRY(check_cuda(cudaGetLastError(), "distill begin launch"));

@@ -122,6 +122,7 @@ SIGNATURES = {
     "b2_embedding_bwd_workspace_bytes": [i64, i64, i64],
     "b2_embedding_bwd": [vp, i32, i64, vp, i64, i32, i64, i64, f32, i64, vp, vp, sz, vp],
     "b2_distill_workspace_bytes": [i64],
+    "b2_distill_set_wait_limit": [i64],
     "b2_distill_loss_fwd": [vp, i64, i32, i64, i64, vp, i64, i32, vp, i64, i32, i64, f32, vp, i32, vp, vp, vp, i64, vp,
                             sz, vp],
     "b2_distill_loss_bwd": [vp, i64, i32, i64, i64, vp, i64, i32, vp, i64, i32, i64, f32, vp, i32, vp, vp, i32, vp, i64,

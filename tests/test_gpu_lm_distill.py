@@ -349,3 +349,30 @@ def test_entries_masked_with_the_lowest_value(dev, N, V, dtype, tau):
     z[5, 1:], ids[5, 0], t[5, 0] = lowest, 0, 6.0 * tau       # all but the first logit
     loss, _ = check(z, t, ids, tau, None, "none", dev)
     assert loss[2:10].isfinite().all() and (loss[2:10] > 1e33).all()
+
+
+@pytest.fixture
+def short_waits():
+    # restored whatever happens
+    _abi.call("b2_distill_set_wait_limit", 1)
+    yield
+    _abi.call("b2_distill_set_wait_limit", 0)
+
+
+@pytest.mark.parametrize("N,V", [(900, 32768), (460, 40001), (250, 131072), (131, 262139)])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("train", [True, False])
+def test_a_wait_that_runs_out_ends_the_call(dev, short_waits, N, V, reduction, train):
+    # a limit below the time of any copy: the waits give up at the first rows, the kernel ends by itself, reports it
+    # and leaves NaN; then the same call without the limit is what it always was
+    xdna_train.device_status(0)
+    z, t, ids, w = make(N, V, 4, torch.bfloat16, 13)
+    w[::3] = 0                                 # masked rows among the others
+    zd = z.to(dev).requires_grad_(train)
+    args = (t.to(dev), ids.to(dev), 1.0, w.to(dev), reduction)
+    loss = lm.distill_loss(zd, *args)
+    assert loss.isnan().any()
+    assert xdna_train.device_status(0) == 4    # B2_ERR_TIMEOUT
+    _abi.call("b2_distill_set_wait_limit", 0)
+    check(z, t, ids, 1.0, w, reduction, dev)
+    assert xdna_train.device_status(0) == 0

@@ -83,3 +83,9 @@ def test_argument_errors_need_no_gpu():
     assert L.b2_distill_loss_fwd(*args) == 5 and b"workspace" in L.b2_last_error()
     assert L.b2_distill_loss_fwd(*args[:12], -1.0, *args[13:]) == 1 and b"temperature" in L.b2_last_error()
     assert L.b2_distill_loss_fwd(*args[:11], 1025, *args[12:]) == 3 and b"1024" in L.b2_last_error()
+
+
+def test_wait_limit_is_checked():
+    L = _abi.lib()
+    assert L.b2_distill_set_wait_limit(-1) == 1 and b"negative" in L.b2_last_error()
+    assert L.b2_distill_set_wait_limit(0) == 0
