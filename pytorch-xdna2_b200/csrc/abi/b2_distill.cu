@@ -582,8 +582,11 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
         bulk_load_1d(smem_u32(held) + at, src + at, min(16384u, bytes - at), smem_u32(&bar));
     }
   };
+  // false: not in time; the copy has landed all the same before its shared memory
+  // is used again or the CTA leaves
   auto landed = [&] {
-    const bool ok = mbar_wait(smem_u32(&bar), parity, a.status, nullptr);
+    const bool ok = mbar_wait_parked<false>(smem_u32(&bar), parity, a.status, nullptr, a.wait_ns);
+    if (!ok) mbar_wait_parked<false>(smem_u32(&bar), parity, a.status, nullptr, kWaitLimitNs);
     parity ^= 1;
     return ok;
   };
@@ -621,15 +624,17 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
       edge2 = load1(edge_tail);
       run.add1(edge2);
     }
+    bool lost = false;
     for (long long b = v0; b < v1; b += a.tile) {
       if (b > v0) {
         __syncthreads();  // everyone is done with the tile before
         fetch(b);
       }
-      landed();
+      lost |= !landed();
       run.add_slice(held, int(threadIdx.x), int(min(a.tile, v1 - b)), THREADS);
     }
     MaxSum ms = run.ms;
+    if (lost) ms.s = __int_as_float(0x7fc00000);  // a wait ran out: the row's loss and gradient are NaN
     // this CTA's pair
     {
       ms = warp_pair<32>(ms, c);
@@ -680,12 +685,13 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
       const float f = tch.bad ? __int_as_float(0x7fc00000) : w * a.tau;
       const Prob<T> q(c, ms.m, l2s);
       for (long long b = v0; b < v1; b += a.tile) {
+        float fb = f;
         if (!single) {
           __syncthreads();
           fetch(b);
-          landed();
+          if (!landed()) fb = __int_as_float(0x7fc00000);
         }
-        grad_slice<T>(held, out + part.head + b * E, int(threadIdx.x), int(min(a.tile, v1 - b)), THREADS, q, f);
+        grad_slice<T>(held, out + part.head + b * E, int(threadIdx.x), int(min(a.tile, v1 - b)), THREADS, q, fb);
       }
       if (has_head) store1(out + threadIdx.x, f * q(edge));
       if (has_tail) store1(out + part.head + part.vecs * E + threadIdx.x, f * q(edge2));

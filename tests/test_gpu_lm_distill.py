@@ -376,3 +376,25 @@ def test_a_wait_that_runs_out_ends_the_call(dev, short_waits, N, V, reduction, t
     _abi.call("b2_distill_set_wait_limit", 0)
     check(z, t, ids, 1.0, w, reduction, dev)
     assert xdna_train.device_status(0) == 0
+
+
+@pytest.mark.parametrize("N,V", [(4000, 12001), (3, 450002), (20, 900001)])
+@pytest.mark.parametrize("train", [True, False])
+def test_rows_of_a_cluster_whose_wait_runs_out(dev, short_waits, N, V, train):
+    # the kernel with a cluster a row (4000 rows that wait for the memory system; rows of several tiles a CTA, whose
+    # second copy starts right before its wait): such a row's loss and gradient are NaN, and the call without a limit
+    # is right
+    xdna_train.device_status(0)
+    z, t, ids, _ = make(N, V, 4, torch.float32, 14)
+    ids[:, 0], t[:, 0] = 5, 0.0                # every row has an entry
+    zd = z.to(dev).requires_grad_(train)
+    loss = lm.distill_loss(zd, t.to(dev), ids.to(dev), reduction="none")
+    if train:
+        (dz,) = torch.autograd.grad(loss.sum(), [zd])
+    lost = loss.detach().isnan()
+    assert lost.any() and xdna_train.device_status(0) == 4
+    if train:
+        assert dz[lost].isnan().any(1).all()
+    _abi.call("b2_distill_set_wait_limit", 0)
+    check(z, t, ids, 1.0, None, "none", dev)
+    assert xdna_train.device_status(0) == 0
