@@ -68,8 +68,7 @@ class GatedMlp : public torch::autograd::Function<GatedMlp> {
                             const at::Tensor& wu, const at::Tensor& wd, int64_t act) {
     const Call c = check(x, wg, wu, wd);
     at::Tensor kept = empty({c.M, saved_width(c.F)}, at::kBFloat16, x.device().index());
-    ctx->save_for_backward({x, wg, wu, wd});
-    ctx->saved_data["kept"] = kept;
+    ctx->save_for_backward({x, wg, wu, wd, kept});  // released, and seen by hooks, like any saved tensor
     ctx->saved_data["act"] = act;
     return run_fwd(c, x.sizes(), act, kept);
   }
@@ -80,7 +79,7 @@ class GatedMlp : public torch::autograd::Function<GatedMlp> {
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const Call c = check(saved[0], saved[1], saved[2], saved[3]);
-    const at::Tensor kept = ctx->saved_data["kept"].toTensor();
+    const at::Tensor kept = saved[4].contiguous();  // (a hook may have moved it)
     const c10::Device dev = c.x.device();
     c10::cuda::CUDAGuard g(dev.index());
     materialize(grads[0]);

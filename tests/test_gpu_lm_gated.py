@@ -279,3 +279,41 @@ def test_few_tokens_keep_infinities(dev):
     w = torch.full((8, 8), 2.0 ** 8).bfloat16()
     y = lm.gated_mlp(x.to(dev), w.to(dev), w.to(dev), torch.ones(8, 8).bfloat16().to(dev), activation="relu")
     assert (xdna_train.as_cuda(y) == float("inf")).all()
+
+
+def test_kept_tensors_are_autograds(dev):
+    # what the forward keeps is a saved tensor like any other: hooks see it, it can be moved to the host, a checkpoint
+    # makes it again, and it is freed by the backward, not with the graph
+    from torch.utils.checkpoint import checkpoint
+    M, D, F, E = 300, 64, 1000, 72
+    x, wg, wu, wd, dy = (t.to(dev) for t in make(M, D, F, E, 8))
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    seen = []
+
+    def pack(t):
+        seen.append(t.numel())
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = lm.gated_mlp(*leaves)
+    assert max(seen) >= 4 * M * F
+    want = torch.autograd.grad(y, leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        moved = lm.gated_mlp(*leaves)
+    again = checkpoint(lambda *a: lm.gated_mlp(*a), *leaves, use_reentrant=False, preserve_rng_state=False)
+    for other in (moved, again):
+        assert torch.equal(other, y)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(other, leaves, dy), want))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(again, leaves, dy)
+
+
+def test_kept_tensors_are_freed_by_the_backward(dev):
+    M, D, F, E = 1024, 64, 8192, 64
+    x, wg, wu, wd, dy = (t.to(dev) for t in make(M, D, F, E, 9))
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    y = lm.gated_mlp(*leaves)
+    before = xdna_train.allocator_stats()["allocated_bytes"]
+    grads = torch.autograd.grad(y, leaves, dy)          # y and its graph stay in scope
+    held = sum(g.numel() * g.element_size() for g in grads)
+    assert xdna_train.allocator_stats()["allocated_bytes"] <= before + held + (8 << 20) - 8 * M * F
