@@ -112,13 +112,15 @@ def _plain_distill_loss(logits, teacher_logits, teacher_ids, temperature, row_we
     if ids.numel() and int(ids.max()) >= logits.shape[-1]:
         raise IndexError("distill_loss: teacher id outside the vocabulary")
     t = (teacher_logits.detach().float() / temperature).masked_fill(ids < 0, float("-inf"))
-    has = (t > float("-inf")).any(-1, keepdim=True) if t.shape[-1] else t.new_zeros(t.shape[:-1] + (1,), dtype=torch.bool)
+    has = t.new_zeros(t.shape[:-1] + (1,), dtype=torch.bool)
+    if t.shape[-1]:
+        has = (t != float("-inf")).any(-1, keepdim=True)  # (a NaN counts: it is not to go unseen)
     logp = torch.log_softmax(t.masked_fill(~has, 0.0), -1)
     p = torch.where(has, logp.exp(), 0.0)
     active = has if row_weight is None else has & (row_weight != 0).unsqueeze(-1)
     z = logits.float().masked_fill(~active, 0.0) / temperature
     logq = torch.log_softmax(z, -1).gather(-1, ids.clamp(min=0))
-    keep = (p > 0) & active
+    keep = (p != 0) & active
     rows = temperature ** 2 * torch.where(keep, p * (logp.masked_fill(~keep, 0.0) - torch.where(keep, logq, 0.0)),
                                           0.0).sum(-1)
     w = torch.ones_like(rows) if row_weight is None else row_weight

@@ -89,3 +89,15 @@ def test_wait_limit_is_checked():
     L = _abi.lib()
     assert L.b2_distill_set_wait_limit(-1) == 1 and b"negative" in L.b2_last_error()
     assert L.b2_distill_set_wait_limit(0) == 0
+
+
+def test_distill_loss_keeps_a_teachers_nan_on_cpu():
+    # as on the device: a NaN teacher logit makes its row's loss NaN, unless the entry is absent or the row masked
+    z = torch.randn(4, 6)
+    t = torch.zeros(4, 3)
+    t[:3, 1] = math.nan
+    ids = torch.tensor([[0, 1, 2], [3, -1, 4], [0, 1, 2], [0, 1, 2]])
+    loss = lm.distill_loss(z, t, ids, row_weight=torch.tensor([1.0, 1.0, 0.0, 1.0]), reduction="none")
+    assert loss.isnan().tolist() == [True, False, False, False] and loss[2] == 0
+    t[0] = math.nan
+    assert lm.distill_loss(z, t, ids, reduction="none").isnan().tolist() == [True, False, True, False]
