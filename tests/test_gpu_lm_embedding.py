@@ -176,3 +176,22 @@ def test_plain_path_in_mode_0(dev):
     finally:
         xdna_train.set_npu_mode(2)
     assert torch.equal(native.cpu(), plain.cpu())
+
+
+@pytest.mark.parametrize("T,V,D", [(33, 40, 33), (512, 300, 40), (513, 300, 40), (3001, 5000, 129), (4096, 700, 12),
+                                   (4097, 3000, 40), (20011, 100, 18), (65536, 90000, 72), (262145, 50000, 8),
+                                   (300000, 50000, 4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["uniform", "zipf", "one", "falling"])
+def test_sums_of_whole_numbers_are_exact(dev, T, V, D, dtype, kind):
+    # whole numbers below 8: fp32 holds every partial sum (at most 7 * 300000 < 2^24) in any order, so that a token
+    # lost, counted twice or added to another row shows at any count; the result is rounded once
+    g = torch.Generator().manual_seed(T + D)
+    ids = _ids(kind, T, V, g)
+    pad = V - 1 if kind == "zipf" else None
+    dy = torch.randint(-7, 8, (T, D), generator=g).to(dtype)
+    w = torch.zeros(V, D, dtype=dtype, device=dev, requires_grad=True)
+    (dw,) = torch.autograd.grad(lm.embedding(ids.to(dev), w, padding_idx=pad), [w], dy.to(dev))
+    keep = torch.ones(T, dtype=torch.bool) if pad is None else ids != pad
+    ref = torch.zeros(V, D, dtype=torch.float64).index_add_(0, ids[keep], dy.double()[keep])
+    assert torch.equal(dw.cpu(), ref.to(dtype))
