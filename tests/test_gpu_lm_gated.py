@@ -317,3 +317,94 @@ def test_kept_tensors_are_freed_by_the_backward(dev):
     grads = torch.autograd.grad(y, leaves, dy)          # y and its graph stay in scope
     held = sum(g.numel() * g.element_size() for g in grads)
     assert xdna_train.allocator_stats()["allocated_bytes"] <= before + held + (8 << 20) - 8 * M * F
+
+
+def _decode(saved, M, F):
+    """h, P = u act'(g) and A = act(g) of the forward's buffer: 16-bit words h, upper half of P, of A, and the next 8
+    bits of both (P's above A's)"""
+    words = saved.view(torch.int16).view(M, 4, -1)[:, :, :F].long() & 0xffff
+    h, p, a, r = words.unbind(1)
+    f32 = lambda bits: (bits - ((bits >> 31) << 32)).int().view(torch.float32).double()  # noqa: E731
+    return f32(h << 16), f32((p << 16) | (r & 0xff00)), f32((a << 16) | ((r & 0xff) << 8))
+
+
+@pytest.mark.parametrize("M,D,F,E", [
+    (1, 256, 688, 64), (3, 64, 104, 40), (16, 512, 1531, 64), (24, 1024, 4096, 64),            # few tokens
+    (64, 1024, 512, 64), (40, 2045, 300, 33), (129, 2048, 333, 64),                            # split reductions
+    (300, 64, 1000, 64), (257, 100, 130, 64), (2048, 128, 1536, 64), (5, 61, 77, 13),          # whole ones
+])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_kept_factors_have_sixteen_bits(cuda, M, D, F, E, act):
+    # truncated to 16 bits of significand: 2^-15 of themselves.  fp32 sums leave 2^-20 of the absolute sums in g and u
+    # (act and act' move by at most 1.2 a unit), the activation's own arithmetic 2^-19.  As bf16 they would be off by
+    # up to 2^-7.
+    x, wg, wu, wd, _ = (t.to(cuda) for t in make(M, D, F, E, 6))
+    L, Fp = _abi.lib(), (F + 7) // 8 * 8
+    y = torch.empty(M, E, dtype=torch.bfloat16, device=cuda)
+    saved = torch.zeros(M * 4 * Fp, dtype=torch.bfloat16, device=cuda)
+    need = L.b2_gated_mlp_fwd_workspace_bytes(M, D, F, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    _abi.call("b2_gated_mlp_fwd_bf16", x.data_ptr(), D, wg.data_ptr(), D, wu.data_ptr(), D, wd.data_ptr(), F,
+              ["silu", "gelu", "relu"].index(act), y.data_ptr(), E, saved.data_ptr(), M, D, F, E, ws.data_ptr(), need,
+              torch.cuda.current_stream().cuda_stream)
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    g, u = x @ wg.t(), x @ wu.t()
+    a = ACT[act](g)
+    sig, pdf = torch.sigmoid(g), torch.exp(-g * g / 2) / (2 * torch.pi) ** 0.5
+    slope = {"silu": sig * (1 + g * (1 - sig)), "gelu": 0.5 * (1 + torch.erf(g / 2 ** 0.5)) + g * pdf,
+             "relu": (g > 0).double()}[act]
+    eg, eu = (2.0 ** -20 * (x.abs() @ w.abs().t()) for w in (wg, wu))
+    h, P, A = _decode(saved, M, F)
+    sure = g.abs() > eg if act == "relu" else torch.ones_like(g, dtype=torch.bool)
+    eP = 1.2 * (u.abs() + eu) * eg + slope.abs() * eu + 2.0 ** -19 * u.abs()
+    assert ((P - u * slope).abs() <= 2.0 ** -15 * (u * slope).abs() + eP)[sure].all()
+    assert ((A - a).abs() <= 2.0 ** -15 * a.abs() + 1.2 * eg + 2.0 ** -19).all()
+    eh = a.abs() * eu + (u.abs() + eu) * (1.2 * eg + 2.0 ** -19)
+    assert ((h - a * u).abs() <= EPS * (a * u).abs() + 1.01 * eh).all()
+
+
+@pytest.mark.parametrize("M,F", [(1, 8), (37, 64), (64, 128), (200, 130), (2048, 1536), (64, 1024), (33, 2061)])
+def test_backward_takes_all_sixteen_bits(cuda, M, F):
+    # x and w_down are unit matrices, so that dh = dy and dw_gate = (dy P)^T, dw_up = (dy A)^T: exact fp32 products of
+    # 8 by 16 bits, rounded once to bf16 -- the same bits as torch's.  Whole and split reductions of dh.
+    g = torch.Generator().manual_seed(M + F)
+    Fp = (F + 7) // 8 * 8
+    dy = torch.randn(M, F, generator=g).bfloat16().to(cuda)
+    factors = (torch.randn(2, M, F, generator=g).to(cuda).view(torch.int32) & -256).view(torch.float32)
+    words = torch.zeros(M, 4, Fp, dtype=torch.int64, device=cuda)
+    bits = factors.view(torch.int32).long() & 0xffffffff
+    words[:, 1:3, :F] = (bits >> 16).transpose(0, 1)
+    words[:, 3, :F] = (bits[0] & 0xff00) | ((bits[1] >> 8) & 0xff)
+    saved = (words - ((words >> 15) << 16)).short().contiguous()
+    x, wd = (torch.eye(n, dtype=torch.bfloat16, device=cuda) for n in (M, F))
+    w = torch.zeros(F, M, dtype=torch.bfloat16, device=cuda)
+    out = [torch.full((F, M), 7.0, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    need = _abi.lib().b2_gated_mlp_bwd_workspace_bytes(M, M, F, F)
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    _abi.call("b2_gated_mlp_bwd_bf16", dy.data_ptr(), F, x.data_ptr(), M, w.data_ptr(), M, w.data_ptr(), M,
+              wd.data_ptr(), F, 0, saved.data_ptr(), None, out[0].data_ptr(), out[1].data_ptr(), None, M, M, F, F,
+              ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    for got, factor in zip(out, factors):
+        want = (dy.float() * factor).bfloat16()
+        assert torch.equal(got.t(), want)
+        assert M * F < 64 or not torch.equal((dy.float() * factor.bfloat16().float()).bfloat16(), want)
+
+
+@pytest.mark.parametrize("M,D,F,E", [(16, 512, 1024, 512), (64, 512, 1024, 512), (300, 1001, 1300, 999),
+                                     (1024, 512, 2048, 512)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_two_roundings_and_no_more(dev, M, D, F, E, act):
+    # y and dw_down carry the rounding of h and their own, dx, dw_gate and dw_up that of dg and du and their own.  One
+    # rounding of normally distributed numbers leaves 0.435 eps in the 2-norm (0.39 for significands spread evenly over
+    # their logarithm), two independent ones 0.615; a third, of the factors, would make it 0.75, truncated bf16
+    # factors more than 1.
+    one = torch.randn(1 << 16, generator=torch.Generator().manual_seed(0))
+    assert 0.42 * EPS < (one.bfloat16() - one).norm() / one.norm() < 0.45 * EPS
+    x, wg, wu, wd, dy = make(M, D, F, E, 7)
+    leaves = [t.to(dev).requires_grad_() for t in (x, wg, wu, wd)]
+    y = lm.gated_mlp(*leaves, activation=act)
+    grads = torch.autograd.grad(y, leaves, dy.to(dev))
+    for got, (want, _), what in zip((y, *grads), reference(x, wg, wu, wd, dy, act),
+                                    ("y", "dx", "dw_gate", "dw_up", "dw_down")):
+        err = (xdna_train.as_cuda(got.detach()).double() - want).norm() / want.norm()
+        assert err <= 0.7 * EPS, (what, err.item() / EPS)
