@@ -398,3 +398,24 @@ def test_rows_of_a_cluster_whose_wait_runs_out(dev, short_waits, N, V, train):
     _abi.call("b2_distill_set_wait_limit", 0)
     check(z, t, ids, 1.0, None, "none", dev)
     assert xdna_train.device_status(0) == 0
+
+
+@pytest.mark.parametrize("N,V,K", [(5, 40000, 12), (9, 70001, 33), (3, 131072, 64), (2, 450002, 1024), (700, 33000, 7)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_other_upstream_gradients_of_long_rows(dev, N, V, K, dtype):
+    # rows that the backward takes in several pieces, aligned and not, entries and closed logits in all of them
+    z, t, ids, w = make(N, V, K, dtype, 15)
+    ids[0, :3] = torch.tensor([0, V - 1, V // 2])
+    z[1, V // 3:V // 2] = -math.inf
+    check(z, t, ids, 1.5, w, "mean", dev, upstream=torch.tensor(-0.3))
+    check(z, t, ids, 1.0, None, "sum", dev, upstream=torch.tensor(3.0))
+    up = torch.randn(N, generator=torch.Generator().manual_seed(16))
+    up[0], up[-1] = 1.0, 0.0
+    check(z, t, ids, 1.5, w, "none", dev, upstream=up)
+
+
+@pytest.mark.parametrize("lo,hi", [(1, 60001), (3, 59996), (8, 60008)])
+def test_other_upstream_gradients_of_long_views(dev, lo, hi):
+    z, _, _, _ = make(6, 60015, 1, torch.bfloat16, 17)
+    _, t, ids, w = make(6, hi - lo, 12, torch.bfloat16, 18)
+    check(z, t, ids, 1.0, w, "mean", dev, upstream=torch.tensor(0.5), lo=lo, hi=hi)
