@@ -51,8 +51,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the vocabulary of {weight.shape[0]}")
     C = _native(weight)
     if C is None:
-        y = F.embedding(ids, weight, padding_idx)
-        return y if scale == 1.0 else (y.float() * scale).to(weight.dtype)
+        # through an fp32 table, so that the gradient is summed in fp32 and rounded once
+        table = weight if weight.dtype == torch.float64 else weight.float()
+        return (F.embedding(ids, table, padding_idx) * scale).to(weight.dtype)
     return C.lm_embedding(ids, weight, float(scale), -1 if padding_idx is None else int(padding_idx))
 
 

@@ -101,3 +101,20 @@ def test_distill_loss_keeps_a_teachers_nan_on_cpu():
     assert loss.isnan().tolist() == [True, False, False, False] and loss[2] == 0
     t[0] = math.nan
     assert lm.distill_loss(z, t, ids, reduction="none").isnan().tolist() == [True, False, True, False]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_embedding_sums_in_fp32_on_cpu(dtype):
+    # as on the device: the gradient of a frequent id is rounded once, not after every token (bf16 sums stop at 256)
+    w = torch.randn(4, 3).to(dtype).requires_grad_()
+    ids = torch.tensor([1] * 1000 + [2] * 3 + [0])
+    y = lm.embedding(ids, w, scale=3.0, padding_idx=0)
+    assert y.dtype == dtype and torch.equal(y, (3.0 * w.detach().float()).to(dtype)[ids])
+    (dw,) = torch.autograd.grad(y, [w], torch.ones_like(y))
+    assert dw.dtype == dtype and dw[:, 0].tolist() == [0.0, 3000.0 if dtype == torch.float32 else 3008.0, 9.0, 0.0]
+
+
+def test_embedding_of_doubles_on_cpu():
+    w = torch.randn(5, 3, dtype=torch.float64, requires_grad=True)
+    ids = torch.tensor([4, 0, 4])
+    assert torch.autograd.gradcheck(lambda t: lm.embedding(ids, t, scale=1.7), [w])
