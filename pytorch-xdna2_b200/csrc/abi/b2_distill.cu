@@ -145,15 +145,12 @@ struct MaxSum {
 };
 // R = m c, rounded: never fused into what it is added to
 __device__ __forceinline__ float offset_of(float m, float c) { return __fmul_rn(m, c); }
-// What that rounding left of m c: a sum of the plain form is relative to R, others to m c itself
-__device__ __forceinline__ float left_of(float m, float c) {
-  const float r = offset_of(m, c);
-  return fabsf(r) < kPlain ? fmaf(m, c, -r) : 0.f;
-}
-// log2 of the factor that brings a sum relative to `from` to one relative to `to`
+// log2 of the factor that brings a sum relative to `from` to one relative to `to`.
+// (A sum of the plain form is relative to R, others to m c itself: where they meet,
+// around kPlain, R's rounding of at most 2^-17 stays in the sum.)
 __device__ __forceinline__ float rescale(float from, float to, float c) {
   const float a = offset_of(from, c), b = offset_of(to, c);
-  return fabsf(a) < kPlain && fabsf(b) < kPlain ? a - b : fmaf(from - to, c, left_of(to, c) - left_of(from, c));
+  return fabsf(a) < kPlain && fabsf(b) < kPlain ? a - b : (from - to) * c;
 }
 __device__ __forceinline__ MaxSum merge(MaxSum a, MaxSum b, float c) {
   const float m = fmaxf(a.m, b.m);
@@ -174,61 +171,72 @@ __device__ __forceinline__ MaxSum warp_pair(MaxSum v, float c) {
   for (int o = W / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return {m, s};
 }
-// One value: 2^(x c - R) if it is the maximum, NaN if it is +inf (inf - inf)
-__device__ __forceinline__ MaxSum one_value(float x, float c) {
-  return {x, x == INFINITY ? __int_as_float(0x7fc00000) : ex2(left_of(x, c))};
+// One value: 2^0 of the sum if it is the maximum, NaN if it is +inf (inf - inf)
+__device__ __forceinline__ MaxSum one_value(float x) {
+  return {x, x == INFINITY ? __int_as_float(0x7fc00000) : 1.f};
 }
 
-// Waits of a warp (all lanes call and get the same answer): parked by the
-// hardware (a hint of 1 ms a try) instead of polling, since the pollers of one CTA
-// would take the issue slots of the others on the SM; polling where the limit is
-// shorter than that, since the hardware parks for longer than a short hint.  False,
-// with B2_ERR_TIMEOUT recorded, after `limit` ns, or when another warp of the CTA
-// has given up (*gave_up, if there is one).  CLUSTER: the phase is completed by
-// other CTAs' arrivals, whose stores become visible.
+// One look at a phase: parked by the hardware for up to kParkNs, or (PARK false)
+// not at all.  CLUSTER: the phase is completed by other CTAs' arrivals, whose
+// stores become visible.
+constexpr uint32_t kParkNs = 1000000;
+template <bool CLUSTER, bool PARK>
+__device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  if constexpr (!PARK)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  else if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kParkNs)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kParkNs)
+        : "memory");
+  return ok != 0;
+}
+
+// A wait that the first look did not end: false, with B2_ERR_TIMEOUT recorded,
+// after `limit` ns, or when another warp of the CTA has given up (*gave_up, if
+// there is one).  Out of line: it is rare, and in every wait its code cost 1 %.
+template <bool CLUSTER>
+__device__ __noinline__ bool mbar_wait_on(uint32_t bar, uint32_t parity, int* status, volatile int* gave_up,
+                                          unsigned long long limit) {
+  const unsigned long long t0 = globaltimer();
+  for (;;) {
+    if (limit < kParkNs ? mbar_look<CLUSTER, false>(bar, parity) : mbar_look<CLUSTER, true>(bar, parity)) return true;
+    if (gave_up && *gave_up) return false;
+    if (globaltimer() - t0 > limit) {
+      record_status(status, B2_ERR_TIMEOUT);
+      if (gave_up) *gave_up = 1;
+      return false;
+    }
+  }
+}
+
+// Waits of the persistent kernel's warps (all lanes call and get the same answer):
+// parked instead of polling, since the pollers of one CTA would take the issue
+// slots of the others on the SM (limits too short for that are polled).
 template <bool CLUSTER>
 __device__ __forceinline__ bool mbar_wait_parked(uint32_t bar, uint32_t parity, int* status, volatile int* gave_up,
                                                  unsigned long long limit) {
-  constexpr uint32_t kHint = 1000000;
-  unsigned long long t0 = 0;
-  bool done = false;
-  for (;;) {
-    uint32_t ok;
-    if (limit < kHint)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity)
-          : "memory");
-    else if constexpr (CLUSTER)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity), "r"(kHint)
-          : "memory");
-    else
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(ok)
-          : "r"(bar), "r"(parity), "r"(kHint)
-          : "memory");
-    done = ok != 0;
-    if (done || (gave_up && *gave_up)) break;
-    const unsigned long long t = globaltimer();
-    if (t0 == 0) t0 = t;
-    if (t - t0 > limit) {
-      record_status(status, B2_ERR_TIMEOUT);
-      if (gave_up) *gave_up = 1;
-      break;
-    }
-  }
-  return __all_sync(0xffffffffu, done);
+  bool ok = limit >= kParkNs && mbar_look<CLUSTER, true>(bar, parity);
+  if (!ok) ok = mbar_wait_on<CLUSTER>(bar, parity, status, gave_up, limit);
+  return __all_sync(0xffffffffu, ok);
 }
 
 template <typename F>
@@ -360,7 +368,7 @@ struct Running {
     plain = fabsf(ref) < kPlain;
   }
   __device__ __forceinline__ void add1(float x) {
-    ms = merge(ms, one_value(x, c), c);
+    ms = merge(ms, one_value(x), c);
     ref = offset_of(ms.m, c);
     plain = fabsf(ref) < kPlain;
   }
@@ -585,8 +593,9 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
   // false: not in time; the copy has landed all the same before its shared memory
   // is used again or the CTA leaves
   auto landed = [&] {
-    const bool ok = mbar_wait_parked<false>(smem_u32(&bar), parity, a.status, nullptr, a.wait_ns);
-    if (!ok) mbar_wait_parked<false>(smem_u32(&bar), parity, a.status, nullptr, kWaitLimitNs);
+    const bool ok = mbar_look<false, false>(smem_u32(&bar), parity) ||
+                    mbar_wait_on<false>(smem_u32(&bar), parity, a.status, nullptr, a.wait_ns);
+    if (!ok) mbar_wait_on<false>(smem_u32(&bar), parity, a.status, nullptr, kWaitLimitNs);
     parity ^= 1;
     return ok;
   };
@@ -779,7 +788,8 @@ __device__ __forceinline__ float slice_logit(const uint4* slice, const RowMeta& 
                          : load1(reinterpret_cast<const T*>(slice) + (id - parts.head - v0 * Vec16<T>::N));
 }
 
-// A barrier of the compute warps that is a vote: true if none of them has given up.
+// Barriers of the compute warps; the second is a vote: true if none of them has given up.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool compute_all(bool ok) {
   uint32_t all;
   __syncwarp();
@@ -957,7 +967,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
     // ------------------------------ the compute warps -----------------------
     long long counted = 0;  // rows with statistics
     int flip = 0;
-    // Statistics of the held row, its loss, its gradient; frees the buffer.  False: a warp gave up.
+    // Statistics of the held row, its loss, its gradient; frees the buffer.
     auto finish = [&](long long n, MaxSum ms, float parts_m, float side, float P) {
       const RowMeta& mt = meta;
       const long long r = mt.row;
@@ -992,7 +1002,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         const long long tail0 = parts.head + parts.vecs * E;
         if (rank == 0 && tid < parts.head) store1(out + tid, f * q(mt.head[tid]));
         if (rank == cluster - 1 && tid < parts.tail) store1(out + tail0 + tid, f * q(mt.tail[tid]));
-        if (!compute_all(true)) return false;  // the entries' elements are written again, from both terms
+        compute_sync();  // the entries' elements are written again, from both terms
         const long long lo = rank == 0 ? 0 : parts.head + v0 * E;
         const long long hi = rank == cluster - 1 ? a.V : parts.head + v1 * E;
         const int top_at = int(n & 1);
@@ -1005,11 +1015,11 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&empty));
-      return true;
     };
     // Leaving early: a warp whose wait ran out goes to the vote behind the loop and
     // meets the others at their next one (in the loop or behind it), where all of
-    // them learn of it and leave.  So every warp comes to the same number of votes.
+    // them learn of it and leave.  So every warp comes to the same number of votes
+    // (and of finish's barriers: one for every row whose vote passed).
     bool ok = true, all = true;  // this warp's waits were well; every warp's, by the last vote
     long long n = 0, r = first;
     for (; r < a.N; r += step, ++n) {
@@ -1070,7 +1080,10 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         __syncwarp();
         ok = mbar_wait_parked<true>(smem_u32(&slot_bar[at]), uint32_t(counted / kSlots) & 1u, a.status, &gave_up,
                                     a.wait_ns);
-        if (!ok) break;
+        if (!ok) {
+          if constexpr (GRAD) compute_sync();  // finish's
+          break;
+        }
         float4 of{-INFINITY, 0.f, 0.f, 0.f};
         if (lane % kMaxCluster < cluster) of = slot[at][lane % kMaxCluster];
         ms = warp_pair<kMaxCluster>({of.x, of.y}, c);
@@ -1079,8 +1092,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamPerSm) distill_stream_k
         P = of.w;
         ++counted;
       }
-      all = finish(n, ms, slice_m, side, P);
-      if (!all) break;
+      finish(n, ms, slice_m, side, P);
     }
     if (all) all = compute_all(ok);
     if (!all && rank == 0 && tid == 0)  // rows without a loss
