@@ -216,11 +216,13 @@ __device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
 template <bool CLUSTER>
 __device__ __noinline__ bool mbar_wait_on(uint32_t bar, uint32_t parity, int* status, volatile int* gave_up,
                                           unsigned long long limit) {
-  const unsigned long long t0 = globaltimer();
+  unsigned long long t0 = 0;
   for (;;) {
     if (limit < kParkNs ? mbar_look<CLUSTER, false>(bar, parity) : mbar_look<CLUSTER, true>(bar, parity)) return true;
     if (gave_up && *gave_up) return false;
-    if (globaltimer() - t0 > limit) {
+    const unsigned long long t = globaltimer();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > limit) {
       record_status(status, B2_ERR_TIMEOUT);
       if (gave_up) *gave_up = 1;
       return false;
@@ -593,7 +595,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
   // false: not in time; the copy has landed all the same before its shared memory
   // is used again or the CTA leaves
   auto landed = [&] {
-    const bool ok = mbar_look<false, false>(smem_u32(&bar), parity) ||
+    const bool ok = (a.wait_ns >= kParkNs && mbar_try_wait(smem_u32(&bar), parity)) ||
                     mbar_wait_on<false>(smem_u32(&bar), parity, a.status, nullptr, a.wait_ns);
     if (!ok) mbar_wait_on<false>(smem_u32(&bar), parity, a.status, nullptr, kWaitLimitNs);
     parity ^= 1;
