@@ -72,8 +72,9 @@ __device__ __forceinline__ long long load_id(const void* ids, int is64, long lon
 // CTA, U rows' loads in flight per thread.  An id outside [0, V) gives a row of
 // NaN and B2_ERR_INVALID in the device status word; nothing out of range is read.
 // Bound by HBM: 65536 tokens of 131072 x 2048 bf16 rows 76 us (one row in flight a
-// thread 87, eight 76), 0.54 GB with repeated rows; few tokens by latency, so
-// their columns are spread over CTAs.
+// thread 87, eight 76), 0.54 GB with repeated rows; few tokens by latency (16 rows
+// of 1024 bf16 in two CTAs 4 us), and where a row has more than 256 vectors their
+// columns are spread over CTAs.
 // ---------------------------------------------------------------------------
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(256) embed_fwd_kernel(const void* __restrict__ ids, int is64, long long tokens,
@@ -744,8 +745,14 @@ b2_status run_fwd(const void* ids, int is64, int64_t tokens, const void* w, int6
   const int ll = log_lanes_for(vecs);
   const int rows = (256 >> ll) * U;
   const int64_t bx = (tokens + rows - 1) / rows;
-  // few tokens: spread the columns over CTAs instead
-  const int by = bx >= 148 ? 1 : std::max(1, std::min((vecs + (1 << ll) - 1) >> ll, 64));
+  // long rows of too few tokens for every SM: their columns over CTAs
+  const int slabs = (vecs + (1 << ll) - 1) >> ll;
+  int by = 1;
+  if (slabs > 1) {
+    int dev = 0;
+    B2_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+    if (bx < sm_count(dev)) by = std::min(slabs, 64);
+  }
   if (bx > INT32_MAX) return set_error(B2_ERR_UNSUPPORTED, "b2_embedding_fwd: too many tokens");
   embed_fwd_kernel<T, N, U><<<dim3(unsigned(bx), unsigned(by)), 256, 0, st>>>(
       ids, is64, tokens, static_cast<const T*>(w), ldw, V, vecs, ll, scale, static_cast<T*>(y), D,

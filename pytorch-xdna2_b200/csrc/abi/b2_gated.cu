@@ -137,8 +137,8 @@ struct Config {
   static constexpr int kBHalf = PBN / 2;
   static constexpr int kStage = kABytes + kBHalf * BK * 2;
   // per epilogue warp: kStore two 32 x 64 boxes, kGate four 32 x 32 boxes, kGateBwd triples of 32 x 32 boxes.
-  // Of these one beside a fifth stage at PBN 256 (dh of 8192 tokens, 4096 x 12288: 700 us, 750 with two triples and
-  // four stages, 886 with three), two at 128 (512 tokens, 1024 x 4096: 13.3 us, 13.8 with one).
+  // Of these one beside a fifth stage at PBN 256 (dh of 8192 tokens, 4096 x 12288, in passes under the power cap: 700
+  // us, 750 with two triples and four stages, 886 with three), two at 128 (512 tokens, 1024 x 4096: 13.3 us, 13.8 with one).
   static constexpr int kTriples = PBN == 256 ? 1 : 2;
   static constexpr int kEpiBytes = EPI == kGateBwd ? kTriples * 6144 : 2 * 4096;
   static constexpr int kStages = PBN == 256 ? 5 : (EPI == kGateBwd ? 5 : 6);
@@ -205,9 +205,10 @@ __device__ __forceinline__ void store_box_rows(const uint8_t* box, uint16_t* dst
   }
 }
 
-// 8192 tokens, 4096 x 12288: gate 1203 us, down 580, dh 779, dx 1141, the three
-// weight gradients 1899 -- 1.32 PFLOP/s over all five under the power cap (the
-// clock falls with it), 1.45 in runs of a few milliseconds.  512 tokens, 1024 x
+// 8192 tokens, 4096 x 12288, each launch by itself: gate 1130 us, down 531, dh 617,
+// dx 1100, the three weight gradients 1737 -- 1.45 PFLOP/s over all five; in
+// passes one after the other 5.64 ms, 1.32 PFLOP/s, under the power cap (the clock
+// falls with it).  512 tokens, 1024 x
 // 4096, forward and backward 78 us: there each product's launch, first tiles and
 // epilogue (2.5, 2 and 4 us) outweigh its 3 us of tensor work.
 template <int EPI, int PBN, bool A_MN, bool B_MN, int ACT>
@@ -1261,6 +1262,11 @@ struct Gate {
   int64_t ldf = 0;
 };
 
+int current_sms() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
+}
+
 // Carves a workspace; with a null base it only counts.
 struct Carve {
   uint8_t* base;
@@ -1299,15 +1305,10 @@ struct Padder {
   }
   b2_status run(cudaStream_t st) {
     if (a.n == 0) return B2_OK;
-    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 7) / 8, 148 * 16));
+    const unsigned blocks = unsigned(std::min<long long>((a.begin[a.n] + 7) / 8, current_sms() * 16LL));
     return launch_chained(gated_pad_kernel, dim3(blocks), 256, 0, st, "gated pad launch", a);
   }
 };
-
-int current_sms() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 148;
-}
 
 b2_status launch_reduce_store(const ReduceArgs& r, int pbn, cudaStream_t st) {
   // Units of 8 columns where those of 32 would be fewer than 8 warps a SM (19
@@ -1316,7 +1317,7 @@ b2_status launch_reduce_store(const ReduceArgs& r, int pbn, cudaStream_t st) {
   const long long wide = (long long)(r.q.M + 31) / 32 * r.q.tiles_n * (pbn / 32);
   const bool narrow = wide < 8LL * current_sms();
   const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * (pbn / (narrow ? 8 : 32));
-  const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
+  const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, current_sms() * 16LL)));
   auto kern = pbn == 256 ? (narrow ? gated_reduce_store_kernel<256, 8> : gated_reduce_store_kernel<256, 32>)
                          : (narrow ? gated_reduce_store_kernel<128, 8> : gated_reduce_store_kernel<128, 32>);
   return launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r);
@@ -1423,7 +1424,7 @@ b2_status run_products(const Product* pr, int n, const Plan& plan, void* partial
         B2_TRY(launch_reduce_store(r, pbn, st));
     } else {
       const long long units = (long long)r.q.tiles_m * r.q.tiles_n * 8 * ((EPI == kGate ? pbn / 2 : pbn) / 8);
-      const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, 148 * 16)));
+      const dim3 blocks(unsigned(std::min<long long>((units + 7) / 8, current_sms() * 16LL)));
       auto kern = pbn == 256 ? gated_reduce_kernel<EPI, 256, ACT> : gated_reduce_kernel<EPI, 128, ACT>;
       B2_TRY(launch_chained(kern, blocks, 256, 0, st, "gated reduce launch", r));
     }
