@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a, int 
 // logits, not divided by tau, are finite where the logits are).
 //
 // 8192 rows of 131072 bf16 logits with 64 entries, a seventh of them masked:
-// 858 us with the gradient (5.0 TB/s of the 6.45 measured), 530 us the loss
+// 864 us with the gradient (4.6 TB/s of the 6.45 measured), 515 us the loss
 // alone; a row's 10 us in a CTA are 2.5 of copy, 2.5 of sums, 0.7 of reduction,
 // 1.6 of exchange, 2.1 of gradient and 0.9 of entries.  (One CTA of 16 warps a SM
 // with a ring of three slices took 1610 us: a row at a time leaves the SM waiting
@@ -1275,7 +1275,7 @@ b2_status launch_fwd(Args a, cudaStream_t st) {
   if (many && vecs * 16 <= kShortBytes) {
     // Many short rows: a CTA each, of half the threads, so that twice as many
     // rows overlap their latencies (8192 rows with the gradient: 2000 bf16 logits
-    // 50 us, with all threads 81, in the persistent kernel 76; 16000 logits 119,
+    // 50 us, with all threads 81, in the persistent kernel 76; 16000 logits 121,
     // 143 and 146; 24000 logits 173 and 185 in the persistent one, 2000 rows of
     // 32000 68 and 64; 500 rows of 2000 11.1 us against 10.7 with all threads).
     a.slice = a.tile = vecs;
@@ -1285,7 +1285,7 @@ b2_status launch_fwd(Args a, cudaStream_t st) {
     return launch_clusters(kern, a.N, 1, kShortThreads, size_t(vecs) * 16 + top, st, a, 1);
   }
   // Persistent clusters where every CTA gets at least two slices, else CTAs of a
-  // row's own (bf16, with the gradient): 8192 x 131072 858 us against 958; 300 x
+  // row's own (bf16, with the gradient): 8192 x 131072 864 us against 958; 300 x
   // 32000 18.4 against 17.1, 148 x 32000 13.3 against 12.5, where rows are too
   // few; the same at 1800 x 32000 (59).
   if (many && held <= kStreamSmem) {

@@ -65,9 +65,11 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     ``[E, F]`` (as ``nn.Linear`` keeps them), all bfloat16; the result is
     ``[..., E]``.  ``activation``: ``"silu"``, ``"gelu"`` (erf form) or
     ``"relu"``.  Sums are fp32; the hidden tensor is rounded to bfloat16
-    between the products, and the backward keeps it and the two factors
-    ``act(gate)`` and ``up * act'(gate)`` (16 bits of significand): eight bytes
-    a hidden element.  Inside ``torch.autocast("xdna")`` other
+    between the products (of up to four tokens whose rows, and those of
+    ``w_gate`` and ``w_up``, are 16-byte aligned, to two bfloat16 numbers), and
+    the backward keeps it and the two factors ``act(gate)`` and
+    ``up * act'(gate)`` (16 bits of significand): eight bytes a hidden element,
+    saved as autograd's tensors.  Inside ``torch.autocast("xdna")`` other
     floating-point arguments are cast first, as for a matrix product."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"gated_mlp: activation must be one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
