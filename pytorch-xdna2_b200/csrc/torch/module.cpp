@@ -417,7 +417,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("optimizer_step_boundary", [] { note_optimizer_step(); });
   m.def("as_cuda", [](const at::Tensor& t) {
     TORCH_CHECK(t.device().type() == kXdna, "as_cuda: expected an xdna tensor");
-    return to_cuda(t);
+    return cuda_view(t);
   });
   m.def("adopt", [](const at::Tensor& t) {
     TORCH_CHECK(t.device().type() == c10::DeviceType::CUDA, "adopt: expected a CUDA tensor");

@@ -37,6 +37,12 @@ namespace {
 
 void noop_delete(void*) {}
 
+struct ViewCtx {
+  c10::Storage xdna_storage;
+};
+
+void view_delete(void* ctx) { delete static_cast<ViewCtx*>(ctx); }
+
 struct AdoptCtx {
   c10::Storage cuda_storage;
 };
@@ -58,11 +64,11 @@ bool record_adopted(const c10::DataPtr& ptr, cudaStream_t s) {
   return true;
 }
 
-at::Tensor to_cuda_nosync(const at::Tensor& t) {
-  if (!t.defined() || t.device().type() != kXdna) return t;
+namespace {
+
+// t's memory, held by dp, as a CUDA tensor
+at::Tensor cuda_over(const at::Tensor& t, c10::DataPtr dp) {
   const c10::Storage& st = t.storage();
-  const c10::DeviceIndex dev = t.device().index();
-  c10::DataPtr dp(st.mutable_data(), st.mutable_data(), &noop_delete, c10::Device(c10::DeviceType::CUDA, dev));
   // Resizable through the CUDA allocator: an out= op that grows the alias gets
   // a new CUDA block, which the fallback then adopts back into the xdna tensor.
   c10::Storage cst(c10::Storage::use_byte_size_t(), st.nbytes(), std::move(dp),
@@ -73,6 +79,22 @@ at::Tensor to_cuda_nosync(const at::Tensor& t) {
   if (t.is_conj()) r._set_conj(true);
   if (t.is_neg()) r._set_neg(true);
   return r;
+}
+
+c10::Device cuda_of(const at::Tensor& t) { return c10::Device(c10::DeviceType::CUDA, t.device().index()); }
+
+}  // namespace
+
+at::Tensor to_cuda_nosync(const at::Tensor& t) {
+  if (!t.defined() || t.device().type() != kXdna) return t;
+  void* p = t.storage().mutable_data();
+  return cuda_over(t, c10::DataPtr(p, p, &noop_delete, cuda_of(t)));
+}
+
+at::Tensor cuda_view(const at::Tensor& t) {
+  materialize(t);
+  const c10::Storage& st = t.storage();
+  return cuda_over(t, c10::DataPtr(st.mutable_data(), new ViewCtx{st}, &view_delete, cuda_of(t)));
 }
 
 at::Tensor to_cuda(const at::Tensor& t) {

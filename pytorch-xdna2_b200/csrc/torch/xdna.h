@@ -65,6 +65,8 @@ at::Tensor to_cuda_nosync(const at::Tensor& t);
 // xdna tensor over the memory of a CUDA tensor (the xdna storage keeps the
 // CUDA storage alive).
 at::Tensor adopt(const at::Tensor& cuda_tensor);
+// as_cuda: a CUDA view (to_cuda's aliases are for the length of a call) that keeps the memory alive
+at::Tensor cuda_view(const at::Tensor& t);
 
 // ---- deferred weight gradients (deferred.cpp) -----------------------------
 // A job produces the contents of one storage.  Readers run it first; freeing

@@ -416,7 +416,8 @@ def materialize(tensor: torch.Tensor) -> None:
 
 
 def as_cuda(tensor: torch.Tensor) -> torch.Tensor:
-    """Zero-copy CUDA view of an xdna tensor (for NCCL collectives)."""
+    """Zero-copy CUDA view of an xdna tensor, whose memory it keeps alive (for NCCL
+    collectives, and for what CUDA code does with a result)."""
     register_xdna_device()
     return _C.as_cuda(tensor)
 

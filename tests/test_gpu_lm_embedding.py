@@ -195,3 +195,19 @@ def test_sums_of_whole_numbers_are_exact(dev, T, V, D, dtype, kind):
     keep = torch.ones(T, dtype=torch.bool) if pad is None else ids != pad
     ref = torch.zeros(V, D, dtype=torch.float64).index_add_(0, ids[keep], dy.double()[keep])
     assert torch.equal(dw.cpu(), ref.to(dtype))
+
+
+def test_cuda_views_of_results_keep_their_memory(dev):
+    # the way out of an operator: the view is all that is left of its result
+    want = torch.randn(64, 4096, generator=torch.Generator().manual_seed(7))
+    w, ids = want.to(dev), torch.arange(64).to(dev)
+    views = [xdna_train.as_cuda(lm.embedding(ids, w)) for _ in range(4)]
+    again = [lm.embedding(ids, w, scale=0.0) for _ in range(8)]   # would take the memory of results that are gone
+    assert all(torch.equal(v.cpu(), want) for v in views) and not any(a.cpu().any() for a in again)
+    part = xdna_train.as_cuda(lm.embedding(ids, w)[3:5, 7:])
+    back = xdna_train.as_xdna(xdna_train.as_cuda(lm.embedding(ids, w)))
+    again = [lm.embedding(ids, w, scale=0.0) for _ in range(8)]
+    assert torch.equal(part.cpu(), want[3:5, 7:]) and torch.equal(back.cpu(), want)
+    before = xdna_train.allocator_stats()["allocated_bytes"]
+    del views, part, back
+    assert xdna_train.allocator_stats()["allocated_bytes"] <= before - 6 * want.numel() * 4
